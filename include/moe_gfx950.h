@@ -352,6 +352,66 @@ int moe_blockwise_stages(const moe_bwmm_args* args, unsigned stages, void* strea
 size_t moe_kmajor_weights_bytes(const moe_bwmm_args* args, int which);
 int moe_prepare_kmajor_weights(const moe_bwmm_args* args, void* gate_up_kmajor, void* down_kmajor, void* stream);
 
+/* ---- tokens into block order and back, with gradients -------------------------------------- */
+
+/* No counterpart in the reference, whose kernels gather and scatter inside the layer (bwmm_shard_on_block.py:972-1038):
+ * for programs that multiply the experts themselves, and for the backward pass of a layer.  Slot s = 0 .. S-1 of the block
+ * table holds token token_position_to_id[s] (padding where that is outside [0, T): T, or -1 with skip_token) and belongs to
+ * expert block_to_expert[s / B].  dtype: MOE_DT_BF16 / FP16 / FP32 rows of H elements, contiguous, at any address that its
+ * element is aligned to.  Sums run over a token's slots in ascending order in fp32 and are rounded once.
+ *
+ * moe_token_slots: the table's inverse, int32 [T, 1 + top_k]: how many slots token t has, then the slots, ascending, then -1.
+ * top_k <= 64.  A token that the table lists more than top_k times keeps the true count: the calls below give NaN for it (its
+ * row, its slots' rows, its affinities).
+ *
+ * moe_permute_tokens: out[s] = x[token of s], zero rows for padding; any element type (rows of row_bytes bytes).
+ *
+ * moe_combine_tokens: out[t] = sum over t's slots s of expert_affinities[t, e(s)] * y[s]; affinities [T1 >= T, E] bf16 / fp32.
+ * Slots of blocks whose expert is outside [0, E) count for nothing and are not read; rows of padding slots are not read.  With
+ * expert_affinities and block_to_expert NULL every weight is 1: the backward pass of moe_permute_tokens.  S = N * B rows in y.
+ *
+ * moe_combine_tokens_bwd: d_y[s] = expert_affinities[t, e(s)] * d_out[t], zero rows for padding; d_affinities fp32 [T1, E] =
+ * sum over t's slots s of e of <d_out[t], y[s]>, zero elsewhere (fp32 whatever the affinities' type: a router's gradient is a
+ * difference of these). */
+int moe_token_slots(const int32_t* token_position_to_id, int64_t S, int64_t T, int top_k, int32_t* token_slots,
+                    void* stream);
+int moe_permute_tokens(const void* x, const int32_t* token_position_to_id, int64_t S, int64_t T, int64_t row_bytes,
+                       void* out, void* stream);
+int moe_combine_tokens(const void* y, int dtype, const void* expert_affinities, int aff_dtype, int64_t T1, int64_t E,
+                       const int32_t* block_to_expert, int64_t B, int64_t N, const int32_t* token_slots, int top_k,
+                       int64_t S, int64_t T, int64_t H, void* out, void* stream);
+int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtype, const void* expert_affinities, int aff_dtype,
+                           int64_t T1, int64_t E, const int32_t* token_position_to_id, const int32_t* block_to_expert,
+                           int64_t B, int64_t N, const int32_t* token_slots, int top_k, int64_t T, int64_t H, void* d_y,
+                           float* d_affinities, void* stream);
+
+/* ---- the gated activation with its inputs kept in 8 bits ------------------------------------ */
+
+/* No counterpart in the reference (its checkpoints are bf16, moe_cte.py:145-150).  A record of R rows of I gate and I up values:
+ * codes uint8 [R, 2, I] (OCP e4m3) and scales uint8 [R, 2, ceil(I/32)], one E8M0 byte per 32 neighbours; a value is
+ * code * 2^(byte - 127).  The scale is the smallest power of two with amax / scale <= 448 over the group's finite values;
+ * infinities and NaN are kept as NaN codes.  I <= 131072.  clamp_mask: MOE_CLAMP_*; clamps: host, gate upper, gate lower, up
+ * upper, up lower (NULL when clamp_mask is 0).  token_position_to_id int32 [R] (nullable): rows of padding slots (outside
+ * [0, n_tokens)) are not read, and zero in every output.
+ *
+ * moe_glu_checkpoint: gate_up [R, 2, I] -> intermediate [R, I] = act(gate) * up and the record of the clamped values.
+ * moe_pack_gate_up_checkpoint: the same record of what moe_blockwise left in gate_up_activations_T (bf16 [N, 2, I, B]; R = N*B).
+ * moe_glu_checkpoint_bwd: the record and d_intermediate [R, I] -> d_gate_up [R, 2, I] (zero where the recorded value lies at or
+ * beyond its clamp) and, unless NULL, intermediate [R, I] of the recorded values (what the down weights' gradient needs).
+ * moe_dequantize_checkpoint: `rows` rows of I codes with ceil(I/32) scales each -> values (bf16 holds them exactly, down to 2^-133). */
+int moe_glu_checkpoint(const void* gate_up, int dtype, int64_t R, int64_t I, int act_fn, int clamp_mask,
+                       const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens, void* intermediate,
+                       uint8_t* codes, uint8_t* scales, void* stream);
+int moe_pack_gate_up_checkpoint(const void* gate_up_activations_T, int64_t N, int64_t I, int64_t B,
+                                const int32_t* token_position_to_id, int64_t n_tokens, uint8_t* codes, uint8_t* scales,
+                                void* stream);
+int moe_glu_checkpoint_bwd(const uint8_t* codes, const uint8_t* scales, const void* d_intermediate, int dtype, int64_t R,
+                           int64_t I, int act_fn, int clamp_mask, const float* clamps,
+                           const int32_t* token_position_to_id, int64_t n_tokens, void* d_gate_up, void* intermediate,
+                           void* stream);
+int moe_dequantize_checkpoint(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t I, void* out, int dtype,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

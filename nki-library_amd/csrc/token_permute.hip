@@ -1,0 +1,396 @@
+// Tokens into the order of the block table and back, with their gradients.
+//
+//   permute           out[s] = x[id(s)]                           0 where slot s holds padding
+//   permute, backward dx[t]  = sum over the slots s of t of d[s]
+//   combine           out[t] = sum over the slots s of t of a[t, e(s)] y[s]
+//   combine, backward dy[s]  = a[t, e(s)] dout[t],  da[t, e] = sum over t's slots s of e of <dout[t], y[s]>
+//
+// id(s) = token_position_to_id[s], padding where it is no token; e(s) = block_to_expert[s / B].  All four move rows and
+// hardly compute: their bound is memory.  Sums run over the slots in ascending order in 32 bits and are rounded once, so
+// that a result depends on its inputs alone.  (The layer's own combine, combine.hip, adds in bf16 as the reference does.)
+//
+// Three of the four work by token: a token's row is read or written once whatever k is.  They go by a list of every token's
+// slots, which token_slots_kernel inverts the table into.
+#include <type_traits>
+
+#include "rows.hpp"
+
+namespace moe {
+
+constexpr int SLOTS_MAX_K = 64;        // most slots a list holds per token
+constexpr int SLOTS_LDS_WORDS = 12288;  // 48 KB of lists per workgroup
+
+// lists [T][1 + k]: how many slots the token has (more than k: the list is cut), its slots ascending, -1 behind them.
+// A workgroup owns `range` tokens and reads the whole table, which the L2 hands out: a table of 98 k slots is 0.4 MB, and
+// one launch without global atomics or cleared counters is shorter than the two that those would take.
+__global__ __launch_bounds__(1024) void token_slots_kernel(const int32_t* __restrict__ tp2id, int64_t S, int64_t T, int k,
+                                                           int range, int32_t* __restrict__ lists) {
+  __shared__ int s_list[SLOTS_LDS_WORDS];
+  const int64_t t0 = (int64_t)blockIdx.x * range;
+  const int nt = (int)(T - t0 < range ? T - t0 : range), w = 1 + k;
+  for (int i = threadIdx.x; i < nt; i += 1024) s_list[i * w] = 0;
+  __syncthreads();
+  auto take = [&](int64_t s, int id) {
+    const int64_t t = (int64_t)id - t0;
+    if (t >= 0 && t < nt) {
+      const int p = atomicAdd(&s_list[(int)t * w], 1);
+      if (p < k) s_list[(int)t * w + 1 + p] = (int)s;
+    }
+  };
+  const int64_t n4 = ((uintptr_t)tp2id & 15) == 0 ? S / 4 : 0;
+  constexpr int U = 4;
+  for (int64_t i0 = threadIdx.x; i0 < n4; i0 += 1024 * U) {
+    int4 d[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + 1024 * u < n4) d[u] = ((const int4*)tp2id)[i0 + 1024 * u];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + 1024 * u;
+      if (i < n4) {
+        take(4 * i, d[u].x);
+        take(4 * i + 1, d[u].y);
+        take(4 * i + 2, d[u].z);
+        take(4 * i + 3, d[u].w);
+      }
+    }
+  }
+  for (int64_t s = 4 * n4 + threadIdx.x; s < S; s += 1024) take(s, tp2id[s]);
+  __syncthreads();
+  // the slots were taken in any order: each goes to the place that its rank names
+  for (int i = threadIdx.x; i < nt * w; i += 1024) {
+    const int t = i / w, j = i - t * w, n = s_list[t * w], held = n < k ? n : k;
+    int32_t* out = lists + (t0 + t) * w;
+    if (j == 0) {
+      out[0] = n;
+    } else if (j > held) {
+      out[j] = -1;
+    } else {
+      const int mine = s_list[t * w + j];
+      int rank = 1;
+      for (int o = 1; o <= held; ++o) rank += s_list[t * w + o] < mine;
+      out[rank] = mine;
+    }
+  }
+}
+
+// ---- permute ----------------------------------------------------------------------------------------------------
+
+typedef uint32_t bytes16 __attribute__((ext_vector_type(4), aligned(1)));
+
+// TPR threads per slot (a whole number of waves, so that everything about a slot is uniform); rows of any number of bytes.
+template <int TPR>
+__device__ __forceinline__ int64_t row_of_group() {
+  return (int64_t)blockIdx.x * (256 / TPR) + __builtin_amdgcn_readfirstlane((int)(threadIdx.x / TPR));
+}
+template <int TPR>
+__global__ __launch_bounds__(256) void permute_kernel(const uint8_t* __restrict__ x, const int32_t* __restrict__ tp2id, int64_t S,
+                                                      int64_t T, int64_t row_bytes, uint8_t* __restrict__ out) {
+  const int lane = threadIdx.x % TPR;
+  const int64_t whole = row_bytes / 16;
+  for (int64_t s = row_of_group<TPR>(); s < S; s += (int64_t)gridDim.x * (256 / TPR)) {
+    const int64_t id = tp2id[s];
+    const bool token = id >= 0 && id < T;
+    const uint8_t* src = x + (token ? id : 0) * row_bytes;
+    uint8_t* dst = out + s * row_bytes;
+    for (int64_t c = lane; c < whole; c += TPR) {
+      bytes16 v = {0, 0, 0, 0};
+      if (token) v = *(const bytes16*)(src + 16 * c);
+      __builtin_nontemporal_store(v, (bytes16*)(dst + 16 * c));
+    }
+    for (int64_t b = 16 * whole + lane; b < row_bytes; b += TPR) dst[b] = token ? src[b] : (uint8_t)0;
+  }
+}
+
+// ---- combine, and the backward pass of permute --------------------------------------------------------------------
+
+struct SlotTables {
+  const int32_t* lists;  // [T][1 + k]
+  const int32_t* b2e;    // null: every weight is one
+  const void* aff;       // [>= T][E]
+  int aff_dtype, k;
+  uint32_t B, N;
+  int64_t E, S;          // S: rows of y
+};
+// Eight neighbours of a token's list: rows and weights.  A slot of a block without an expert counts for nothing and is
+// not read (row -1), nor is one that lies outside of y (a list made of another table).
+struct SlotGroup {
+  int64_t row[8];
+  float w[8];
+  int e[8];
+};
+__device__ __forceinline__ void load_group(const SlotTables& a, const int32_t* list, int64_t t, int j0, int n, SlotGroup& g) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    g.row[j] = j0 + j < n ? list[1 + j0 + j] : -1;
+    if (g.row[j] >= a.S) g.row[j] = -1;
+    g.w[j] = 1.f;
+    g.e[j] = 0;
+  }
+  if (!a.b2e) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (g.row[j] >= 0) {
+      const uint32_t b = (uint32_t)g.row[j] / a.B;
+      const int e = b < a.N ? a.b2e[b] : -1;
+      g.e[j] = e;
+      if (e < 0 || e >= a.E) g.row[j] = -1;
+      else g.w[j] = load_as_f32(a.aff, a.aff_dtype, t * a.E + e);
+    }
+}
+
+// TPR threads per token.
+template <int DT, int TPR>
+__global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __restrict__ y, const SlotTables a, int64_t T,
+                                                             int64_t H, uint8_t* __restrict__ out) {
+  typedef Elem<DT> EL;
+  typedef typename EL::raw raw;
+  constexpr int N = EL::N;
+  const int lane = threadIdx.x % TPR;
+  const int64_t whole = H / N * N;
+  for (int64_t t = row_of_group<TPR>(); t < T; t += (int64_t)gridDim.x * (256 / TPR)) {
+    const int32_t* list = a.lists + t * (1 + a.k);
+    const bool cut = list[0] > a.k;  // the table lists the token more often than its caller said: no sum of a part
+    const int n = cut ? 0 : list[0];
+    const float start = cut ? __builtin_nanf("") : 0.f;
+    SlotGroup g;
+    load_group(a, list, t, 0, n, g);
+    for (int64_t c = (int64_t)lane * N; c < whole; c += TPR * N) {
+      float acc[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = start;
+      for (int j0 = 0; j0 < n; j0 += 8) {
+        if (n > 8) load_group(a, list, t, j0, n, g);
+        u32x4 d[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (g.row[j] >= 0) d[j] = load_piece<DT>(y + (g.row[j] * H + c) * EL::SIZE);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (g.row[j] >= 0) {
+            float v[N];
+            unpack<DT>(d[j], v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] = fmaf(g.w[j], v[i], acc[i]);
+          }
+      }
+      store_piece<DT>(out + (t * H + c) * EL::SIZE, pack<DT>(acc));
+    }
+    for (int64_t c = whole + lane; c < H; c += TPR) {
+      float acc = start;
+      for (int j0 = 0; j0 < n; j0 += 8) {
+        if (n > 8) load_group(a, list, t, j0, n, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (g.row[j] >= 0) acc = fmaf(g.w[j], elem_to_f32<DT>(((const raw*)y)[g.row[j] * H + c]), acc);
+      }
+      ((raw*)out)[t * H + c] = f32_to_elem<DT>(acc);
+    }
+  }
+}
+
+// ---- combine, backward --------------------------------------------------------------------------------------------
+
+// Jobs [0, T) take a token each: its row of dout is read once per eight slots, eight rows of y and dy beside it.  The next
+// ceil(S / PAD_SLOTS) write the rows of slots that no token's list holds, the last one the rows of da behind T.
+constexpr int PAD_SLOTS = 64;
+template <int DT>
+__global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* __restrict__ dout, const uint8_t* __restrict__ y,
+                                                                 const SlotTables a, const int32_t* __restrict__ tp2id,
+                                                                 int64_t S, int64_t T, int64_t T1, int64_t H,
+                                                                 uint8_t* __restrict__ dy, float* __restrict__ daff) {
+  typedef Elem<DT> EL;
+  typedef typename EL::raw raw;
+  constexpr int N = EL::N;
+  __shared__ float s_part[4][8], s_dot[SLOTS_MAX_K];
+  __shared__ int s_e[SLOTS_MAX_K];
+  const int tid = threadIdx.x;
+  const int64_t whole = H / N * N, n_pad = (S + PAD_SLOTS - 1) / PAD_SLOTS;
+  for (int64_t job = blockIdx.x; job < T + n_pad + 1; job += gridDim.x) {
+    if (job == T + n_pad) {
+      for (int64_t i = T * a.E + tid; i < T1 * a.E; i += 256) daff[i] = 0.f;
+      continue;
+    }
+    if (job >= T) {
+      const int64_t s0 = (job - T) * PAD_SLOTS, s1 = s0 + PAD_SLOTS < S ? s0 + PAD_SLOTS : S;
+      for (int64_t s = s0; s < s1; ++s) {
+        const int64_t id = tp2id[s];
+        const int e = a.b2e[(uint32_t)s / a.B];
+        const bool token = id >= 0 && id < T && e >= 0 && e < a.E;
+        const bool cut = token && a.lists[id * (1 + a.k)] > a.k;
+        if (token && !cut) continue;
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = cut ? __builtin_nanf("") : 0.f;
+        for (int64_t c = (int64_t)tid * N; c < whole; c += 256 * N) store_piece<DT>(dy + (s * H + c) * EL::SIZE, pack<DT>(v));
+        for (int64_t c = whole + tid; c < H; c += 256) ((raw*)dy)[s * H + c] = f32_to_elem<DT>(v[0]);
+      }
+      continue;
+    }
+    const int64_t t = job;
+    const int32_t* list = a.lists + t * (1 + a.k);
+    const int n = list[0];
+    if (n > a.k) {
+      for (int64_t e = tid; e < a.E; e += 256) daff[t * a.E + e] = __builtin_nanf("");
+      continue;
+    }
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      SlotGroup g;
+      load_group(a, list, t, j0, n, g);
+      float dot[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot[j] = 0.f;
+      for (int64_t c = (int64_t)tid * N; c < whole; c += 256 * N) {
+        u32x4 d[8];
+        const u32x4 dg = load_piece_kept<DT>(dout + (t * H + c) * EL::SIZE);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (g.row[j] >= 0) d[j] = load_piece<DT>(y + (g.row[j] * H + c) * EL::SIZE);
+        float gv[N];
+        unpack<DT>(dg, gv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (g.row[j] >= 0) {
+            float v[N];
+            unpack<DT>(d[j], v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              dot[j] = fmaf(gv[i], v[i], dot[j]);
+              v[i] = g.w[j] * gv[i];
+            }
+            store_piece<DT>(dy + (g.row[j] * H + c) * EL::SIZE, pack<DT>(v));
+          }
+      }
+      for (int64_t c = whole + tid; c < H; c += 256) {
+        const float gv = elem_to_f32<DT>(((const raw*)dout)[t * H + c]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (g.row[j] >= 0) {
+            dot[j] = fmaf(gv, elem_to_f32<DT>(((const raw*)y)[g.row[j] * H + c]), dot[j]);
+            ((raw*)dy)[g.row[j] * H + c] = f32_to_elem<DT>(g.w[j] * gv);
+          }
+      }
+      __syncthreads();  // (the sums of the group before, and of the token before, have been read)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = wave_sum(dot[j]);
+        if ((tid & 63) == 0) s_part[tid >> 6][j] = v;
+        if (tid == 0 && j0 + j < n) s_e[j0 + j] = g.row[j] >= 0 ? g.e[j] : -1;
+      }
+      __syncthreads();
+      if (tid < 8 && j0 + tid < n) s_dot[j0 + tid] = (s_part[0][tid] + s_part[1][tid]) + (s_part[2][tid] + s_part[3][tid]);
+    }
+    __syncthreads();
+    for (int64_t e = tid; e < a.E; e += 256) {
+      float v = 0.f;
+      for (int j = 0; j < n; ++j)
+        if (s_e[j] == e) v += s_dot[j];
+      daff[t * a.E + e] = v;
+    }
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------
+
+// (a launch holds fewer than 2^32 threads; what lies beyond a million workgroups is a second round of the same ones)
+static unsigned grid_of(int64_t jobs) { return (unsigned)(jobs < ((int64_t)1 << 20) ? jobs : (int64_t)1 << 20); }
+static int check_tables(const SlotTables& a, int64_t T, int64_t T1) {
+  if (!a.b2e) return MOE_OK;
+  if (!a.aff || (a.aff_dtype != MOE_DT_BF16 && a.aff_dtype != MOE_DT_FP32)) return MOE_E_BAD_ARG;
+  if (a.E <= 0 || a.E >= (int64_t)1 << 31 || T1 < T) return MOE_E_BAD_SHAPE;
+  return MOE_OK;
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" int moe_token_slots(const int32_t* token_position_to_id, int64_t S, int64_t T, int top_k, int32_t* token_slots,
+                               void* stream) {
+  if ((!token_position_to_id && S > 0) || !token_slots || S < 0 || T < 0) return MOE_E_BAD_ARG;
+  if (top_k < 1 || top_k > SLOTS_MAX_K || S >= (int64_t)1 << 31 || T >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
+  if (T == 0) return MOE_OK;
+  const int most = SLOTS_LDS_WORDS / (1 + top_k);
+  int64_t range = (T + 255) / 256;  // a workgroup per CU
+  if (range > most) range = most;
+  hipLaunchKernelGGL(token_slots_kernel, dim3((unsigned)((T + range - 1) / range)), dim3(1024), 0, (hipStream_t)stream,
+                     token_position_to_id, S, T, top_k, (int)range, token_slots);
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
+extern "C" int moe_permute_tokens(const void* x, const int32_t* token_position_to_id, int64_t S, int64_t T, int64_t row_bytes,
+                                  void* out, void* stream) {
+  if (!x || !token_position_to_id || !out || S < 0 || T < 0 || row_bytes < 0) return MOE_E_BAD_ARG;
+  if (S >= (int64_t)1 << 31 || T >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
+  if (S == 0 || row_bytes == 0) return MOE_OK;
+  const hipStream_t s = (hipStream_t)stream;
+  if (row_bytes > 2048)
+    hipLaunchKernelGGL(permute_kernel<256>, dim3(grid_of(S)), dim3(256), 0, s, (const uint8_t*)x, token_position_to_id, S, T,
+                       row_bytes, (uint8_t*)out);
+  else
+    hipLaunchKernelGGL(permute_kernel<64>, dim3(grid_of((S + 3) / 4)), dim3(256), 0, s, (const uint8_t*)x,
+                       token_position_to_id, S, T, row_bytes, (uint8_t*)out);
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
+template <int DT>
+static void launch_combine_tokens(const void* y, const SlotTables& a, int64_t T, int64_t H, void* out, hipStream_t s) {
+  if (H * Elem<DT>::SIZE > 2048)
+    hipLaunchKernelGGL((combine_tokens_kernel<DT, 256>), dim3(grid_of(T)), dim3(256), 0, s, (const uint8_t*)y, a, T, H,
+                       (uint8_t*)out);
+  else
+    hipLaunchKernelGGL((combine_tokens_kernel<DT, 64>), dim3(grid_of((T + 3) / 4)), dim3(256), 0, s, (const uint8_t*)y, a, T,
+                       H, (uint8_t*)out);
+}
+
+extern "C" int moe_combine_tokens(const void* y, int dtype, const void* expert_affinities, int aff_dtype, int64_t T1, int64_t E,
+                                  const int32_t* block_to_expert, int64_t B, int64_t N, const int32_t* token_slots, int top_k,
+                                  int64_t S, int64_t T, int64_t H, void* out, void* stream) {
+  if (!y || !token_slots || !out || S < 0 || T < 0 || H < 0) return MOE_E_BAD_ARG;
+  if ((expert_affinities != nullptr) != (block_to_expert != nullptr)) return MOE_E_BAD_ARG;
+  if (top_k < 1 || top_k > SLOTS_MAX_K || T >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
+  if (S >= (int64_t)1 << 31 || (block_to_expert && (B <= 0 || N < 0 || S != B * N))) return MOE_E_BAD_SHAPE;
+  const SlotTables a{token_slots, block_to_expert, expert_affinities, aff_dtype, top_k, (uint32_t)B, (uint32_t)N, E, S};
+  const int rc = check_tables(a, T, T1);
+  if (rc != MOE_OK) return rc;
+  if (T == 0 || H == 0) return MOE_OK;
+  const hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case MOE_DT_BF16: launch_combine_tokens<MOE_DT_BF16>(y, a, T, H, out, s); break;
+    case MOE_DT_FP16: launch_combine_tokens<MOE_DT_FP16>(y, a, T, H, out, s); break;
+    case MOE_DT_FP32: launch_combine_tokens<MOE_DT_FP32>(y, a, T, H, out, s); break;
+    default: return MOE_E_BAD_ARG;
+  }
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
+extern "C" int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtype, const void* expert_affinities, int aff_dtype,
+                                      int64_t T1, int64_t E, const int32_t* token_position_to_id, const int32_t* block_to_expert,
+                                      int64_t B, int64_t N, const int32_t* token_slots, int top_k, int64_t T, int64_t H,
+                                      void* d_y, float* d_affinities, void* stream) {
+  if (!d_out || !y || !expert_affinities || !token_position_to_id || !block_to_expert || !token_slots || !d_y ||
+      !d_affinities || T < 0 || H < 0 || N < 0)
+    return MOE_E_BAD_ARG;
+  if (top_k < 1 || top_k > SLOTS_MAX_K || T >= (int64_t)1 << 31 || B <= 0 || B * N >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
+  const int64_t S = B * N;
+  const SlotTables a{token_slots, block_to_expert, expert_affinities, aff_dtype, top_k, (uint32_t)B, (uint32_t)N, E, S};
+  const int rc = check_tables(a, T, T1);
+  if (rc != MOE_OK) return rc;
+  const unsigned grid = grid_of(T + (S + PAD_SLOTS - 1) / PAD_SLOTS + 1);
+  const hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+#define MOE_BWD(DT)                                                                                                           \
+  hipLaunchKernelGGL(combine_tokens_bwd_kernel<DT>, dim3(grid), dim3(256), 0, s, (const uint8_t*)d_out,               \
+                     (const uint8_t*)y, a, token_position_to_id, S, T, T1, H, (uint8_t*)d_y, d_affinities)
+    case MOE_DT_BF16: MOE_BWD(MOE_DT_BF16); break;
+    case MOE_DT_FP16: MOE_BWD(MOE_DT_FP16); break;
+    case MOE_DT_FP32: MOE_BWD(MOE_DT_FP32); break;
+#undef MOE_BWD
+    default: return MOE_E_BAD_ARG;
+  }
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}

@@ -50,6 +50,14 @@ EXPORTED_SYMBOLS = (
     "moe_blockwise_stages",
     "moe_kmajor_weights_bytes",
     "moe_prepare_kmajor_weights",
+    "moe_token_slots",
+    "moe_permute_tokens",
+    "moe_combine_tokens",
+    "moe_combine_tokens_bwd",
+    "moe_glu_checkpoint",
+    "moe_pack_gate_up_checkpoint",
+    "moe_glu_checkpoint_bwd",
+    "moe_dequantize_checkpoint",
 )
 
 
@@ -182,6 +190,23 @@ def lib():
     L.moe_prepare_kmajor_weights.argtypes = [POINTER(BwmmArgs), c_void_p, c_void_p, c_void_p]
     L.moe_blockwise_stages.restype = c_int
     L.moe_blockwise_stages.argtypes = [POINTER(BwmmArgs), ctypes.c_uint, c_void_p]
+    for name, args in {
+        "moe_token_slots": [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p],
+        "moe_permute_tokens": [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p],
+        "moe_combine_tokens": [c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                               c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p],
+        "moe_combine_tokens_bwd": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p,
+                                   c_int64, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+        "moe_glu_checkpoint": [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p,
+                               c_void_p, c_void_p, c_void_p],
+        "moe_pack_gate_up_checkpoint": [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                        c_void_p],
+        "moe_glu_checkpoint_bwd": [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p,
+                                   c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
+        "moe_dequantize_checkpoint": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p],
+    }.items():
+        getattr(L, name).restype = c_int
+        getattr(L, name).argtypes = args
     _lib = L
     return L
 

@@ -1,0 +1,108 @@
+"""What the training operators refuse, through the C ABI: checked before anything is launched, so no GPU is needed."""
+
+import ctypes
+
+import pytest
+
+BAD_ARG, BAD_SHAPE = -1, -2
+P = ctypes.c_void_p(4096)  # (never dereferenced)
+
+
+@pytest.fixture
+def L():
+    from nkilib import _native as nv
+
+    return nv.lib()
+
+
+def test_token_slots_refusals(L):
+    assert L.moe_token_slots(None, 4, 4, 2, P, None) == BAD_ARG
+    assert L.moe_token_slots(P, 4, 4, 2, None, None) == BAD_ARG
+    assert L.moe_token_slots(P, -1, 4, 2, P, None) == BAD_ARG
+    for k in (0, 65):
+        assert L.moe_token_slots(P, 4, 4, k, P, None) == BAD_SHAPE
+    assert L.moe_token_slots(P, 2**31, 4, 2, P, None) == BAD_SHAPE
+    assert L.moe_token_slots(P, 4, 2**31, 2, P, None) == BAD_SHAPE
+    assert L.moe_token_slots(P, 4, 0, 2, P, None) == 0  # no tokens: nothing to write
+
+
+def test_permute_refusals(L):
+    assert L.moe_permute_tokens(None, P, 4, 4, 16, P, None) == BAD_ARG
+    assert L.moe_permute_tokens(P, P, 4, 4, -1, P, None) == BAD_ARG
+    assert L.moe_permute_tokens(P, P, 2**31, 4, 16, P, None) == BAD_SHAPE
+    assert L.moe_permute_tokens(P, P, 0, 4, 16, P, None) == 0
+    assert L.moe_permute_tokens(P, P, 4, 4, 0, P, None) == 0
+
+
+def _combine(L, **kw):
+    a = dict(y=P, dtype=0, aff=P, aff_dtype=0, T1=5, E=3, b2e=P, B=4, N=2, slots=P, k=2, S=8, T=0, H=16, out=P)
+    a.update(kw)
+    return L.moe_combine_tokens(a["y"], a["dtype"], a["aff"], a["aff_dtype"], a["T1"], a["E"], a["b2e"], a["B"], a["N"],
+                                a["slots"], a["k"], a["S"], a["T"], a["H"], a["out"], None)
+
+
+def test_combine_refusals(L):
+    assert _combine(L) == 0  # (no tokens)
+    assert _combine(L, T=4, dtype=7) == BAD_ARG and _combine(L, T=4, dtype=3) == BAD_ARG
+    assert _combine(L, aff=None) == BAD_ARG and _combine(L, b2e=None) == BAD_ARG
+    assert _combine(L, slots=None) == BAD_ARG and _combine(L, y=None) == BAD_ARG and _combine(L, out=None) == BAD_ARG
+    assert _combine(L, aff_dtype=1) == BAD_ARG  # fp16 affinities
+    assert _combine(L, T=6) == BAD_SHAPE  # fewer rows of affinities than tokens
+    assert _combine(L, E=0) == BAD_SHAPE
+    assert _combine(L, k=0) == BAD_SHAPE and _combine(L, k=65) == BAD_SHAPE
+    assert _combine(L, B=0) == BAD_SHAPE and _combine(L, S=9) == BAD_SHAPE and _combine(L, S=2**31, B=2**30) == BAD_SHAPE
+
+
+def test_combine_bwd_refusals(L):
+    def call(**kw):
+        a = dict(d=P, y=P, dtype=0, aff=P, aff_dtype=0, T1=5, E=3, tp=P, b2e=P, B=4, N=2, slots=P, k=2, T=4, H=16, dy=P, da=P)
+        a.update(kw)
+        return L.moe_combine_tokens_bwd(a["d"], a["y"], a["dtype"], a["aff"], a["aff_dtype"], a["T1"], a["E"], a["tp"],
+                                        a["b2e"], a["B"], a["N"], a["slots"], a["k"], a["T"], a["H"], a["dy"], a["da"], None)
+
+    for name in ("d", "y", "aff", "tp", "b2e", "slots", "dy", "da"):
+        assert call(**{name: None}) == BAD_ARG, name
+    assert call(dtype=6) == BAD_ARG and call(aff_dtype=1) == BAD_ARG and call(H=-1) == BAD_ARG
+    assert call(T=6) == BAD_SHAPE and call(k=65) == BAD_SHAPE and call(B=0) == BAD_SHAPE and call(B=2**30, N=2) == BAD_SHAPE
+
+
+def test_glu_refusals(L):
+    f = (ctypes.c_float * 4)()
+
+    def fwd(x=P, dtype=0, R=4, I=64, act=0, mask=0, clamps=None, n=0, h=P, c=P, s=P):
+        return L.moe_glu_checkpoint(x, dtype, R, I, act, mask, clamps, None, n, h, c, s, None)
+
+    def bwd(c=P, s=P, d=P, dtype=0, R=4, I=64, act=0, mask=0, clamps=None, dgu=P):
+        return L.moe_glu_checkpoint_bwd(c, s, d, dtype, R, I, act, mask, clamps, None, 0, dgu, None, None)
+
+    assert fwd(R=0) == 0 and bwd(R=0) == 0
+    assert fwd(x=None) == BAD_ARG and fwd(h=None) == BAD_ARG and fwd(c=None) == BAD_ARG and fwd(s=None) == BAD_ARG
+    assert bwd(c=None) == BAD_ARG and bwd(d=None) == BAD_ARG and bwd(dgu=None) == BAD_ARG
+    for call in (fwd, bwd):
+        assert call(dtype=3) == BAD_ARG and call(act=4) == BAD_ARG and call(act=-1) == BAD_ARG
+        assert call(I=0) == BAD_ARG and call(R=-1) == BAD_ARG
+        assert call(mask=16, clamps=f) == BAD_ARG and call(mask=1) == BAD_ARG
+        assert call(I=2**17 + 1) == BAD_SHAPE and call(R=2**31) == BAD_SHAPE
+    pack = lambda x=P, N=2, I=64, B=4: L.moe_pack_gate_up_checkpoint(x, N, I, B, None, 0, P, P, None)
+    assert pack(N=0) == 0
+    assert pack(x=None) == BAD_ARG and pack(B=0) == BAD_ARG and pack(I=0) == BAD_ARG
+    assert pack(I=2**17 + 1) == BAD_SHAPE and pack(N=2**29) == BAD_SHAPE
+    assert L.moe_dequantize_checkpoint(P, P, 2, 64, P, 3, None) == BAD_ARG
+    assert L.moe_dequantize_checkpoint(P, None, 2, 64, P, 0, None) == BAD_ARG
+    assert L.moe_dequantize_checkpoint(P, P, 0, 64, P, 0, None) == 0
+
+
+def test_host_tensors_are_refused():
+    """There is no CPU path: the operators say so."""
+    import torch
+    from nkilib._native import NativeLibraryError
+    from nkilib.core.moe.glu_checkpoint import glu_checkpoint, glu_checkpoint_bwd, pack_gate_up_checkpoint
+    from nkilib.core.moe.token_permute import build_token_slots, combine_tokens, permute_tokens
+
+    x, t = torch.zeros(4, 8), torch.zeros(8, dtype=torch.int32)
+    u8 = torch.zeros(4, 2, 8, dtype=torch.uint8)
+    for call in (lambda: permute_tokens(x, t), lambda: build_token_slots(t, 4, 2), lambda: combine_tokens(x, x, t, t, 1, 4, 2),
+                 lambda: glu_checkpoint(x.view(2, 2, 8)), lambda: glu_checkpoint_bwd(u8, u8, x),
+                 lambda: pack_gate_up_checkpoint(x.view(1, 2, 2, 8).bfloat16())):
+        with pytest.raises(NativeLibraryError, match="no CPU path"):
+            call()
