@@ -119,6 +119,20 @@ int moe_router_topk(const void* x, const void* w, const void* w_bias, int bias_d
                     void* expert_affinities, int aff_dtype, float* topk_affinities, void* workspace,
                     size_t workspace_bytes, void* stream);
 
+/* The gradient of moe_router_topk.  No counterpart in the reference.  d_affinities [>= T, E] bf16 / fp32 (moe_combine_tokens_bwd's
+ * d_affinities; rows from T on are not read), x / w as in the forward call, router_logits [T, E] bf16 / fp32 and expert_index
+ * [T, k] as it returned them (an index outside [0, E) counts for nothing, one named twice counts once), the same act_fn,
+ * router_pre_norm and norm_topk_prob.  mask_to_topk != 0, router_pre_norm == 0 or norm_topk_prob: the gradients of
+ * unselected experts are not read.  mask_to_topk == 0 otherwise: the full table was handed out, and all are.
+ * Writes d_x bf16 [T, H], d_w bf16 [H, E] and, unless NULL, d_bias [E] (bias_dtype bf16 / fp32).  The gradient of the logits is
+ * fp32; in the two products it is the sum of two bf16 (2^-17), summed in fp32.  k <= 8, E <= 512, H % 128 == 0, H <= 2^20,
+ * 1 <= T <= 2^26.  workspace: moe_router_topk_bwd_workspace_bytes(T, H, E) bytes, 16-byte aligned. */
+size_t moe_router_topk_bwd_workspace_bytes(int64_t T, int64_t H, int64_t E);
+int moe_router_topk_bwd(const void* d_affinities, int aff_dtype, const void* x, const void* w, const void* router_logits,
+                        int logits_dtype, const int32_t* expert_index, int64_t T, int64_t H, int64_t E, int k, int act_fn,
+                        int router_pre_norm, int norm_topk_prob, int mask_to_topk, void* d_x, void* d_w, void* d_bias,
+                        int bias_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- token -> block index construction ---------------------------------------------- */
 
 /* Device version of generate_token_position_to_id_and_experts

@@ -21,7 +21,7 @@ OBJ_DIR = os.path.join(HERE, "build")
 OUT_DIR = os.path.join(HERE, "nkilib", "_lib")
 OUT = os.path.join(OUT_DIR, "libmoe_gfx950.so")
 SOURCES = ["rmsnorm_quant.hip", "build_blocks.hip", "combine.hip", "bwmm.hip", "bwmm_mx.hip", "bwmm_rows.hip", "router_topk.hip", "index_ops.hip", "token_permute.hip",
-           "glu_checkpoint.hip", "capi.hip"]
+           "glu_checkpoint.hip", "router_bwd.hip", "capi.hip"]
 # (stage, weight format, K that ends inside a slice) instances of the large-tile MX GEMM; formats as MX_WFMT_* in csrc/bwmm.hpp
 MX_INSTANCES = [(1, 4, 0), (1, 3, 0), (1, 0, 0), (1, 1, 0), (1, 2, 0), (2, 4, 0), (2, 3, 0), (2, 0, 0), (2, 1, 0), (2, 2, 0),
                 (2, 0, 1), (2, 1, 1), (2, 2, 1)]

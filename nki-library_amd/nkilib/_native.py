@@ -58,6 +58,8 @@ EXPORTED_SYMBOLS = (
     "moe_pack_gate_up_checkpoint",
     "moe_glu_checkpoint_bwd",
     "moe_dequantize_checkpoint",
+    "moe_router_topk_bwd_workspace_bytes",
+    "moe_router_topk_bwd",
 )
 
 
@@ -204,9 +206,13 @@ def lib():
         "moe_glu_checkpoint_bwd": [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p,
                                    c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
         "moe_dequantize_checkpoint": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p],
+        "moe_router_topk_bwd": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int,
+                                c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p],
     }.items():
         getattr(L, name).restype = c_int
         getattr(L, name).argtypes = args
+    L.moe_router_topk_bwd_workspace_bytes.restype = c_size_t
+    L.moe_router_topk_bwd_workspace_bytes.argtypes = [c_int64, c_int64, c_int64]
     _lib = L
     return L
 

@@ -83,12 +83,14 @@ def _router_topk(x, w, w_bias, router_logits, expert_affinities, expert_index, a
 router_topk = KernelEntry(_router_topk)
 
 
-def route_for_moe(x, w, w_bias, k, act_fn=RouterActFnType.SOFTMAX, norm_topk_prob=False):
+def route_for_moe(x, w, w_bias, k, act_fn=RouterActFnType.SOFTMAX, norm_topk_prob=False, return_router_logits=False):
     """Hidden states ``[T+1, H]`` (last row = the padding token, as ``moe_cte`` takes them) -> what ``moe_cte`` and
     ``build_token_blocks`` consume: top-k ids ``[T, k]`` int32 and the masked affinity table ``[T+1, E]`` bf16
-    (zero outside the top-k, zero padding row)."""
+    (zero outside the top-k, zero padding row).  With ``return_router_logits`` also the logits ``[T, E]`` in float32, which
+    ``router_topk_bwd`` takes."""
     T = x.shape[0] - 1
-    _, idx, aff = _router_topk(x[:T], w, w_bias, None, None, None, act_fn, k, x_hbm_layout=1, router_pre_norm=True,
-                               norm_topk_prob=norm_topk_prob, skip_store_router_logits=True, _mask_to_topk=True,
-                               _pad_row=True)
-    return idx, aff
+    logits = torch.empty((T, w.shape[1]), dtype=torch.float32, device=x.device) if return_router_logits else None
+    _, idx, aff = _router_topk(x[:T], w, w_bias, logits, None, None, act_fn, k, x_hbm_layout=1, router_pre_norm=True,
+                               norm_topk_prob=norm_topk_prob, skip_store_router_logits=not return_router_logits,
+                               _mask_to_topk=True, _pad_row=True)
+    return (idx, aff, logits) if return_router_logits else (idx, aff)

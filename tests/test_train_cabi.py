@@ -106,3 +106,23 @@ def test_host_tensors_are_refused():
                  lambda: pack_gate_up_checkpoint(x.view(1, 2, 2, 8).bfloat16())):
         with pytest.raises(NativeLibraryError, match="no CPU path"):
             call()
+
+
+def test_router_bwd_refusals(L):
+    ws = L.moe_router_topk_bwd_workspace_bytes
+    need = ws(64, 256, 8)
+    assert need > 0 and ws(0, 256, 8) == 0 and ws(64, 200, 8) == 0 and ws(64, 256, 513) == 0 and ws(2**26 + 1, 128, 8) == 0
+
+    def call(**kw):
+        a = dict(g=P, gd=2, x=P, w=P, l=P, ld=2, ids=P, T=64, H=256, E=8, k=2, act=1, pre=1, norm=0, mask=1, dx=P, dw=P, db=None, bd=2,
+                 ws=P, n=need)
+        a.update(kw)
+        return L.moe_router_topk_bwd(a["g"], a["gd"], a["x"], a["w"], a["l"], a["ld"], a["ids"], a["T"], a["H"], a["E"], a["k"],
+                                     a["act"], a["pre"], a["norm"], a["mask"], a["dx"], a["dw"], a["db"], a["bd"], a["ws"], a["n"], None)
+
+    for name in ("g", "x", "w", "l", "ids", "dx", "dw"):
+        assert call(**{name: None}) == BAD_ARG, name
+    assert call(gd=1) == BAD_ARG and call(ld=3) == BAD_ARG and call(act=2) == BAD_ARG and call(db=P, bd=1) == BAD_ARG
+    assert call(T=0) == BAD_ARG and call(H=192) == BAD_SHAPE and call(E=513) == BAD_SHAPE and call(k=0) == BAD_SHAPE
+    assert call(k=9) == BAD_SHAPE and call(E=4, k=5) == BAD_SHAPE
+    assert call(ws=None) == -3 and call(n=need - 1) == -3 and call(ws=ctypes.c_void_p(4100)) == BAD_ARG
