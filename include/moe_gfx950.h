@@ -126,7 +126,7 @@ int moe_router_topk(const void* x, const void* w, const void* w_bias, int bias_d
  * unselected experts are not read.  mask_to_topk == 0 otherwise: the full table was handed out, and all are.
  * Writes d_x bf16 [T, H], d_w bf16 [H, E] and, unless NULL, d_bias [E] (bias_dtype bf16 / fp32).  The gradient of the logits is
  * fp32; in the two products it is the sum of two bf16 (2^-17), summed in fp32.  k <= 8, E <= 512, H % 128 == 0, H <= 2^20,
- * 1 <= T <= 2^26.  workspace: moe_router_topk_bwd_workspace_bytes(T, H, E) bytes, 16-byte aligned. */
+ * 1 <= T <= 2^26.  workspace: moe_router_topk_bwd_workspace_bytes(T, H, E) bytes.  x, d_x and workspace 16-byte aligned. */
 size_t moe_router_topk_bwd_workspace_bytes(int64_t T, int64_t H, int64_t E);
 int moe_router_topk_bwd(const void* d_affinities, int aff_dtype, const void* x, const void* w, const void* router_logits,
                         int logits_dtype, const int32_t* expert_index, int64_t T, int64_t H, int64_t E, int k, int act_fn,

@@ -7,17 +7,19 @@
 //   sigmoid, divided by the chosen's sum S        dl_j = (g_j - sum g a) / S  s_j (1 - s_j),  a_j = s_j / S
 //   dx = dl w^T    dw = x^T dl    db = sum over the tokens of dl
 //
-// Everything up to dl is fp32.  The two products run on bf16 MFMAs with dl as the sum of two bf16 (hi + lo, 2^-17 of the value): a
-// softmax's dl sum to zero over the experts, and a single bf16 (2^-8) would leave that much of every term where the terms
-// cancel.  x and w are bf16 as they are.  Sums are fp32; splits of the token axis are added in a fixed order.
+// Everything up to dl is fp32.  A token has k of them at most, but for the softmax over all experts ("dense").  dw runs on bf16
+// MFMAs with dl as the sum of two bf16 (hi + lo, 2^-17 of the value): a single bf16 (2^-8) would double the error of a result
+// that is rounded to bf16 itself, and leave more than that where terms cancel over the tokens.  dx of k experts is k
+// multiply-adds per value, in fp32 from a slice of w in LDS; dense, it runs on MFMAs like dw (there a single bf16 would leave
+// 2^-8 of every term of sums that vanish by construction: dl add up to zero over the experts).  x and w are bf16 as they are.
+// Sums are fp32; parts of the token axis are added in a fixed order.
 //
 // Three launches:
-//   1. router_dlogits_kernel  a workgroup takes 32 tokens: dl in LDS, then hi / lo fragments of 16 bytes per lane in the order
-//                             in which either product reads them, and the tokens' part of db; further workgroups bring w into
-//                             fragment order (w is a few MB, any E, padded with zeros to the K of an MFMA);
-//   2. router_grad_kernel     jobs of dw, then jobs of dx, in one launch: the one reads the tokens and the other writes
-//                             their gradients, and neither waits for the other;
-//   3. router_reduce_kernel   adds up the parts of dw and of db.
+//   1. router_dlogits_kernel   a workgroup takes 32 tokens: dl in LDS, then hi / lo fragments of 16 bytes per lane in the order in
+//                              which the products read them, each token's list of (expert, dl), and the tokens' part of db;
+//                              further workgroups transpose w (dense: bring it into fragment order);
+//   2. router_dw_kernel        bound by the matrix pipes at the clock that they leave (1.6 to 1.7 GHz of 2.4);
+//   3. router_dx_list_kernel   dx (router_dx_kernel: dense), then the sums of the parts of dw and of db.
 #include <type_traits>
 
 #include "common.hpp"
@@ -35,16 +37,19 @@ struct RouterBwdArgs {
   int aff_dtype, logits_dtype;
   int64_t T, H, E, k;
   int softmax, chosen, norm, full;  // chosen: activation of the chosen logits only; full: affinities of all experts were handed out
+  int dense, kp;                    // dense: every expert has a part in dl; kp: k rounded up to a power of two
   u32x4* dlx;   // [tokens / 16][KS][2][64]   K = experts, for dx
   u32x4* dlw;   // [tokens / 32][2 KS][2][64] K = tokens, for dw
-  u32x4* wp;    // [H / 64][4][KS][64]
+  u32x4* wp;    // [H / 64][4][KS][64], for dense dx
+  uint16_t* wt; // [E][H], for sparse dx
+  uint2* list;  // [T][KP] expert and dl, k of them and zeros of the first expert behind them, for sparse dx
   float* dbp;   // [tokens / 32][E]
   uint16_t *dx, *dw;
   float* dwp;   // [splits][H][E]
   void* db;
   int db_dtype;
   int64_t steps, splits;  // steps of 32 tokens; parts of them for dw
-  int64_t n_dw, mt, hb_per;  // jobs of dw; 16-token tiles and 64-column blocks of a job of dx
+  int64_t x_splits;          // parts of the tokens for dx
 };
 
 __device__ __forceinline__ uint32_t hi_lo(float a, float b, uint32_t& lo) {
@@ -70,8 +75,24 @@ __global__ __launch_bounds__(256) void router_dlogits_kernel(const RouterBwdArgs
   constexpr int EP = 32 * KS, PITCH = EP + 4;
   extern __shared__ __attribute__((aligned(16))) float s_dl[];  // [32][PITCH]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (blockIdx.x >= a.steps) {  // w: 64 rows into fragment order; lane (r, g) of tile m holds row 16 (r / 4) + 4 m + r % 4, so that a
-    const int64_t hb = blockIdx.x - a.steps;  // lane's results are 16 neighbours
+  if (blockIdx.x >= a.steps) {  // 64 rows of w
+    const int64_t hb = blockIdx.x - a.steps;
+    if (!a.dense) {
+      uint16_t* s_w = (uint16_t*)s_dl;  // [64][E]
+      const uint16_t* src = a.w + hb * 64 * a.E;
+      for (int i = tid; i < 64 * (int)a.E; i += 256) s_w[i] = src[i];
+      __syncthreads();
+      for (int i = tid; i < 8 * (int)a.E; i += 256) {
+        const int e = i >> 3, p = i & 7;
+        u32x4 v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          v[q] = (uint32_t)s_w[(8 * p + 2 * q) * (int)a.E + e] | (uint32_t)s_w[(8 * p + 2 * q + 1) * (int)a.E + e] << 16;
+        *(u32x4*)(a.wt + e * a.H + hb * 64 + 8 * p) = v;
+      }
+      return;
+    }
+    // fragments: lane (r, g) of tile m holds row 16 (r / 4) + 4 m + r % 4, so that a lane's results are 16 neighbours
     for (int i = tid; i < 4 * KS * 64; i += 256) {
       const int l = i & 63, ks = (i >> 6) % KS, m = (i >> 6) / KS, r = l & 15;
       const int64_t h = hb * 64 + 16 * (r >> 2) + 4 * m + (r & 3), e = 32 * ks + 8 * (l >> 4);
@@ -105,26 +126,32 @@ __global__ __launch_bounds__(256) void router_dlogits_kernel(const RouterBwdArgs
     }
     const float l = on ? load_as_f32(a.logits, a.logits_dtype, t * a.E + id) : -__builtin_inff();
     const float g = on ? load_as_f32(a.d_aff, a.aff_dtype, t * a.E + id) : 0.f;
-    if (a.softmax && !(a.chosen || a.norm)) {
-      if (on) s_dl[tl * PITCH + id] = g;  // below
+    float dl = 0.f;
+    if (a.dense) {
+      dl = g;  // below
     } else if (a.softmax) {
       const float p = on ? expf(l - max8(on ? l : -__builtin_inff())) : 0.f;
       const float q = p / sum8(p);
       const float mean = sum8(on ? g * q : 0.f);
-      if (on) s_dl[tl * PITCH + id] = q * (g - mean);
+      dl = q * (g - mean);
     } else {
       const float e = expf(-fabsf(l)), r = 1.f / (1.f + e);  // sigmoid(|l|); sigmoid(l) = r or e r
       const float s = on ? (l >= 0.f ? r : e * r) : 0.f, slope = e * r * r;
-      float gg = g;
-      if (a.norm && !a.chosen) {
+      dl = g * slope;
+      if (a.norm) {
         const float total = sum8(s);
         const float mean = sum8(on ? g * s : 0.f) / total;
-        gg = (g - mean) / total;
+        dl = (g - mean) / total * slope;
       }
-      if (on) s_dl[tl * PITCH + id] = gg * slope;
+    }
+    if (on) s_dl[tl * PITCH + id] = dl;
+    if (!a.dense && t < a.T && j < a.kp) {
+      const uint64_t who = __ballot(on) >> (lane & 56) & 0xff;
+      const int first = __shfl(id, (lane & 56) | (who ? __builtin_ctzll(who) : 0), 64);
+      a.list[t * a.kp + j] = on ? make_uint2((uint32_t)id, __float_as_uint(dl)) : make_uint2(who ? (uint32_t)first : 0u, 0u);
     }
   }
-  if (a.full || (a.softmax && !(a.chosen || a.norm))) {
+  if (a.dense) {
     // every expert has a part: the lanes of a wave share a token's row
     __syncthreads();
     constexpr int NE = (EP + 63) / 64;
@@ -176,7 +203,7 @@ __global__ __launch_bounds__(256) void router_dlogits_kernel(const RouterBwdArgs
     a.dbp[blockIdx.x * a.E + e] = v;
   }
   const int c = lane & 15, g = lane >> 4;
-  for (int i = wave; i < 2 * KS; i += 4) {  // dx: token tile i / KS, 32 experts i % KS
+  for (int i = a.dense ? wave : 2 * KS; i < 2 * KS; i += 4) {  // dx: token tile i / KS, 32 experts i % KS
     const float* row = s_dl + (16 * (i / KS) + c) * PITCH + 32 * (i % KS) + 8 * g;
     u32x4 h, lo;
 #pragma unroll
@@ -208,18 +235,32 @@ __device__ __forceinline__ v4f mfma(const u32x4& x, const u32x4& y, const v4f& c
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x), __builtin_bit_cast(v8bf, y), c, 0, 0, 0);
 }
 
-constexpr int GRAD_THREADS = 512;
-constexpr int GRAD_LDS = 128 * 1024;
+constexpr int DW_THREADS = 512, DX_THREADS = 256, DX_LIST_THREADS = 1024;
 
-// dw: 128 columns of x by up to 256 experts over a part of the tokens.  Waves 0 .. 3 and 4 .. 7 take alternate steps of 32 tokens;
-// within either four, a wave has a quarter of the experts.  x is read in rows (16 bytes of 8 columns per lane) and turned in
-// registers: lane (r, g) holds 8 tokens x 8 columns, i.e. the fragments of eight row tiles whose row r is column 8 r + j.
+// Rows [t0, t0 + 32) of x or dx, as a buffer: what lies behind the last token reads as zeros and is not written.  No branch
+// stands around a load or store then, and the waits count the operations that are really out.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t token_rows(const uint16_t* base, int64_t t0, int64_t t1, int64_t H, int rows) {
+  const int64_t left = t1 - t0 < rows ? t1 - t0 : rows;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(base + t0 * H), 0, left > 0 ? (int)(left * H * 2) : 0, 0x00020000);
+}
+
+// dw: 128 columns of x by up to 256 experts over a part of the tokens.  Waves 0 .. 3 and 4 .. 7 take alternate steps of 32 tokens
+// (two waves per SIMD: the one multiplies while the other waits), a quarter of the experts per wave.  A step's rows (256 bytes
+// each) go through LDS.  Lane (r, g) reads 8 tokens x 8 columns of them and turns them in registers: they are the fragments of
+// eight row tiles whose row r is column 8 r + j.  A step goes over them twice, for dl's hi and for its lo parts, so that the
+// fragments of either part arrive in registers that the other half step has no use for; the rows are asked for two steps ahead.
 template <int KS>
-__device__ __forceinline__ void grad_w(const RouterBwdArgs& a, int64_t job, uint8_t* smem) {
-  constexpr int NQ = KS > 8 ? KS / 8 : 1;          // column blocks of 256 experts
-  constexpr int NT = KS > 8 ? 4 : KS / 2;          // 16-expert tiles per wave
+struct GradW {
+  static constexpr int NQ = KS > 8 ? KS / 8 : 1;  // column blocks of 256 experts
+  static constexpr int NT = KS > 8 ? 4 : KS / 2;  // 16-expert tiles per wave
+};
+template <int KS>
+__global__ __launch_bounds__(DW_THREADS) void router_dw_kernel(const RouterBwdArgs a) {
+  constexpr int NQ = GradW<KS>::NQ, NT = GradW<KS>::NT;
+  __shared__ __attribute__((aligned(16))) u32x4 s_x[2][2][512];  // [group][buffer][32 tokens][16]; at the end the sums of a quarter
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4, kg = wave >> 2, nq = wave & 3;
+  const int tid = threadIdx.x & 255, kg = wave >> 2, nq = wave & 3, r = lane & 15, g = lane >> 4;
+  const int64_t job = blockIdx.x;
   const int64_t nb = job % NQ, hb = job / NQ % (a.H / 128), sp = job / NQ / (a.H / 128);
   const int64_t s0 = a.steps * sp / a.splits, s1 = a.steps * (sp + 1) / a.splits;
   const int n0 = (int)nb * 16 + nq * NT;  // first of the wave's 16-expert tiles
@@ -228,24 +269,26 @@ __device__ __forceinline__ void grad_w(const RouterBwdArgs& a, int64_t job, uint
   for (int j = 0; j < 8; ++j)
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[j][n] = (v4f){0.f, 0.f, 0.f, 0.f};
-  const uint16_t* xc = a.x + hb * 128 + 8 * r;
-  for (int64_t s = s0 + kg; s < s1; s += 2) {
-    u32x4 x[8], b[NT], bl[NT];
-    const int64_t t = s * 32 + 8 * g;
+  const int off = (int)(((tid >> 4) * a.H + hb * 128 + 8 * (tid & 15)) * 2), half = (int)(16 * a.H * 2);
+  u32x4 in[2], b[NT], bl[NT];
+  auto fetch_x = [&](int64_t s) {
+    const __amdgpu_buffer_rsrc_t rows = token_rows(a.x, s * 32, s < s1 ? a.T : 0, a.H, 32);
+    in[0] = __builtin_amdgcn_raw_buffer_load_b128(rows, off, 0, 0);
+    in[1] = __builtin_amdgcn_raw_buffer_load_b128(rows, off + half, 0, 0);
+  };
+  auto store_x = [&](u32x4* buf) {
+    buf[tid] = in[0];
+    buf[256 + tid] = in[1];
+  };
+  auto fetch_dl = [&](int64_t s, int part, u32x4(&d)[NT]) {
+    const u32x4* src = a.dlw + (((s < s1 ? s : s1 - 1) * 2 * KS + n0) * 2 + part) * 64 + lane;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = u32x4{0, 0, 0, 0};
-      if (t + j < a.T) {
-        const u32x4_any d = *(const u32x4_any*)(xc + (t + j) * a.H);
-        x[j] = u32x4{d[0], d[1], d[2], d[3]};
-      }
-    }
-    const u32x4* src = a.dlw + ((s * 2 * KS + n0) * 2) * 64 + lane;
+    for (int n = 0; n < NT; ++n) d[n] = src[n * 128];
+  };
+  auto multiply = [&](const u32x4* buf, const u32x4(&d)[NT]) {
+    u32x4 x[8];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      b[n] = src[n * 128];
-      bl[n] = src[n * 128 + 64];
-    }
+    for (int j = 0; j < 8; ++j) x[j] = buf[(8 * g + j) * 16 + r];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       u32x4 f;
@@ -253,180 +296,304 @@ __device__ __forceinline__ void grad_w(const RouterBwdArgs& a, int64_t job, uint
       for (int q = 0; q < 4; ++q)  // tokens 2 q and 2 q + 1 of column j
         f[q] = __builtin_amdgcn_perm(x[2 * q + 1][j / 2], x[2 * q][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) acc[j][n] = mfma(f, b[n], acc[j][n]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) acc[j][n] = mfma(f, bl[n], acc[j][n]);
+      for (int n = 0; n < NT; ++n) acc[j][n] = mfma(f, d[n], acc[j][n]);
     }
-  }
-  v4f* s_acc = (v4f*)smem + (int64_t)nq * (8 * NT * 64) + lane;
-  if (kg == 1) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s_acc[(j * NT + n) * 64] = acc[j][n];
-  }
+  };
+  // both groups take as many turns: in one without a step the rows are zeros (and dl some step's, which they leave at zero)
+  const int64_t turns = (s1 - s0 + 1) / 2;
+  fetch_x(s0 + kg);
+  store_x(s_x[kg][0]);
+  fetch_x(s0 + kg + 2);
+  fetch_dl(s0 + kg, 0, b);
   __syncthreads();
+  for (int64_t i = 0; i < turns; ++i) {
+    const int64_t s = s0 + 2 * i + kg;
+    const u32x4* buf = s_x[kg][i & 1];
+    fetch_dl(s, 1, bl);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(buf, b);
+    __builtin_amdgcn_sched_barrier(0);
+    store_x(s_x[kg][(i + 1) & 1]);
+    fetch_dl(s + 2, 0, b);
+    fetch_x(s + 4);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(buf, bl);
+    __syncthreads();
+  }
+  // the second group's sums to the first by way of LDS, two row tiles of 16 columns at a time
+  v4f* s_acc = (v4f*)s_x + nq * (2 * NT * 64) + lane;
+#pragma unroll
+  for (int j0 = 0; j0 < 8; j0 += 2) {
+    if (kg == 1) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s_acc[(j * NT + n) * 64] = acc[j0 + j][n];
+    }
+    __syncthreads();
+    if (kg == 0) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[j0 + j][n] += s_acc[(j * NT + n) * 64];
+    }
+    __syncthreads();
+  }
   if (kg == 1) return;
   const bool whole = a.splits == 1;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int n = 0; n < NT; ++n) {
+    const int64_t e = (n0 + n) * 16 + r;
+    if (e < a.E) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const v4f v = acc[j][n] + s_acc[(j * NT + n) * 64];
-      const int64_t e = (n0 + n) * 16 + r;
-      if (e < a.E) {
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 8; ++j) {
           const int64_t at = (hb * 128 + 8 * (4 * g + i) + j) * a.E + e;
-          if (whole) a.dw[at] = f32_to_bf16_bits(v[i]);
-          else a.dwp[sp * a.H * a.E + at] = v[i];
+          if (whole) a.dw[at] = f32_to_bf16_bits(acc[j][n][i]);
+          else a.dwp[sp * a.H * a.E + at] = acc[j][n][i];
         }
+    }
+  }
+}
+
+// The parts of dw and db added up, by the workgroups that have written dx.
+__device__ __forceinline__ void reduce_parts(const RouterBwdArgs& a, int threads) {
+  const int64_t first = (int64_t)blockIdx.x * threads + threadIdx.x, step = (int64_t)gridDim.x * threads;
+  if (a.splits > 1) {
+    const int64_t n = a.H * a.E;  // (H is a multiple of 128: whole pieces of four)
+    for (int64_t i = first; i < n / 4; i += step) {
+      v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
+      for (int64_t s = 0; s < a.splits; ++s) v += ((const v4f*)(a.dwp + s * n))[i];
+      typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+      *(u32x2_any*)(a.dw + 4 * i) = u32x2_any{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3])};
+    }
+  }
+  if (a.db)
+    for (int64_t e = first >> 6; e < a.E; e += step >> 6) {
+      float v = 0.f;
+      for (int64_t s = threadIdx.x & 63; s < a.steps; s += 64) v += a.dbp[s * a.E + e];
+      v = wave_sum(v);
+      if ((threadIdx.x & 63) == 0) {
+        if (a.db_dtype == MOE_DT_FP32) ((float*)a.db)[e] = v;
+        else ((uint16_t*)a.db)[e] = f32_to_bf16_bits(v);
       }
     }
 }
 
-// dx: up to 128 tokens, whose dl lie in LDS, by some blocks of 64 columns, each wave a block at a time with the block's w in
-// registers.
-template <int KS>
-__device__ __forceinline__ void grad_x(const RouterBwdArgs& a, int64_t job, uint8_t* smem) {
-  constexpr int NM = KS > 8 ? 2 : 4;  // row tiles whose w is held at a time
+// dx of k experts per token: a workgroup keeps the slice of w of 64 * CPL columns in LDS, a wave takes a token at a time, CPL
+// columns per lane: k reads of LDS and k multiply-adds per value, expert and dl in scalar registers.
+template <int CPL, int KP>
+__global__ __launch_bounds__(DX_LIST_THREADS) void router_dx_list_kernel(const RouterBwdArgs a) {
+  constexpr int COLS = 64 * CPL, W = CPL / 2;  // words of a lane
+  extern __shared__ __attribute__((aligned(16))) uint32_t s_w[];  // [E][COLS / 2]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  const int64_t parts = (a.H / 64 + a.hb_per - 1) / a.hb_per, tg = job / parts, hp = job % parts;
-  const int64_t tile0 = tg * a.mt, tiles = a.steps * 2;
-  const int mt = (int)(tiles - tile0 < a.mt ? tiles - tile0 : a.mt);
-  u32x4* s_dl = (u32x4*)smem;
-  const u32x4* src = a.dlx + tile0 * (KS * 128);
-  for (int i = threadIdx.x; i < mt * KS * 128; i += GRAD_THREADS) s_dl[i] = src[i];
+  const int64_t slices = (a.H + COLS - 1) / COLS, c0 = blockIdx.x % slices * COLS, sp = blockIdx.x / slices;
+  const int cols = (int)(a.H - c0 < COLS ? a.H - c0 : COLS);  // (H is a multiple of 128)
+  const int pieces = cols / 8;
+  for (int i = threadIdx.x; i < (int)a.E * pieces; i += DX_LIST_THREADS) {
+    const int e = i / pieces, p = i - e * pieces;
+    *(u32x4*)(s_w + e * (COLS / 2) + 4 * p) = *(const u32x4*)(a.wt + e * a.H + c0 + 8 * p);
+  }
   __syncthreads();
-  const int64_t hb1 = (hp + 1) * a.hb_per < a.H / 64 ? (hp + 1) * a.hb_per : a.H / 64;
-  for (int64_t hb = hp * a.hb_per + wave; hb < hb1; hb += GRAD_THREADS / 64) {
-#pragma unroll 1
-    for (int m0 = 0; m0 < 4; m0 += NM) {
-      u32x4 w[NM][KS];
+  const int64_t t0 = a.T * sp / a.x_splits, t1 = a.T * (sp + 1) / a.x_splits;
+  const bool mine = lane * CPL < cols;
+  // (address space 4: read-only for the launch, uniform over the wave.  The lists come by scalar loads, which no store is waited
+  // for ahead of, a token early)
+  typedef const __attribute__((address_space(4))) uint32_t* list_ptr;
+  auto fetch = [&](int64_t t, uint32_t(&l)[2 * KP]) {
+    const list_ptr src = (list_ptr)(uintptr_t)(a.list + (t < t1 ? t : t1 - 1) * KP);
 #pragma unroll
-      for (int m = 0; m < NM; ++m)
+    for (int i = 0; i < 2 * KP; ++i) l[i] = src[i];
+  };
+  constexpr int WAVES = DX_LIST_THREADS / 64;
+  uint32_t now[2 * KP], next[2 * KP];
+  if (t0 + wave < t1) fetch(t0 + wave, now);
+  for (int64_t t = t0 + wave; t < t1; t += WAVES) {
+    fetch(t + WAVES, next);
+    float acc[CPL];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) w[m][ks] = a.wp[((hb * 4 + m0 + m) * KS + ks) * 64 + lane];
-#pragma unroll 1
-      for (int i = 0; i < mt; ++i) {
-        v4f acc[NM];
+    for (int i = 0; i < CPL; ++i) acc[i] = 0.f;
+    uint32_t v[KP][W];
 #pragma unroll
-        for (int m = 0; m < NM; ++m) acc[m] = (v4f){0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < KP; ++j)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const u32x4 h = s_dl[(i * KS + ks) * 128 + lane], lo = s_dl[(i * KS + ks) * 128 + 64 + lane];
+      for (int q = 0; q < W; ++q) v[j][q] = s_w[now[2 * j] * (COLS / 2) + lane * W + q];
 #pragma unroll
-          for (int m = 0; m < NM; ++m) acc[m] = mfma(w[m][ks], h, acc[m]);
+    for (int j = 0; j < KP; ++j) {
+      const float dl = __uint_as_float(now[2 * j + 1]);
 #pragma unroll
-          for (int m = 0; m < NM; ++m) acc[m] = mfma(w[m][ks], lo, acc[m]);
-        }
-        const int64_t t = (tile0 + i) * 16 + c;
-        if (t < a.T) {
-          uint16_t* dst = a.dx + t * a.H + hb * 64 + 16 * g + 4 * m0;
-#pragma unroll
-          for (int m = 0; m < NM; m += 2) {
-            const u32x4_any v = {pack2_bf16(acc[m][0], acc[m][1]), pack2_bf16(acc[m][2], acc[m][3]),
-                                 pack2_bf16(acc[m + 1][0], acc[m + 1][1]), pack2_bf16(acc[m + 1][2], acc[m + 1][3])};
-            *(u32x4_any*)(dst + 4 * m) = v;
-          }
-        }
+      for (int q = 0; q < W; ++q) {
+        acc[2 * q] = fmaf(dl, bf16_lo(v[j][q]), acc[2 * q]);
+        acc[2 * q + 1] = fmaf(dl, bf16_hi(v[j][q]), acc[2 * q + 1]);
       }
     }
+    if (mine) {
+      uint32_t* dst = (uint32_t*)(a.dx + t * a.H + c0) + lane * W;
+      if constexpr (W == 2) {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        __builtin_nontemporal_store((u32x2{pack2_bf16(acc[0], acc[1]), pack2_bf16(acc[2], acc[3])}), (u32x2*)dst);
+      } else {
+        __builtin_nontemporal_store(pack2_bf16(acc[0], acc[1]), dst);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * KP; ++i) now[i] = next[i];
   }
+  reduce_parts(a, DX_LIST_THREADS);
 }
 
+// Dense dx: each wave keeps the w of 64 columns (32 beyond 256 experts) in registers and multiplies 16 tokens after 16 tokens of a
+// part of them, whose dl go through LDS, the next ones' while these are multiplied.
 template <int KS>
-__global__ __launch_bounds__(GRAD_THREADS) void router_grad_kernel(const RouterBwdArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+struct GradX {
+  static constexpr int NM = KS > 8 ? 2 : 4;         // row tiles of 16 columns per wave
+  static constexpr int COLS = NM * 16 * 4;          // columns of a workgroup
+};
+template <int KS>
+__global__ __launch_bounds__(DX_THREADS, 2) void router_dx_kernel(const RouterBwdArgs a) {
+  __shared__ __attribute__((aligned(16))) u32x4 s_dl[2 * KS * 128];  // [2][KS][2][64]
   const int64_t job = blockIdx.x;
-  if (job < a.n_dw) grad_w<KS>(a, job, smem);
-  else grad_x<KS>(a, job - a.n_dw, smem);
-}
-
-__global__ __launch_bounds__(256) void router_reduce_kernel(const RouterBwdArgs a, int64_t n_w) {
-  if (blockIdx.x < n_w) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = a.H * a.E;
-    if (i >= n) return;
-    float v = 0.f;
-    for (int64_t s = 0; s < a.splits; ++s) v += a.dwp[s * n + i];
-    a.dw[i] = f32_to_bf16_bits(v);
-    return;
+  constexpr int NM = GradX<KS>::NM, PIECES = KS * 128 / DX_THREADS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int64_t groups = (a.H + GradX<KS>::COLS - 1) / GradX<KS>::COLS, hg = job % groups, sp = job / groups;
+  const int64_t tiles = (a.T + 15) / 16, i0 = tiles * sp / a.x_splits, i1 = tiles * (sp + 1) / a.x_splits;
+  const int64_t unit = hg * 4 + wave;  // of 16 NM columns
+  const bool mine = unit * NM / 4 < a.H / 64;  // (the others multiply the last block once more and keep nothing)
+  const int64_t hb = mine ? unit * NM / 4 : a.H / 64 - 1, m0 = unit * NM % 4;
+  u32x4 w[NM][KS];
+#pragma unroll
+  for (int m = 0; m < NM; ++m)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) w[m][ks] = a.wp[((hb * 4 + m0 + m) * KS + ks) * 64 + lane];
+  u32x4 in[PIECES];
+  auto fetch = [&](int64_t i) {
+    const u32x4* src = a.dlx + (i < i1 ? i : i1 - 1) * (KS * 128) + tid;
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) in[q] = src[q * DX_THREADS];
+  };
+  auto store = [&](u32x4* buf) {
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) buf[q * DX_THREADS + tid] = in[q];
+  };
+  fetch(i0);
+  store(s_dl);
+  fetch(i0 + 1);
+  __syncthreads();
+  const int off = (int)((c * a.H + hb * 64 + 16 * g + 4 * m0) * 2);
+  for (int64_t i = i0; i < i1; ++i) {
+    const u32x4* buf = s_dl + ((i - i0) & 1) * (KS * 128);
+    v4f acc[NM];
+#pragma unroll
+    for (int m = 0; m < NM; ++m) acc[m] = (v4f){0.f, 0.f, 0.f, 0.f};
+    // the next 32 experts' dl are read from LDS while these are multiplied
+    u32x4 h[2], lo[2];
+    h[0] = buf[lane];
+    lo[0] = buf[64 + lane];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS) {
+        h[(ks + 1) & 1] = buf[(ks + 1) * 128 + lane];
+        lo[(ks + 1) & 1] = buf[(ks + 1) * 128 + 64 + lane];
+      }
+      if (ks == KS / 2) {
+        store(s_dl + ((i + 1 - i0) & 1) * (KS * 128));
+        fetch(i + 2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int m = 0; m < NM; ++m) acc[m] = mfma(w[m][ks], h[ks & 1], acc[m]);
+#pragma unroll
+      for (int m = 0; m < NM; ++m) acc[m] = mfma(w[m][ks], lo[ks & 1], acc[m]);
+    }
+    const __amdgpu_buffer_rsrc_t rows = token_rows(a.dx, i * 16, mine ? a.T : 0, a.H, 16);
+#pragma unroll
+    for (int m = 0; m < NM; m += 2) {
+      const u32x4 v = {pack2_bf16(acc[m][0], acc[m][1]), pack2_bf16(acc[m][2], acc[m][3]),
+                       pack2_bf16(acc[m + 1][0], acc[m + 1][1]), pack2_bf16(acc[m + 1][2], acc[m + 1][3])};
+      __builtin_amdgcn_raw_buffer_store_b128(v, rows, off + 8 * m, 0, 0);
+    }
+    __syncthreads();
   }
-  const int64_t e = (int64_t)(blockIdx.x - n_w) * 4 + (threadIdx.x >> 6);
-  if (e >= a.E) return;
-  float v = 0.f;
-  for (int64_t s = threadIdx.x & 63; s < a.steps; s += 64) v += a.dbp[s * a.E + e];
-  v = wave_sum(v);
-  if ((threadIdx.x & 63) == 0) {
-    if (a.db_dtype == MOE_DT_FP32) ((float*)a.db)[e] = v;
-    else ((uint16_t*)a.db)[e] = f32_to_bf16_bits(v);
-  }
+  reduce_parts(a, DX_THREADS);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 
 struct RouterBwdPlan {
   int ks;
-  int64_t steps, splits, mt, hb_per, n_dw, n_dx;
-  size_t dlx, dlw, wp, dbp, dwp, total;
+  int64_t steps, splits, n_dw;
+  size_t dlx, dlw, w, list, dbp, dwp, total;
 };
 static RouterBwdPlan router_bwd_plan(int64_t T, int64_t H, int64_t E) {
   RouterBwdPlan p;
   p.ks = E <= 64 ? 2 : E <= 128 ? 4 : E <= 256 ? 8 : 16;
   p.steps = (T + 31) / 32;
-  const int64_t nq = p.ks > 8 ? p.ks / 8 : 1, tiles = H / 128 * nq;
-  // dw: a workgroup per CU where the tokens allow parts of eight steps, four per half of a workgroup
+  // a workgroup of dw per CU where the tokens allow parts of eight steps: every part is written and read again
+  const int64_t tiles = H / 128 * (p.ks > 8 ? p.ks / 8 : 1);
   p.splits = 256 / tiles;
   if (p.splits > p.steps / 8) p.splits = p.steps / 8;
   if (p.splits < 1) p.splits = 1;
   p.n_dw = tiles * p.splits;
-  // dx: as many tokens as LDS holds, fewer where that leaves CUs without a job; two blocks of 64 columns per wave, or one
-  const int64_t most = GRAD_LDS / (p.ks * 2048);
-  p.hb_per = 16;
-  p.mt = p.steps * 2 * ((H / 64 + p.hb_per - 1) / p.hb_per) / 256;
-  if (p.mt < 1) {
-    p.hb_per = 8;
-    p.mt = 1;
-  }
-  if (p.mt > (most < 8 ? most : 8)) p.mt = most < 8 ? most : 8;
-  p.n_dx = (p.steps * 2 + p.mt - 1) / p.mt * ((H / 64 + p.hb_per - 1) / p.hb_per);
   auto al = [](size_t v) { return (v + 255) & ~(size_t)255; };
   size_t off = 0;
   p.dlx = off; off += al((size_t)p.steps * 2 * p.ks * 2048);
   p.dlw = off; off += al((size_t)p.steps * 2 * p.ks * 2048);
-  p.wp = off; off += al((size_t)H / 64 * 4 * p.ks * 1024);
+  p.w = off; off += al((size_t)H / 64 * 4 * p.ks * 1024);  // (fragments, or [E][H])
+  p.list = off; off += al((size_t)T * 8 * 8);
   p.dbp = off; off += al((size_t)p.steps * E * 4);
   p.dwp = off; off += p.splits > 1 ? al((size_t)p.splits * H * E * 4) : 0;
   p.total = off;
   return p;
 }
 
-template <int KS>
-static int launch_router_bwd(const RouterBwdArgs& a, const RouterBwdPlan& p, hipStream_t s) {
-  constexpr int LDS1 = 32 * (32 * KS + 4) * 4;
-  if (allow_lds<router_dlogits_kernel<KS>>(LDS1) != hipSuccess) return MOE_E_LAUNCH;
-  if (allow_lds<router_grad_kernel<KS>>(GRAD_LDS) != hipSuccess) return MOE_E_LAUNCH;
-  hipLaunchKernelGGL(router_dlogits_kernel<KS>, dim3((unsigned)(p.steps + a.H / 64)), dim3(256), LDS1, s, a);
+// Parts of the tokens for dx: a workgroup per CU of `slices` slices of columns, `least` tokens each at least.
+static int64_t dx_splits(int64_t slices, int64_t T, int64_t least) {
+  int64_t n = 256 / slices;
+  if (n > (T + least - 1) / least) n = (T + least - 1) / least;
+  return n < 1 ? 1 : n;
+}
+template <int CPL, int KP>
+static int launch_dx_list(RouterBwdArgs& a, hipStream_t s) {
+  constexpr int LDS = 128 * 1024;
+  if (allow_lds<router_dx_list_kernel<CPL, KP>>(LDS) != hipSuccess) return MOE_E_LAUNCH;
+  const int64_t slices = (a.H + 64 * CPL - 1) / (64 * CPL);
+  a.x_splits = dx_splits(slices, a.T, DX_LIST_THREADS / 64);
+  hipLaunchKernelGGL((router_dx_list_kernel<CPL, KP>), dim3((unsigned)(slices * a.x_splits)), dim3(DX_LIST_THREADS), (size_t)a.E * 128 * CPL, s, a);
   MOE_CHECK_LAUNCH();
-  const int lds_w = 4 * 8 * (KS > 8 ? 4 : KS / 2) * 64 * 16, lds_x = (int)p.mt * KS * 2048;
-  hipLaunchKernelGGL(router_grad_kernel<KS>, dim3((unsigned)(p.n_dw + p.n_dx)), dim3(GRAD_THREADS), lds_w > lds_x ? lds_w : lds_x, s,
-                     a);
-  MOE_CHECK_LAUNCH();
-  const int64_t n_w = p.splits > 1 ? (a.H * a.E + 255) / 256 : 0, n_b = a.db ? (a.E + 3) / 4 : 0;
-  if (n_w + n_b > 0) {
-    hipLaunchKernelGGL(router_reduce_kernel, dim3((unsigned)(n_w + n_b)), dim3(256), 0, s, a, n_w);
-    MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+template <int CPL>
+static int launch_dx_list_k(RouterBwdArgs& a, hipStream_t s) {
+  switch (a.kp) {
+    case 1: return launch_dx_list<CPL, 1>(a, s);
+    case 2: return launch_dx_list<CPL, 2>(a, s);
+    case 4: return launch_dx_list<CPL, 4>(a, s);
+    default: return launch_dx_list<CPL, 8>(a, s);
   }
+}
+template <int KS>
+static int launch_router_bwd(RouterBwdArgs& a, const RouterBwdPlan& p, hipStream_t s) {
+  constexpr int LDS = 32 * (32 * KS + 4) * 4;
+  if (allow_lds<router_dlogits_kernel<KS>>(LDS) != hipSuccess) return MOE_E_LAUNCH;
+  hipLaunchKernelGGL(router_dlogits_kernel<KS>, dim3((unsigned)(p.steps + a.H / 64)), dim3(256), LDS, s, a);
+  MOE_CHECK_LAUNCH();
+  hipLaunchKernelGGL(router_dw_kernel<KS>, dim3((unsigned)p.n_dw), dim3(DW_THREADS), 0, s, a);
+  MOE_CHECK_LAUNCH();
+  // (256 experts by 256 columns of w, or 512 by 128, are the 128 KB of LDS that a slice may take)
+  if (!a.dense) return a.E <= 256 ? launch_dx_list_k<4>(a, s) : launch_dx_list_k<2>(a, s);
+  const int64_t groups = (a.H + GradX<KS>::COLS - 1) / GradX<KS>::COLS;
+  a.x_splits = dx_splits(groups, a.T, 16);
+  hipLaunchKernelGGL(router_dx_kernel<KS>, dim3((unsigned)(groups * a.x_splits)), dim3(DX_THREADS), 0, s, a);
+  MOE_CHECK_LAUNCH();
   return MOE_OK;
 }
 
 static int router_bwd_shape(int64_t T, int64_t H, int64_t E) {
   if (T < 1 || H < 1 || E < 1) return MOE_E_BAD_ARG;
-  // (a launch holds fewer than 2^32 threads)
+  // (every launch stays below 2^32 threads: at these limits 2^21 + 2^14 workgroups of 256, 2^14 of 512, 2^13 of 1024)
   if (E > 512 || H % 128 != 0 || H > (int64_t)1 << 20 || T > (int64_t)1 << 26) return MOE_E_BAD_SHAPE;
-  const RouterBwdPlan p = router_bwd_plan(T, H, E);
-  if ((p.n_dw + p.n_dx) * GRAD_THREADS >= (int64_t)1 << 32 || (p.steps + H / 64) * 256 >= (int64_t)1 << 32) return MOE_E_BAD_SHAPE;
   return MOE_OK;
 }
 
@@ -452,7 +619,7 @@ extern "C" int moe_router_topk_bwd(const void* d_affinities, int aff_dtype, cons
   if (k < 1 || k > 8 || k > E) return MOE_E_BAD_SHAPE;
   const RouterBwdPlan p = router_bwd_plan(T, H, E);
   if (!workspace || workspace_bytes < p.total) return MOE_E_WORKSPACE;
-  if (((uintptr_t)workspace & 15) != 0) return MOE_E_BAD_ARG;
+  if ((((uintptr_t)workspace | (uintptr_t)x | (uintptr_t)d_x) & 15) != 0) return MOE_E_BAD_ARG;
   uint8_t* ws = (uint8_t*)workspace;
   RouterBwdArgs a;
   a.d_aff = d_affinities;
@@ -467,16 +634,20 @@ extern "C" int moe_router_topk_bwd(const void* d_affinities, int aff_dtype, cons
   a.chosen = !router_pre_norm;
   a.norm = router_pre_norm && norm_topk_prob;
   a.full = router_pre_norm && !norm_topk_prob && !mask_to_topk;
+  a.dense = a.full || (a.softmax && !a.chosen && !a.norm);
+  a.kp = k > 4 ? 8 : k > 2 ? 4 : k;
   a.dlx = (u32x4*)(ws + p.dlx);
   a.dlw = (u32x4*)(ws + p.dlw);
-  a.wp = (u32x4*)(ws + p.wp);
+  a.wp = (u32x4*)(ws + p.w);
+  a.wt = (uint16_t*)(ws + p.w);
+  a.list = (uint2*)(ws + p.list);
   a.dbp = (float*)(ws + p.dbp);
   a.dx = (uint16_t*)d_x;
   a.dw = (uint16_t*)d_w;
   a.dwp = (float*)(ws + p.dwp);
   a.db = d_bias;
   a.db_dtype = bias_dtype;
-  a.steps = p.steps; a.splits = p.splits; a.n_dw = p.n_dw; a.mt = p.mt; a.hb_per = p.hb_per;
+  a.steps = p.steps; a.splits = p.splits;
   const hipStream_t s = (hipStream_t)stream;
   switch (p.ks) {
     case 2: return launch_router_bwd<2>(a, p, s);

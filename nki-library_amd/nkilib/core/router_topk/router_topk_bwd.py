@@ -29,6 +29,8 @@ def router_topk_bwd(d_expert_affinities, x, w, w_bias, router_logits, expert_ind
     if x.dim() != 2 or w.dim() != 2 or x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16 or x.shape[1] != w.shape[0]:
         kernel_assert(False, f"x and w must be bfloat16 [T, H] and [H, E] but are {x.dtype} {tuple(x.shape)} and {w.dtype} "
                              f"{tuple(w.shape)}")
+    if x.data_ptr() % 16:  # (rows are read in pieces of 16 bytes)
+        x = x.clone()
     (T, H), E = x.shape, w.shape[1]
     if not 1 <= E <= 512:
         kernel_assert(False, f"E must be in [1, 512] but got {E}")
