@@ -376,9 +376,10 @@ int moe_prepare_kmajor_weights(const moe_bwmm_args* args, void* gate_up_kmajor, 
  *
  * moe_token_slots: the table's inverse, int32 [T, 1 + top_k]: how many slots token t has, then the slots, ascending, then -1.
  * top_k <= 64.  A token that the table lists more than top_k times keeps the true count: the calls below give NaN for it (its
- * row, its slots' rows, its affinities).
+ * row, its slots' rows, its affinities).  They take the list in token_slots, or, with build_token_slots != 0, make it there
+ * first from token_position_to_id (only read then by moe_combine_tokens, nullable otherwise).
  *
- * moe_permute_tokens: out[s] = x[token of s], zero rows for padding; any element type (rows of row_bytes bytes).
+ * moe_permute_tokens: out[s] = x[token of s], zero rows for padding; any element type (rows of row_bytes < 2^31 bytes).
  *
  * moe_combine_tokens: out[t] = sum over t's slots s of expert_affinities[t, e(s)] * y[s]; affinities [T1 >= T, E] bf16 / fp32.
  * Slots of blocks whose expert is outside [0, E) count for nothing and are not read; rows of padding slots are not read.  With
@@ -392,12 +393,13 @@ int moe_token_slots(const int32_t* token_position_to_id, int64_t S, int64_t T, i
 int moe_permute_tokens(const void* x, const int32_t* token_position_to_id, int64_t S, int64_t T, int64_t row_bytes,
                        void* out, void* stream);
 int moe_combine_tokens(const void* y, int dtype, const void* expert_affinities, int aff_dtype, int64_t T1, int64_t E,
-                       const int32_t* block_to_expert, int64_t B, int64_t N, const int32_t* token_slots, int top_k,
-                       int64_t S, int64_t T, int64_t H, void* out, void* stream);
+                       const int32_t* token_position_to_id, const int32_t* block_to_expert, int64_t B, int64_t N,
+                       int32_t* token_slots, int top_k, int build_token_slots, int64_t S, int64_t T, int64_t H, void* out,
+                       void* stream);
 int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtype, const void* expert_affinities, int aff_dtype,
                            int64_t T1, int64_t E, const int32_t* token_position_to_id, const int32_t* block_to_expert,
-                           int64_t B, int64_t N, const int32_t* token_slots, int top_k, int64_t T, int64_t H, void* d_y,
-                           float* d_affinities, void* stream);
+                           int64_t B, int64_t N, int32_t* token_slots, int top_k, int build_token_slots, int64_t T,
+                           int64_t H, void* d_y, float* d_affinities, void* stream);
 
 /* ---- the gated activation with its inputs kept in 8 bits ------------------------------------ */
 

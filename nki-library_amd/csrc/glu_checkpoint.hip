@@ -69,20 +69,24 @@ __device__ __forceinline__ float clamp_value(float x, int mask, int hi_bit, int 
   return x;
 }
 
-// Largest finite magnitude among the group's four lanes -> scale byte.
+__device__ __forceinline__ uint32_t max_finite(uint32_t m, float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u && b > m ? b : m;
+}
+// Bits of the largest finite magnitude -> scale byte.
+__device__ __forceinline__ uint32_t scale_of(uint32_t m) {
+  const int s = (int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u ? 1 : 0);  // 448 = 1.75 * 2^8
+  return (uint32_t)(s < 0 ? 0 : s);
+}
+// The scale byte of a group that four neighbouring lanes hold.
 __device__ __forceinline__ uint32_t group_scale(const float (&v)[8]) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-    m = b < 0x7f800000u && b > m ? b : m;
-  }
+  for (int i = 0; i < 8; ++i) m = max_finite(m, v[i]);
   uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, true);  // lanes 1 0 3 2 of each four
   m = o > m ? o : m;
   o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, true);  // 2 3 0 1
-  m = o > m ? o : m;
-  const int s = (int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u ? 1 : 0);  // 448 = 1.75 * 2^8
-  return (uint32_t)(s < 0 ? 0 : s);
+  return scale_of(o > m ? o : m);
 }
 // Eight values -> eight codes.  (The values are at most 448 by then; infinities and NaN are written as such.)
 __device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t scale) {
@@ -157,9 +161,11 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n) {
     if (i < n) w[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
   return make_uint2(w[0], w[1]);
 }
+template <bool PAST = true>
 __device__ __forceinline__ void store_codes(uint8_t* p, int n, const uint2& c) {
   if (n == 8) {
-    __builtin_nontemporal_store((codes8{c.x, c.y}), (codes8*)p);
+    if (PAST) __builtin_nontemporal_store((codes8{c.x, c.y}), (codes8*)p);
+    else *(codes8*)p = codes8{c.x, c.y};
     return;
   }
 #pragma unroll
@@ -174,11 +180,13 @@ struct Place {
   int v, n;  // piece of the row, values in it
   bool in, on;  // a row; one that is not padding
 };
-__device__ __forceinline__ Place place_of(const GluArgs& a, int64_t row0, uint32_t rem0, uint32_t i) {
+__device__ __forceinline__ Place place_of(const GluArgs& a) {
+  // (a launch has fewer than 2^32 pieces: 32 bits, a division in 64 would take longer than the rest of a piece's arithmetic)
+  const uint32_t V = (uint32_t)a.V, base = blockIdx.x * 256u, row0 = base / V;
   Place p;
-  const uint32_t j = rem0 + i, dr = __umulhi(j, a.v_magic);
-  p.row = row0 + dr;
-  p.v = (int)(j - dr * (uint32_t)a.V);
+  const uint32_t j = base - row0 * V + threadIdx.x, dr = __umulhi(j, a.v_magic);
+  p.row = (int64_t)row0 + dr;
+  p.v = (int)(j - dr * V);
   p.in = p.row < a.R;
   p.on = p.in;
   if (p.in && a.tp2id) {
@@ -195,8 +203,7 @@ __global__ __launch_bounds__(256) void glu_checkpoint_kernel(const GluArgs a, co
                                                              uint8_t* __restrict__ h, uint8_t* __restrict__ codes,
                                                              uint8_t* __restrict__ scales) {
   constexpr int ES = Elem<DT>::SIZE;
-  const int64_t base = (int64_t)blockIdx.x * 256, row0 = base / a.V;
-  const Place p = place_of(a, row0, (uint32_t)(base - row0 * a.V), threadIdx.x);
+  const Place p = place_of(a);
   if (!p.in) return;  // (whole groups of four lanes: V is a multiple of four)
   const int64_t G = a.V / 4, off = p.row * 2 * a.I + 8 * p.v;
   float g[8], u[8], r[8];
@@ -235,8 +242,7 @@ __global__ __launch_bounds__(256) void glu_checkpoint_bwd_kernel(const GluArgs a
                                                                  const uint8_t* __restrict__ dh, uint8_t* __restrict__ d_gate_up,
                                                                  uint8_t* __restrict__ h) {
   constexpr int ES = Elem<DT>::SIZE;
-  const int64_t base = (int64_t)blockIdx.x * 256, row0 = base / a.V;
-  const Place p = place_of(a, row0, (uint32_t)(base - row0 * a.V), threadIdx.x);
+  const Place p = place_of(a);
   if (!p.in || p.n == 0) return;
   const int64_t G = a.V / 4, off = p.row * 2 * a.I + 8 * p.v;
   float dg[8], du[8], r[8];
@@ -277,8 +283,7 @@ __global__ __launch_bounds__(256) void glu_checkpoint_bwd_kernel(const GluArgs a
 template <int DT>
 __global__ __launch_bounds__(256) void dequantize_checkpoint_kernel(const GluArgs a, const uint8_t* __restrict__ codes,
                                                                     const uint8_t* __restrict__ scales, uint8_t* __restrict__ out) {
-  const int64_t base = (int64_t)blockIdx.x * 256, row0 = base / a.V;
-  const Place p = place_of(a, row0, (uint32_t)(base - row0 * a.V), threadIdx.x);
+  const Place p = place_of(a);
   if (!p.in || p.n == 0) return;
   const int64_t off = p.row * a.I + 8 * p.v;
   float v[8];
@@ -288,52 +293,79 @@ __global__ __launch_bounds__(256) void dequantize_checkpoint_kernel(const GluArg
 
 // ---- pack ---------------------------------------------------------------------------------------------------------
 
-// The checkpoint of moe_cte has a block's rows side by side: [N][2 I][B].  A workgroup turns a tile of `tb` rows x `tc` columns
-// (tb * tc = PACK_TILE, tc a multiple of 32) in LDS and writes each row's codes as runs along I.
+// The checkpoint of moe_cte has a block's rows side by side: [N][2 I][B].  A workgroup takes a tile of tb rows x tc columns (tb a
+// power of two up to 64, tb * tc = PACK_TILE, tc a multiple of 32) through LDS: read in pieces of eight neighbours, 16 bytes, then
+// a row and a group of 32 columns per thread.  Two bytes per value from LDS: neighbouring lanes hold neighbouring rows.
+// (Groups lie max(8, tb) values apart beyond their length, so that lanes of several groups do not meet in a bank.)
 constexpr int PACK_TILE = 8192;
 __global__ __launch_bounds__(256) void pack_checkpoint_kernel(const uint16_t* __restrict__ x, const int32_t* __restrict__ tp2id,
                                                               int64_t n_tokens, int64_t I, int64_t B, int ltb,
                                                               uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  __shared__ uint16_t s_x[PACK_TILE + 8 * 256];
-  const int tb = 1 << ltb, tc = PACK_TILE >> ltb, pitch = tc + 8;
+  __shared__ __attribute__((aligned(16))) uint16_t s_x[PACK_TILE + PACK_TILE / 32 * 8];
+  const int tid = threadIdx.x, tb = 1 << ltb, tc = PACK_TILE >> ltb, pad = tb > 8 ? tb : 8;
   const int64_t G = (I + 31) / 32, tiles_c = (I + tc - 1) / tc, tiles_b = (B + tb - 1) / tb;
-  int64_t i = blockIdx.x;
-  const int64_t ci = i % tiles_c;
-  i /= tiles_c;
+  uint32_t i = blockIdx.x;  // (divided in 32 bits: the tiles of one block are fewer than 2^24)
+  const int64_t ci = i % (uint32_t)tiles_c;
+  i /= (uint32_t)tiles_c;
   const int64_t z = i % 2;
   i /= 2;
-  const int64_t bi = i % tiles_b, blk = i / tiles_b;
+  const int64_t bi = i % (uint32_t)tiles_b, blk = i / (uint32_t)tiles_b;
   const int64_t c0 = ci * tc, r0 = bi * tb;
   const int nc = (int)(I - c0 < tc ? I - c0 : tc), nr = (int)(B - r0 < tb ? B - r0 : tb);
+  // the thread's row and group; a tile of padding alone is not read
+  const int r = tid & (tb - 1), cg = tid >> ltb;
+  bool on = r < nr;
+  if (tp2id && on) {
+    const int id = tp2id[blk * B + r0 + r];
+    on = id >= 0 && id < n_tokens;
+  }
+  const bool any = __syncthreads_or(on);
   const uint16_t* src = x + ((blk * 2 + z) * I + c0) * B + r0;
-  for (int e = threadIdx.x; e < PACK_TILE; e += 256) {
-    const int r = e & (tb - 1), c = e >> ltb;
-    uint16_t v = 0;
-    if (r < nr && c < nc) {
-      bool on = true;
-      if (tp2id) {
-        const int id = tp2id[blk * B + r0 + r];
-        on = id >= 0 && id < n_tokens;
+  auto at = [&](int c, int row) { return c / 32 * (32 * tb + pad) + (c % 32) * tb + row; };
+  if (any) {
+    if (((B % 8 == 0 && tb >= 8) || B == tb) && ((uintptr_t)src & 15) == 0 && nc * tb % 8 == 0) {
+      u32x4 d[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int e = 8 * (tid + 256 * q), c = e >> ltb, row = e & (tb - 1);
+        d[q] = u32x4{0, 0, 0, 0};
+        if (c < nc && row < nr) d[q] = __builtin_nontemporal_load((const u32x4*)(src + (int64_t)c * B + row));
       }
-      if (on) v = src[(int64_t)c * B + r];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int e = 8 * (tid + 256 * q);
+        *(u32x4*)(s_x + at(e >> ltb, e & (tb - 1))) = d[q];
+      }
+    } else {
+      for (int e = tid; e < PACK_TILE; e += 256) {
+        const int c = e >> ltb, row = e & (tb - 1);
+        s_x[at(c, row)] = c < nc && row < nr ? src[(int64_t)c * B + row] : (uint16_t)0;
+      }
     }
-    s_x[r * pitch + c] = v;
   }
   __syncthreads();
-  const int pieces = tc / 8;
-  for (int e = threadIdx.x; e < PACK_TILE / 8; e += 256) {
-    const int r = e / pieces, v8 = e - r * pieces;
-    float v[8];
+  const int left = nc - 32 * cg;
+  if (r >= nr || left <= 0) return;
+  float v[32];
+  uint32_t m = 0;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = bf16_bits_to_f32(s_x[r * pitch + 8 * v8 + q]);
-    const uint32_t s = group_scale(v);
-    const int left = nc - 8 * v8, n = left >= 8 ? 8 : left;
-    if (r < nr && n > 0) {
-      const int64_t row = (blk * B + r0 + r) * 2 + z;
-      store_codes(codes + row * I + c0 + 8 * v8, n, encode8(v, s));
-      if ((v8 & 3) == 0) scales[row * G + c0 / 32 + v8 / 4] = (uint8_t)s;
-    }
+  for (int c = 0; c < 32; ++c) {
+    v[c] = on && c < left ? bf16_bits_to_f32(s_x[cg * (32 * tb + pad) + c * tb + r]) : 0.f;
+    m = max_finite(m, v[c]);
   }
+  const uint32_t s = scale_of(m);
+  const int64_t row = (blk * B + r0 + r) * 2 + z;
+  uint8_t* dst = codes + row * I + c0 + 32 * cg;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float part[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[e] = v[8 * q + e];
+    const int n = left - 8 * q;
+    // (not past the caches: a row's 128 bytes come from several waves)
+    if (n > 0) store_codes<false>(dst + 8 * q, n > 8 ? 8 : n, encode8(part, s));
+  }
+  scales[row * G + c0 / 32 + cg] = (uint8_t)s;
 }
 
 }  // namespace moe

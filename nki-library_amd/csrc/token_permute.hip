@@ -9,8 +9,8 @@
 // hardly compute: their bound is memory.  Sums run over the slots in ascending order in 32 bits and are rounded once, so
 // that a result depends on its inputs alone.  (The layer's own combine, combine.hip, adds in bf16 as the reference does.)
 //
-// Three of the four work by token: a token's row is read or written once whatever k is.  They go by a list of every token's
-// slots, which token_slots_kernel inverts the table into.
+// All but permute work by token: a token's row is read or written once whatever k is.  They go by a list of every token's slots,
+// which token_slots_kernel inverts the table into.
 #include <type_traits>
 
 #include "rows.hpp"
@@ -30,28 +30,31 @@ __global__ __launch_bounds__(1024) void token_slots_kernel(const int32_t* __rest
   const int nt = (int)(T - t0 < range ? T - t0 : range), w = 1 + k;
   for (int i = threadIdx.x; i < nt; i += 1024) s_list[i * w] = 0;
   __syncthreads();
+  // (unsigned: whatever lies outside of the range, negative ids too, is far above it)
+  auto mine = [&](int id) { return (uint32_t)id - (uint32_t)t0 < (uint32_t)nt; };
   auto take = [&](int64_t s, int id) {
-    const int64_t t = (int64_t)id - t0;
-    if (t >= 0 && t < nt) {
-      const int p = atomicAdd(&s_list[(int)t * w], 1);
-      if (p < k) s_list[(int)t * w + 1 + p] = (int)s;
+    if (mine(id)) {
+      const int t = (int)((uint32_t)id - (uint32_t)t0), p = atomicAdd(&s_list[t * w], 1);
+      if (p < k) s_list[t * w + 1 + p] = (int)s;
     }
   };
   const int64_t n4 = ((uintptr_t)tp2id & 15) == 0 ? S / 4 : 0;
-  constexpr int U = 4;
+  constexpr int U = 8;
   for (int64_t i0 = threadIdx.x; i0 < n4; i0 += 1024 * U) {
     int4 d[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      d[u] = make_int4(-1, -1, -1, -1);
       if (i0 + 1024 * u < n4) d[u] = ((const int4*)tp2id)[i0 + 1024 * u];
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t i = i0 + 1024 * u;
-      if (i < n4) {
-        take(4 * i, d[u].x);
-        take(4 * i + 1, d[u].y);
-        take(4 * i + 2, d[u].z);
-        take(4 * i + 3, d[u].w);
+      const int64_t i = 4 * (i0 + 1024 * u);
+      if (mine(d[u].x) | mine(d[u].y) | mine(d[u].z) | mine(d[u].w)) {
+        take(i, d[u].x);
+        take(i + 1, d[u].y);
+        take(i + 2, d[u].z);
+        take(i + 3, d[u].w);
       }
     }
   }
@@ -78,14 +81,19 @@ __global__ __launch_bounds__(1024) void token_slots_kernel(const int32_t* __rest
 
 typedef uint32_t bytes16 __attribute__((ext_vector_type(4), aligned(1)));
 
-// TPR threads per slot (a whole number of waves, so that everything about a slot is uniform); rows of any number of bytes.
+// TPR threads per row or part of a row (a whole number of waves, so that everything about a row is uniform).
 template <int TPR>
 __device__ __forceinline__ int64_t row_of_group() {
   return (int64_t)blockIdx.x * (256 / TPR) + __builtin_amdgcn_readfirstlane((int)(threadIdx.x / TPR));
 }
+// Up to four pieces of 16 bytes per thread are asked for before the first is written, and written past the caches: the x rows come
+// as often as they have slots, from the Infinity Cache if the output leaves them there.  T = 8192 tokens of 14 KB in 8 of 98048
+// slots, x in no cache, us: 306; a piece at a time 319, with ordinary stores 359, a workgroup per 512 pieces 361; token by token,
+// each row read once and written to 8 places, 301 with the list of the slots that this takes.  The writes alone, in order: 205.
 template <int TPR>
 __global__ __launch_bounds__(256) void permute_kernel(const uint8_t* __restrict__ x, const int32_t* __restrict__ tp2id, int64_t S,
                                                       int64_t T, int64_t row_bytes, uint8_t* __restrict__ out) {
+  constexpr int U = 4;
   const int lane = threadIdx.x % TPR;
   const int64_t whole = row_bytes / 16;
   for (int64_t s = row_of_group<TPR>(); s < S; s += (int64_t)gridDim.x * (256 / TPR)) {
@@ -93,10 +101,16 @@ __global__ __launch_bounds__(256) void permute_kernel(const uint8_t* __restrict_
     const bool token = id >= 0 && id < T;
     const uint8_t* src = x + (token ? id : 0) * row_bytes;
     uint8_t* dst = out + s * row_bytes;
-    for (int64_t c = lane; c < whole; c += TPR) {
-      bytes16 v = {0, 0, 0, 0};
-      if (token) v = *(const bytes16*)(src + 16 * c);
-      __builtin_nontemporal_store(v, (bytes16*)(dst + 16 * c));
+    for (int64_t c0 = lane; c0 < whole; c0 += TPR * U) {
+      bytes16 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        v[u] = bytes16{0, 0, 0, 0};
+        if (token && c0 + TPR * u < whole) v[u] = *(const bytes16*)(src + 16 * (c0 + TPR * u));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c0 + TPR * u < whole) __builtin_nontemporal_store(v[u], (bytes16*)(dst + 16 * (c0 + TPR * u)));
     }
     for (int64_t b = 16 * whole + lane; b < row_bytes; b += TPR) dst[b] = token ? src[b] : (uint8_t)0;
   }
@@ -139,14 +153,14 @@ __device__ __forceinline__ void load_group(const SlotTables& a, const int32_t* l
     }
 }
 
-// TPR threads per token.
+// TPR threads per token; where the tokens are few, gridDim.y groups of them side by side along the row.
 template <int DT, int TPR>
 __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __restrict__ y, const SlotTables a, int64_t T,
                                                              int64_t H, uint8_t* __restrict__ out) {
   typedef Elem<DT> EL;
   typedef typename EL::raw raw;
   constexpr int N = EL::N;
-  const int lane = threadIdx.x % TPR;
+  const int lane = blockIdx.y * TPR + threadIdx.x % TPR, step = gridDim.y * TPR;
   const int64_t whole = H / N * N;
   for (int64_t t = row_of_group<TPR>(); t < T; t += (int64_t)gridDim.x * (256 / TPR)) {
     const int32_t* list = a.lists + t * (1 + a.k);
@@ -155,7 +169,7 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
     const float start = cut ? __builtin_nanf("") : 0.f;
     SlotGroup g;
     load_group(a, list, t, 0, n, g);
-    for (int64_t c = (int64_t)lane * N; c < whole; c += TPR * N) {
+    for (int64_t c = (int64_t)lane * N; c < whole; c += (int64_t)step * N) {
       float acc[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = start;
@@ -176,7 +190,7 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
       }
       store_piece<DT>(out + (t * H + c) * EL::SIZE, pack<DT>(acc));
     }
-    for (int64_t c = whole + lane; c < H; c += TPR) {
+    for (int64_t c = whole + lane; c < H; c += step) {
       float acc = start;
       for (int j0 = 0; j0 < n; j0 += 8) {
         if (n > 8) load_group(a, list, t, j0, n, g);
@@ -192,8 +206,9 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
 // ---- combine, backward --------------------------------------------------------------------------------------------
 
 // Jobs [0, T) take a token each: its row of dout is read once per eight slots, eight rows of y and dy beside it.  The next
-// ceil(S / PAD_SLOTS) write the rows of slots that no token's list holds, the last one the rows of da behind T.
-constexpr int PAD_SLOTS = 64;
+// ceil(S / PAD_SLOTS) write the rows of slots that no token's list holds (few slots each: padding comes in runs, at an expert's
+// end; with 64 the kernel took 480 us instead of 465 at T = 8192, 98048 slots of 14 KB), the last one the rows of da behind T.
+constexpr int PAD_SLOTS = 8;
 template <int DT>
 __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* __restrict__ dout, const uint8_t* __restrict__ y,
                                                                  const SlotTables a, const int32_t* __restrict__ tp2id,
@@ -212,16 +227,19 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
       continue;
     }
     if (job >= T) {
-      const int64_t s0 = (job - T) * PAD_SLOTS, s1 = s0 + PAD_SLOTS < S ? s0 + PAD_SLOTS : S;
-      for (int64_t s = s0; s < s1; ++s) {
-        const int64_t id = tp2id[s];
-        const int e = a.b2e[(uint32_t)s / a.B];
-        const bool token = id >= 0 && id < T && e >= 0 && e < a.E;
-        const bool cut = token && a.lists[id * (1 + a.k)] > a.k;
-        if (token && !cut) continue;
+      const int64_t s0 = (job - T) * PAD_SLOTS, mine = s0 + (tid & 63);
+      const bool in = mine < S && mine < s0 + PAD_SLOTS;
+      const int64_t id = in ? tp2id[mine] : 0;
+      const int e = in ? a.b2e[(uint32_t)mine / a.B] : 0;
+      const bool token = id >= 0 && id < T && e >= 0 && e < a.E;
+      const bool cut = in && token && a.lists[id * (1 + a.k)] > a.k;
+      const uint64_t nans = __ballot(cut);
+      for (uint64_t left = __ballot(in && (!token || cut)); left; left &= left - 1) {
+        const int i = __builtin_ctzll(left);
+        const int64_t s = s0 + i;
         float v[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = cut ? __builtin_nanf("") : 0.f;
+        for (int q = 0; q < N; ++q) v[q] = (nans >> i) & 1 ? __builtin_nanf("") : 0.f;
         for (int64_t c = (int64_t)tid * N; c < whole; c += 256 * N) store_piece<DT>(dy + (s * H + c) * EL::SIZE, pack<DT>(v));
         for (int64_t c = whole + tid; c < H; c += 256) ((raw*)dy)[s * H + c] = f32_to_elem<DT>(v[0]);
       }
@@ -294,35 +312,32 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
 
 // (a launch holds fewer than 2^32 threads; what lies beyond a million workgroups is a second round of the same ones)
 static unsigned grid_of(int64_t jobs) { return (unsigned)(jobs < ((int64_t)1 << 20) ? jobs : (int64_t)1 << 20); }
-static int check_tables(const SlotTables& a, int64_t T, int64_t T1) {
-  if (!a.b2e) return MOE_OK;
-  if (!a.aff || (a.aff_dtype != MOE_DT_BF16 && a.aff_dtype != MOE_DT_FP32)) return MOE_E_BAD_ARG;
-  if (a.E <= 0 || a.E >= (int64_t)1 << 31 || T1 < T) return MOE_E_BAD_SHAPE;
-  return MOE_OK;
-}
 
 }  // namespace moe
 
 using namespace moe;
 
+static int launch_token_slots(const int32_t* tp2id, int64_t S, int64_t T, int k, int32_t* lists, hipStream_t s) {
+  if (T == 0) return MOE_OK;
+  int64_t range = (T + 255) / 256;  // a workgroup per CU
+  if (range > SLOTS_LDS_WORDS / (1 + k)) range = SLOTS_LDS_WORDS / (1 + k);
+  hipLaunchKernelGGL(token_slots_kernel, dim3((unsigned)((T + range - 1) / range)), dim3(1024), 0, s, tp2id, S, T, k, (int)range,
+                     lists);
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
 extern "C" int moe_token_slots(const int32_t* token_position_to_id, int64_t S, int64_t T, int top_k, int32_t* token_slots,
                                void* stream) {
   if ((!token_position_to_id && S > 0) || !token_slots || S < 0 || T < 0) return MOE_E_BAD_ARG;
   if (top_k < 1 || top_k > SLOTS_MAX_K || S >= (int64_t)1 << 31 || T >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
-  if (T == 0) return MOE_OK;
-  const int most = SLOTS_LDS_WORDS / (1 + top_k);
-  int64_t range = (T + 255) / 256;  // a workgroup per CU
-  if (range > most) range = most;
-  hipLaunchKernelGGL(token_slots_kernel, dim3((unsigned)((T + range - 1) / range)), dim3(1024), 0, (hipStream_t)stream,
-                     token_position_to_id, S, T, top_k, (int)range, token_slots);
-  MOE_CHECK_LAUNCH();
-  return MOE_OK;
+  return launch_token_slots(token_position_to_id, S, T, top_k, token_slots, (hipStream_t)stream);
 }
 
 extern "C" int moe_permute_tokens(const void* x, const int32_t* token_position_to_id, int64_t S, int64_t T, int64_t row_bytes,
                                   void* out, void* stream) {
   if (!x || !token_position_to_id || !out || S < 0 || T < 0 || row_bytes < 0) return MOE_E_BAD_ARG;
-  if (S >= (int64_t)1 << 31 || T >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
+  if (S >= (int64_t)1 << 31 || T >= (int64_t)1 << 31 || row_bytes >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
   if (S == 0 || row_bytes == 0) return MOE_OK;
   const hipStream_t s = (hipStream_t)stream;
   if (row_bytes > 2048)
@@ -337,31 +352,48 @@ extern "C" int moe_permute_tokens(const void* x, const int32_t* token_position_t
 
 template <int DT>
 static void launch_combine_tokens(const void* y, const SlotTables& a, int64_t T, int64_t H, void* out, hipStream_t s) {
-  if (H * Elem<DT>::SIZE > 2048)
-    hipLaunchKernelGGL((combine_tokens_kernel<DT, 256>), dim3(grid_of(T)), dim3(256), 0, s, (const uint8_t*)y, a, T, H,
-                       (uint8_t*)out);
+  // a workgroup per token, or a wave where rows are short; few tokens (decode): several per token, a piece per thread
+  const bool wide = H * Elem<DT>::SIZE > 2048;
+  const int64_t groups = wide ? T : (T + 3) / 4;
+  int64_t parts = 1;
+  if (wide && groups < 512) {
+    parts = (H + 256 * Elem<DT>::N - 1) / (256 * Elem<DT>::N);
+    if (parts > 512 / groups) parts = 512 / groups;
+  }
+  const dim3 grid(grid_of(groups), (unsigned)parts);
+  if (wide)
+    hipLaunchKernelGGL((combine_tokens_kernel<DT, 256>), grid, dim3(256), 0, s, (const uint8_t*)y, a, T, H, (uint8_t*)out);
   else
-    hipLaunchKernelGGL((combine_tokens_kernel<DT, 64>), dim3(grid_of((T + 3) / 4)), dim3(256), 0, s, (const uint8_t*)y, a, T,
-                       H, (uint8_t*)out);
+    hipLaunchKernelGGL((combine_tokens_kernel<DT, 64>), grid, dim3(256), 0, s, (const uint8_t*)y, a, T, H, (uint8_t*)out);
+}
+
+// What the calls that go by lists check alike, and the list itself where it is asked for.
+static int begin_by_list(const SlotTables& a, int64_t T, int64_t T1, const int32_t* tp2id, int build, hipStream_t s) {
+  if (!a.lists || a.S < 0 || T < 0 || (build && !tp2id && a.S > 0)) return MOE_E_BAD_ARG;
+  if (a.k < 1 || a.k > SLOTS_MAX_K || T >= (int64_t)1 << 31 || a.S >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
+  if (a.b2e) {
+    if (!a.aff || (a.aff_dtype != MOE_DT_BF16 && a.aff_dtype != MOE_DT_FP32)) return MOE_E_BAD_ARG;
+    if (a.E <= 0 || a.E >= (int64_t)1 << 31 || T1 < T) return MOE_E_BAD_SHAPE;
+  }
+  return build ? launch_token_slots(tp2id, a.S, T, a.k, (int32_t*)a.lists, s) : MOE_OK;
 }
 
 extern "C" int moe_combine_tokens(const void* y, int dtype, const void* expert_affinities, int aff_dtype, int64_t T1, int64_t E,
-                                  const int32_t* block_to_expert, int64_t B, int64_t N, const int32_t* token_slots, int top_k,
-                                  int64_t S, int64_t T, int64_t H, void* out, void* stream) {
-  if (!y || !token_slots || !out || S < 0 || T < 0 || H < 0) return MOE_E_BAD_ARG;
+                                  const int32_t* token_position_to_id, const int32_t* block_to_expert, int64_t B, int64_t N,
+                                  int32_t* token_slots, int top_k, int build_token_slots, int64_t S, int64_t T, int64_t H, void* out,
+                                  void* stream) {
+  if (!y || !out || H < 0 || dtype < MOE_DT_BF16 || dtype > MOE_DT_FP32) return MOE_E_BAD_ARG;
   if ((expert_affinities != nullptr) != (block_to_expert != nullptr)) return MOE_E_BAD_ARG;
-  if (top_k < 1 || top_k > SLOTS_MAX_K || T >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
-  if (S >= (int64_t)1 << 31 || (block_to_expert && (B <= 0 || N < 0 || S != B * N))) return MOE_E_BAD_SHAPE;
+  if (block_to_expert && (B <= 0 || N < 0 || B >= (int64_t)1 << 31 || N >= (int64_t)1 << 31 || S != B * N)) return MOE_E_BAD_SHAPE;
   const SlotTables a{token_slots, block_to_expert, expert_affinities, aff_dtype, top_k, (uint32_t)B, (uint32_t)N, E, S};
-  const int rc = check_tables(a, T, T1);
+  const hipStream_t s = (hipStream_t)stream;
+  const int rc = begin_by_list(a, T, T1, token_position_to_id, build_token_slots, s);
   if (rc != MOE_OK) return rc;
   if (T == 0 || H == 0) return MOE_OK;
-  const hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case MOE_DT_BF16: launch_combine_tokens<MOE_DT_BF16>(y, a, T, H, out, s); break;
     case MOE_DT_FP16: launch_combine_tokens<MOE_DT_FP16>(y, a, T, H, out, s); break;
-    case MOE_DT_FP32: launch_combine_tokens<MOE_DT_FP32>(y, a, T, H, out, s); break;
-    default: return MOE_E_BAD_ARG;
+    default: launch_combine_tokens<MOE_DT_FP32>(y, a, T, H, out, s); break;
   }
   MOE_CHECK_LAUNCH();
   return MOE_OK;
@@ -369,27 +401,26 @@ extern "C" int moe_combine_tokens(const void* y, int dtype, const void* expert_a
 
 extern "C" int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtype, const void* expert_affinities, int aff_dtype,
                                       int64_t T1, int64_t E, const int32_t* token_position_to_id, const int32_t* block_to_expert,
-                                      int64_t B, int64_t N, const int32_t* token_slots, int top_k, int64_t T, int64_t H,
-                                      void* d_y, float* d_affinities, void* stream) {
-  if (!d_out || !y || !expert_affinities || !token_position_to_id || !block_to_expert || !token_slots || !d_y ||
-      !d_affinities || T < 0 || H < 0 || N < 0)
+                                      int64_t B, int64_t N, int32_t* token_slots, int top_k, int build_token_slots, int64_t T,
+                                      int64_t H, void* d_y, float* d_affinities, void* stream) {
+  if (!d_out || !y || !expert_affinities || !token_position_to_id || !block_to_expert || !d_y || !d_affinities || H < 0 || N < 0 ||
+      dtype < MOE_DT_BF16 || dtype > MOE_DT_FP32)
     return MOE_E_BAD_ARG;
-  if (top_k < 1 || top_k > SLOTS_MAX_K || T >= (int64_t)1 << 31 || B <= 0 || B * N >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
+  if (B <= 0 || B >= (int64_t)1 << 31 || N >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
   const int64_t S = B * N;
   const SlotTables a{token_slots, block_to_expert, expert_affinities, aff_dtype, top_k, (uint32_t)B, (uint32_t)N, E, S};
-  const int rc = check_tables(a, T, T1);
+  const hipStream_t s = (hipStream_t)stream;
+  const int rc = begin_by_list(a, T, T1, token_position_to_id, build_token_slots, s);
   if (rc != MOE_OK) return rc;
   const unsigned grid = grid_of(T + (S + PAD_SLOTS - 1) / PAD_SLOTS + 1);
-  const hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
-#define MOE_BWD(DT)                                                                                                           \
-  hipLaunchKernelGGL(combine_tokens_bwd_kernel<DT>, dim3(grid), dim3(256), 0, s, (const uint8_t*)d_out,               \
-                     (const uint8_t*)y, a, token_position_to_id, S, T, T1, H, (uint8_t*)d_y, d_affinities)
+#define MOE_BWD(DT)                                                                                                             \
+  hipLaunchKernelGGL(combine_tokens_bwd_kernel<DT>, dim3(grid), dim3(256), 0, s, (const uint8_t*)d_out, (const uint8_t*)y, a,   \
+                     token_position_to_id, S, T, T1, H, (uint8_t*)d_y, d_affinities)
     case MOE_DT_BF16: MOE_BWD(MOE_DT_BF16); break;
     case MOE_DT_FP16: MOE_BWD(MOE_DT_FP16); break;
-    case MOE_DT_FP32: MOE_BWD(MOE_DT_FP32); break;
+    default: MOE_BWD(MOE_DT_FP32); break;
 #undef MOE_BWD
-    default: return MOE_E_BAD_ARG;
   }
   MOE_CHECK_LAUNCH();
   return MOE_OK;

@@ -195,10 +195,10 @@ def lib():
     for name, args in {
         "moe_token_slots": [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p],
         "moe_permute_tokens": [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p],
-        "moe_combine_tokens": [c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
-                               c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p],
+        "moe_combine_tokens": [c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                               c_void_p, c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p],
         "moe_combine_tokens_bwd": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p,
-                                   c_int64, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+                                   c_int64, c_int64, c_void_p, c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
         "moe_glu_checkpoint": [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p,
                                c_void_p, c_void_p, c_void_p],
         "moe_pack_gate_up_checkpoint": [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p,

@@ -43,13 +43,18 @@ def _same_device(*tensors):
 
 
 def _slots(tp2id, n_tokens, top_k, token_slots):
+    """The list to go by, and whether the call has yet to make it."""
+    if not 1 <= top_k <= 64:
+        kernel_assert(False, f"top_k must be in [1, 64] but got {top_k}")
+    if n_tokens < 0:
+        kernel_assert(False, f"n_tokens must not be negative but got {n_tokens}")
     if token_slots is None:
-        return build_token_slots(tp2id, n_tokens, top_k)
+        return torch.empty((n_tokens, 1 + top_k), dtype=torch.int32, device=tp2id.device), 1
     token_slots = nv.require_device_tensor(token_slots, "token_slots")
     if token_slots.dtype != torch.int32 or token_slots.shape != (n_tokens, 1 + top_k):
         kernel_assert(False, f"token_slots must be int32 [{n_tokens}, {1 + top_k}] but got {token_slots.dtype} "
                              f"{tuple(token_slots.shape)}")
-    return token_slots
+    return token_slots, 0
 
 
 def _routing(expert_affinities_masked, block_to_expert, block_size, tp2id, n_tokens):
@@ -75,12 +80,8 @@ def build_token_slots(token_position_to_id: torch.Tensor, n_tokens: int, top_k: 
     times (at most 64) comes out as NaN wherever it is summed; ``check=True`` synchronises and raises instead."""
     t = _table(token_position_to_id)
     n_tokens, top_k = int(n_tokens), int(top_k)
-    if not 1 <= top_k <= 64:
-        kernel_assert(False, f"top_k must be in [1, 64] but got {top_k}")
-    if n_tokens < 0:
-        kernel_assert(False, f"n_tokens must not be negative but got {n_tokens}")
     dev = t.device
-    out = torch.empty((n_tokens, 1 + top_k), dtype=torch.int32, device=dev)
+    out, _ = _slots(t, n_tokens, top_k, None)
     if n_tokens == 0:
         return out
     with nv.on_device(dev):
@@ -119,14 +120,14 @@ def permute_tokens_bwd(d_permuted: torch.Tensor, token_position_to_id: torch.Ten
     n_tokens, top_k = int(n_tokens), int(top_k)
     dev = _same_device(d, t)
     dt = nv.dtype_code(d, "d_permuted")
-    slots = _slots(t, n_tokens, top_k, token_slots)
+    slots, build = _slots(t, n_tokens, top_k, token_slots)
     _same_device(d, slots)
     out = torch.empty((n_tokens, d.shape[1]), dtype=d.dtype, device=dev)
     if out.numel() == 0 or t.numel() == 0:
         return out.zero_()
     with nv.on_device(dev):
-        rc = nv.lib().moe_combine_tokens(d.data_ptr(), dt, None, 0, 0, 0, None, 0, 0, slots.data_ptr(), top_k, t.numel(), n_tokens,
-                                         d.shape[1], out.data_ptr(), nv.stream_ptr(dev))
+        rc = nv.lib().moe_combine_tokens(d.data_ptr(), dt, None, 0, 0, 0, t.data_ptr(), None, 0, 0, slots.data_ptr(), top_k, build,
+                                         t.numel(), n_tokens, d.shape[1], out.data_ptr(), nv.stream_ptr(dev))
     nv.check(rc, "permute_tokens_bwd")
     return out
 
@@ -143,15 +144,15 @@ def combine_tokens(permuted: torch.Tensor, expert_affinities_masked: torch.Tenso
     aff, b2e, B = _routing(expert_affinities_masked, block_to_expert, block_size, t, n_tokens)
     dev = _same_device(y, t, aff, b2e)
     dt = nv.dtype_code(y, "permuted")
-    slots = _slots(t, n_tokens, top_k, token_slots)
+    slots, build = _slots(t, n_tokens, top_k, token_slots)
     _same_device(y, slots)
     out = torch.empty((n_tokens, y.shape[1]), dtype=y.dtype, device=dev)
     if out.numel() == 0 or t.numel() == 0:
         return out.zero_()
     with nv.on_device(dev):
         rc = nv.lib().moe_combine_tokens(y.data_ptr(), dt, aff.data_ptr(), nv.dtype_code(aff, "expert_affinities_masked"),
-                                         aff.shape[0], aff.shape[1], b2e.data_ptr(), B, b2e.numel(), slots.data_ptr(), top_k,
-                                         t.numel(), n_tokens, y.shape[1], out.data_ptr(), nv.stream_ptr(dev))
+                                         aff.shape[0], aff.shape[1], t.data_ptr(), b2e.data_ptr(), B, b2e.numel(), slots.data_ptr(),
+                                         top_k, build, t.numel(), n_tokens, y.shape[1], out.data_ptr(), nv.stream_ptr(dev))
     nv.check(rc, "combine_tokens")
     return out
 
@@ -171,7 +172,7 @@ def combine_tokens_bwd(d_output: torch.Tensor, permuted: torch.Tensor, expert_af
     aff, b2e, B = _routing(expert_affinities_masked, block_to_expert, block_size, t, n_tokens)
     dev = _same_device(y, t, d, aff, b2e)
     dt = nv.dtype_code(y, "permuted")
-    slots = _slots(t, n_tokens, top_k, token_slots)
+    slots, build = _slots(t, n_tokens, top_k, token_slots)
     _same_device(y, slots)
     d_y = torch.empty_like(y)
     d_aff = torch.empty(aff.shape, dtype=torch.float32, device=dev)
@@ -180,7 +181,7 @@ def combine_tokens_bwd(d_output: torch.Tensor, permuted: torch.Tensor, expert_af
     with nv.on_device(dev):
         rc = nv.lib().moe_combine_tokens_bwd(d.data_ptr(), y.data_ptr(), dt, aff.data_ptr(),
                                              nv.dtype_code(aff, "expert_affinities_masked"), aff.shape[0], aff.shape[1], t.data_ptr(),
-                                             b2e.data_ptr(), B, b2e.numel(), slots.data_ptr(), top_k, n_tokens, y.shape[1],
+                                             b2e.data_ptr(), B, b2e.numel(), slots.data_ptr(), top_k, build, n_tokens, y.shape[1],
                                              d_y.data_ptr(), d_aff.data_ptr(), nv.stream_ptr(dev))
     nv.check(rc, "combine_tokens_bwd")
     return d_y, d_aff

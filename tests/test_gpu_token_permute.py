@@ -65,10 +65,35 @@ def test_permute_moves_any_bytes():
 
     rng = np.random.default_rng(0)
     tp2id, _, _ = table(rng, 50, 8, 2, 16)
-    for width in (1, 15, 16, 77, 4100):
+    for width in (1, 15, 16, 77, 1030, 1600, 4100, 8190, 8192, 20001):
         x = rng.integers(0, 256, (50, width), dtype=np.uint8)
         got = permute_tokens(torch.from_numpy(x).cuda(), tensor(tp2id, "int32"))
         assert np.array_equal(got.cpu().numpy(), ot.permute(x, tp2id)), width
+
+
+@pytest.mark.parametrize("width,dtype", [(7168, "bfloat16"), (1030, "bfloat16"), (515, "float32"), (530, "bfloat16"), (100, "bfloat16"),
+                                         (9001, "float32")])
+def test_large_permutes(width, dtype):
+    """Tables of 80 MB: tokens without slots, tokens with hundreds; rows longer than a round of a workgroup."""
+    import torch
+    from nkilib.core.moe.token_permute import permute_tokens
+
+    rng = np.random.default_rng(width)
+    es = 2 if dtype == "bfloat16" else 4
+    S, T = (80 << 20) // (width * es), 300
+    ids = rng.integers(-1, T + 2, S).astype(np.int32)
+    ids[ids % 3 == 0] = -1
+    ids[ids == 5] = T
+    ids[rng.permutation(S)[:14]] = 5  # (14 slots; the others have hundreds, or none)
+    x = tensor(rng.standard_normal((T, width)), dtype)
+    tp = torch.from_numpy(ids).cuda()
+    ok = (tp >= 0) & (tp < T)
+    want = torch.where(ok[:, None], x[tp.long().clamp(0, T - 1)], torch.zeros((), dtype=x.dtype, device="cuda"))
+    assert torch.equal(permute_tokens(x, tp), want)
+    T = S // 4
+    tp = torch.from_numpy(rng.permutation(np.repeat(rng.permutation(T), 4).astype(np.int32))).cuda()
+    x = torch.randn((T, width), device="cuda").to(x.dtype)
+    assert torch.equal(permute_tokens(x, tp), x[tp.long()])
 
 
 @pytest.mark.parametrize("shape", SHAPES)

@@ -27,38 +27,39 @@ def test_token_slots_refusals(L):
 
 
 def test_permute_refusals(L):
-    assert L.moe_permute_tokens(None, P, 4, 4, 16, P, None) == BAD_ARG
-    assert L.moe_permute_tokens(P, P, 4, 4, -1, P, None) == BAD_ARG
-    assert L.moe_permute_tokens(P, P, 2**31, 4, 16, P, None) == BAD_SHAPE
-    assert L.moe_permute_tokens(P, P, 0, 4, 16, P, None) == 0
-    assert L.moe_permute_tokens(P, P, 4, 4, 0, P, None) == 0
+    call = lambda x=P, t=P, S=4, T=4, n=16, out=P: L.moe_permute_tokens(x, t, S, T, n, out, None)
+    assert call(x=None) == BAD_ARG and call(t=None) == BAD_ARG and call(out=None) == BAD_ARG and call(n=-1) == BAD_ARG
+    assert call(S=2**31) == BAD_SHAPE and call(T=2**31) == BAD_SHAPE and call(n=2**31) == BAD_SHAPE
+    assert call(S=0) == 0 and call(n=0) == 0
 
 
 def _combine(L, **kw):
-    a = dict(y=P, dtype=0, aff=P, aff_dtype=0, T1=5, E=3, b2e=P, B=4, N=2, slots=P, k=2, S=8, T=0, H=16, out=P)
+    a = dict(y=P, dtype=0, aff=P, aff_dtype=0, T1=5, E=3, tp=P, b2e=P, B=4, N=2, slots=P, k=2, build=0, S=8, T=0, H=16, out=P)
     a.update(kw)
-    return L.moe_combine_tokens(a["y"], a["dtype"], a["aff"], a["aff_dtype"], a["T1"], a["E"], a["b2e"], a["B"], a["N"],
-                                a["slots"], a["k"], a["S"], a["T"], a["H"], a["out"], None)
+    return L.moe_combine_tokens(a["y"], a["dtype"], a["aff"], a["aff_dtype"], a["T1"], a["E"], a["tp"], a["b2e"], a["B"], a["N"],
+                                a["slots"], a["k"], a["build"], a["S"], a["T"], a["H"], a["out"], None)
 
 
 def test_combine_refusals(L):
-    assert _combine(L) == 0  # (no tokens)
+    assert _combine(L) == 0 and _combine(L, build=1) == 0  # (no tokens)
     assert _combine(L, T=4, dtype=7) == BAD_ARG and _combine(L, T=4, dtype=3) == BAD_ARG
     assert _combine(L, aff=None) == BAD_ARG and _combine(L, b2e=None) == BAD_ARG
     assert _combine(L, slots=None) == BAD_ARG and _combine(L, y=None) == BAD_ARG and _combine(L, out=None) == BAD_ARG
+    assert _combine(L, tp=None, build=1) == BAD_ARG and _combine(L, tp=None) == 0
     assert _combine(L, aff_dtype=1) == BAD_ARG  # fp16 affinities
     assert _combine(L, T=6) == BAD_SHAPE  # fewer rows of affinities than tokens
     assert _combine(L, E=0) == BAD_SHAPE
     assert _combine(L, k=0) == BAD_SHAPE and _combine(L, k=65) == BAD_SHAPE
     assert _combine(L, B=0) == BAD_SHAPE and _combine(L, S=9) == BAD_SHAPE and _combine(L, S=2**31, B=2**30) == BAD_SHAPE
+    assert _combine(L, B=2**33, N=2**33) == BAD_SHAPE and _combine(L, T=-1) == BAD_ARG
 
 
 def test_combine_bwd_refusals(L):
     def call(**kw):
-        a = dict(d=P, y=P, dtype=0, aff=P, aff_dtype=0, T1=5, E=3, tp=P, b2e=P, B=4, N=2, slots=P, k=2, T=4, H=16, dy=P, da=P)
+        a = dict(d=P, y=P, dtype=0, aff=P, aff_dtype=0, T1=5, E=3, tp=P, b2e=P, B=4, N=2, slots=P, k=2, build=1, T=4, H=16, dy=P, da=P)
         a.update(kw)
-        return L.moe_combine_tokens_bwd(a["d"], a["y"], a["dtype"], a["aff"], a["aff_dtype"], a["T1"], a["E"], a["tp"],
-                                        a["b2e"], a["B"], a["N"], a["slots"], a["k"], a["T"], a["H"], a["dy"], a["da"], None)
+        return L.moe_combine_tokens_bwd(a["d"], a["y"], a["dtype"], a["aff"], a["aff_dtype"], a["T1"], a["E"], a["tp"], a["b2e"],
+                                        a["B"], a["N"], a["slots"], a["k"], a["build"], a["T"], a["H"], a["dy"], a["da"], None)
 
     for name in ("d", "y", "aff", "tp", "b2e", "slots", "dy", "da"):
         assert call(**{name: None}) == BAD_ARG, name
