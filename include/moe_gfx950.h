@@ -376,8 +376,8 @@ int moe_prepare_kmajor_weights(const moe_bwmm_args* args, void* gate_up_kmajor, 
  *
  * moe_token_slots: the table's inverse, int32 [T, 1 + top_k]: how many slots token t has, then the slots, ascending, then -1.
  * top_k <= 64.  A token that the table lists more than top_k times keeps the true count: the calls below give NaN for it (its
- * row, its slots' rows, its affinities).  They take the list in token_slots, or, with build_token_slots != 0, make it there
- * first from token_position_to_id (only read then by moe_combine_tokens, nullable otherwise).
+ * row, its slots' rows, its affinities).  They take the list in token_slots, or, with build_token_slots != 0, use that as scratch
+ * memory and go by token_position_to_id (only read then by moe_combine_tokens, nullable otherwise).
  *
  * moe_permute_tokens: out[s] = x[token of s], zero rows for padding; any element type (rows of row_bytes < 2^31 bytes).
  *

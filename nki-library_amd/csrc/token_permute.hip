@@ -133,10 +133,11 @@ struct SlotGroup {
   float w[8];
   int e[8];
 };
-__device__ __forceinline__ void load_group(const SlotTables& a, const int32_t* list, int64_t t, int j0, int n, SlotGroup& g) {
+template <class SLOT>
+__device__ __forceinline__ void load_group(const SlotTables& a, SLOT&& slot, int64_t t, int j0, int n, SlotGroup& g) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    g.row[j] = j0 + j < n ? list[1 + j0 + j] : -1;
+    g.row[j] = j0 + j < n ? slot(j0 + j) : -1;
     if (g.row[j] >= a.S) g.row[j] = -1;
     g.w[j] = 1.f;
     g.e[j] = 0;
@@ -153,28 +154,66 @@ __device__ __forceinline__ void load_group(const SlotTables& a, const int32_t* l
     }
 }
 
-// TPR threads per token; where the tokens are few, gridDim.y groups of them side by side along the row.
-template <int DT, int TPR>
-__global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __restrict__ y, const SlotTables a, int64_t T,
-                                                             int64_t H, uint8_t* __restrict__ out) {
+// TPR threads per token; where the tokens are few, gridDim.y groups of them side by side along the row.  tp2id: the table
+// itself, of at most COMBINE_SCAN_SLOTS slots for tokens of a single round of the launch, that every group looks its token up in:
+// a launch less, which at such sizes takes as long as the sums (8 tokens, 64 slots of 14 KB: kernels 6.1 + 3.0 us by the list, 6.8 so; a call 17.6 and
+// 13.0).  Null: by the lists.
+constexpr int64_t COMBINE_SCAN_SLOTS = 2048;
+template <int DT, int TPR, bool SCAN>
+__global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __restrict__ y, const SlotTables a,
+                                                             const int32_t* __restrict__ tp2id, int64_t T, int64_t H,
+                                                             uint8_t* __restrict__ out) {
   typedef Elem<DT> EL;
   typedef typename EL::raw raw;
   constexpr int N = EL::N;
+  __shared__ int s_found[SCAN ? 256 / TPR : 1][1 + SLOTS_MAX_K], s_sorted[SCAN ? 256 / TPR : 1][SLOTS_MAX_K];
   const int lane = blockIdx.y * TPR + threadIdx.x % TPR, step = gridDim.y * TPR;
-  const int64_t whole = H / N * N;
+  if constexpr (SCAN) {
+    int *found = s_found[threadIdx.x / TPR], *sorted = s_sorted[threadIdx.x / TPR];
+    const int i0 = threadIdx.x % TPR, S = (int)a.S;
+    const int t = (int)row_of_group<TPR>();
+    if (i0 == 0) found[0] = 0;
+    __syncthreads();
+    for (int s0 = i0; s0 < S; s0 += 8 * TPR) {
+      int id[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) id[u] = s0 + TPR * u < S ? tp2id[s0 + TPR * u] : -1;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (id[u] == t) {
+          const int p = atomicAdd(&found[0], 1);
+          if (p < a.k) found[1 + p] = s0 + TPR * u;
+        }
+    }
+    __syncthreads();
+    const int held = found[0] < a.k ? found[0] : a.k;
+    for (int i = i0; i < held; i += TPR) {
+      int rank = 0;
+      for (int o = 0; o < held; ++o) rank += found[1 + o] < found[1 + i];
+      sorted[rank] = found[1 + i];
+    }
+    __syncthreads();
+  }
   for (int64_t t = row_of_group<TPR>(); t < T; t += (int64_t)gridDim.x * (256 / TPR)) {
-    const int32_t* list = a.lists + t * (1 + a.k);
-    const bool cut = list[0] > a.k;  // the table lists the token more often than its caller said: no sum of a part
-    const int n = cut ? 0 : list[0];
+    const int32_t* list = SCAN ? nullptr : a.lists + t * (1 + a.k);
+    auto slot = [&](int j) {
+      if constexpr (SCAN) return __builtin_amdgcn_readfirstlane(s_sorted[threadIdx.x / TPR][j]);
+      else return list[1 + j];
+    };
+    const int count = SCAN ? __builtin_amdgcn_readfirstlane(s_found[SCAN ? threadIdx.x / TPR : 0][0]) : list[0];
+    const bool cut = count > a.k;  // the table lists the token more often than its caller said: no sum of a part
+    const int n = cut ? 0 : count;
     const float start = cut ? __builtin_nanf("") : 0.f;
     SlotGroup g;
-    load_group(a, list, t, 0, n, g);
-    for (int64_t c = (int64_t)lane * N; c < whole; c += (int64_t)step * N) {
+    load_group(a, slot, t, 0, n, g);
+    // (the last piece of a row that is no whole number of them begins early and writes what its neighbour writes)
+    for (int64_t c0 = (int64_t)lane * N; c0 < H && H >= N; c0 += (int64_t)step * N) {
+      const int64_t c = c0 < H - N ? c0 : H - N;
       float acc[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = start;
       for (int j0 = 0; j0 < n; j0 += 8) {
-        if (n > 8) load_group(a, list, t, j0, n, g);
+        if (n > 8) load_group(a, slot, t, j0, n, g);
         u32x4 d[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -190,10 +229,10 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
       }
       store_piece<DT>(out + (t * H + c) * EL::SIZE, pack<DT>(acc));
     }
-    for (int64_t c = whole + lane; c < H; c += step) {
+    for (int64_t c = lane; c < H && H < N; c += step) {
       float acc = start;
       for (int j0 = 0; j0 < n; j0 += 8) {
-        if (n > 8) load_group(a, list, t, j0, n, g);
+        if (n > 8) load_group(a, slot, t, j0, n, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (g.row[j] >= 0) acc = fmaf(g.w[j], elem_to_f32<DT>(((const raw*)y)[g.row[j] * H + c]), acc);
@@ -254,7 +293,7 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
     }
     for (int j0 = 0; j0 < n; j0 += 8) {
       SlotGroup g;
-      load_group(a, list, t, j0, n, g);
+      load_group(a, [&](int j) { return list[1 + j]; }, t, j0, n, g);
       float dot[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) dot[j] = 0.f;
@@ -350,8 +389,10 @@ extern "C" int moe_permute_tokens(const void* x, const int32_t* token_position_t
   return MOE_OK;
 }
 
+// tp2id: for the scan, else null
 template <int DT>
-static void launch_combine_tokens(const void* y, const SlotTables& a, int64_t T, int64_t H, void* out, hipStream_t s) {
+static void launch_combine_tokens(const void* y, const SlotTables& a, const int32_t* tp2id, int64_t T, int64_t H, void* out,
+                                  hipStream_t s) {
   // a workgroup per token, or a wave where rows are short; few tokens (decode): several per token, a piece per thread
   const bool wide = H * Elem<DT>::SIZE > 2048;
   const int64_t groups = wide ? T : (T + 3) / 4;
@@ -361,21 +402,26 @@ static void launch_combine_tokens(const void* y, const SlotTables& a, int64_t T,
     if (parts > 512 / groups) parts = 512 / groups;
   }
   const dim3 grid(grid_of(groups), (unsigned)parts);
-  if (wide)
-    hipLaunchKernelGGL((combine_tokens_kernel<DT, 256>), grid, dim3(256), 0, s, (const uint8_t*)y, a, T, H, (uint8_t*)out);
-  else
-    hipLaunchKernelGGL((combine_tokens_kernel<DT, 64>), grid, dim3(256), 0, s, (const uint8_t*)y, a, T, H, (uint8_t*)out);
+#define MOE_COMBINE(TPR, SCAN)                                                                                                  \
+  hipLaunchKernelGGL((combine_tokens_kernel<DT, TPR, SCAN>), grid, dim3(256), 0, s, (const uint8_t*)y, a, tp2id, T, H, (uint8_t*)out)
+  if (wide && tp2id) MOE_COMBINE(256, true);
+  else if (wide) MOE_COMBINE(256, false);
+  else if (tp2id) MOE_COMBINE(64, true);
+  else MOE_COMBINE(64, false);
+#undef MOE_COMBINE
 }
+// (every group of threads reads the table: for few tokens and slots that costs less than the launch it saves)
+static bool combine_scans(int64_t S, int64_t T) { return S <= COMBINE_SCAN_SLOTS && T <= 512; }
 
 // What the calls that go by lists check alike, and the list itself where it is asked for.
-static int begin_by_list(const SlotTables& a, int64_t T, int64_t T1, const int32_t* tp2id, int build, hipStream_t s) {
+static int begin_by_list(const SlotTables& a, int64_t T, int64_t T1, const int32_t* tp2id, int build, bool launch, hipStream_t s) {
   if (!a.lists || a.S < 0 || T < 0 || (build && !tp2id && a.S > 0)) return MOE_E_BAD_ARG;
   if (a.k < 1 || a.k > SLOTS_MAX_K || T >= (int64_t)1 << 31 || a.S >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
   if (a.b2e) {
     if (!a.aff || (a.aff_dtype != MOE_DT_BF16 && a.aff_dtype != MOE_DT_FP32)) return MOE_E_BAD_ARG;
     if (a.E <= 0 || a.E >= (int64_t)1 << 31 || T1 < T) return MOE_E_BAD_SHAPE;
   }
-  return build ? launch_token_slots(tp2id, a.S, T, a.k, (int32_t*)a.lists, s) : MOE_OK;
+  return build && launch ? launch_token_slots(tp2id, a.S, T, a.k, (int32_t*)a.lists, s) : MOE_OK;
 }
 
 extern "C" int moe_combine_tokens(const void* y, int dtype, const void* expert_affinities, int aff_dtype, int64_t T1, int64_t E,
@@ -387,13 +433,15 @@ extern "C" int moe_combine_tokens(const void* y, int dtype, const void* expert_a
   if (block_to_expert && (B <= 0 || N < 0 || B >= (int64_t)1 << 31 || N >= (int64_t)1 << 31 || S != B * N)) return MOE_E_BAD_SHAPE;
   const SlotTables a{token_slots, block_to_expert, expert_affinities, aff_dtype, top_k, (uint32_t)B, (uint32_t)N, E, S};
   const hipStream_t s = (hipStream_t)stream;
-  const int rc = begin_by_list(a, T, T1, token_position_to_id, build_token_slots, s);
+  const bool scan = build_token_slots && combine_scans(S, T);
+  const int rc = begin_by_list(a, T, T1, token_position_to_id, build_token_slots, !scan, s);
   if (rc != MOE_OK) return rc;
   if (T == 0 || H == 0) return MOE_OK;
+  const int32_t* table = scan ? token_position_to_id : nullptr;
   switch (dtype) {
-    case MOE_DT_BF16: launch_combine_tokens<MOE_DT_BF16>(y, a, T, H, out, s); break;
-    case MOE_DT_FP16: launch_combine_tokens<MOE_DT_FP16>(y, a, T, H, out, s); break;
-    default: launch_combine_tokens<MOE_DT_FP32>(y, a, T, H, out, s); break;
+    case MOE_DT_BF16: launch_combine_tokens<MOE_DT_BF16>(y, a, table, T, H, out, s); break;
+    case MOE_DT_FP16: launch_combine_tokens<MOE_DT_FP16>(y, a, table, T, H, out, s); break;
+    default: launch_combine_tokens<MOE_DT_FP32>(y, a, table, T, H, out, s); break;
   }
   MOE_CHECK_LAUNCH();
   return MOE_OK;
@@ -410,7 +458,7 @@ extern "C" int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtyp
   const int64_t S = B * N;
   const SlotTables a{token_slots, block_to_expert, expert_affinities, aff_dtype, top_k, (uint32_t)B, (uint32_t)N, E, S};
   const hipStream_t s = (hipStream_t)stream;
-  const int rc = begin_by_list(a, T, T1, token_position_to_id, build_token_slots, s);
+  const int rc = begin_by_list(a, T, T1, token_position_to_id, build_token_slots, true, s);
   if (rc != MOE_OK) return rc;
   const unsigned grid = grid_of(T + (S + PAD_SLOTS - 1) / PAD_SLOTS + 1);
   switch (dtype) {

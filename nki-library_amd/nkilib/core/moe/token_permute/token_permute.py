@@ -23,7 +23,9 @@ from ...utils.kernel_assert import kernel_assert
 
 
 def _table(token_position_to_id):
-    t = nv.require_device_tensor(token_position_to_id, "token_position_to_id").reshape(-1)
+    t = nv.require_device_tensor(token_position_to_id, "token_position_to_id")
+    if t.dim() != 1:
+        t = t.reshape(-1)
     if t.dtype != torch.int32:
         kernel_assert(False, f"token_position_to_id must be int32 but got {t.dtype}")
     return t
@@ -37,9 +39,11 @@ def _rows(t, what, n=None):
 
 
 def _same_device(*tensors):
-    if any(t.device != tensors[0].device for t in tensors[1:]):
-        kernel_assert(False, f"tensors must be on one device but are on {[str(t.device) for t in tensors]}")
-    return tensors[0].device
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device != dev:
+            kernel_assert(False, f"tensors must be on one device but are on {[str(t.device) for t in tensors]}")
+    return dev
 
 
 def _slots(tp2id, n_tokens, top_k, token_slots):
@@ -49,7 +53,7 @@ def _slots(tp2id, n_tokens, top_k, token_slots):
     if n_tokens < 0:
         kernel_assert(False, f"n_tokens must not be negative but got {n_tokens}")
     if token_slots is None:
-        return torch.empty((n_tokens, 1 + top_k), dtype=torch.int32, device=tp2id.device), 1
+        return tp2id.new_empty((n_tokens, 1 + top_k)), 1
     token_slots = nv.require_device_tensor(token_slots, "token_slots")
     if token_slots.dtype != torch.int32 or token_slots.shape != (n_tokens, 1 + top_k):
         kernel_assert(False, f"token_slots must be int32 [{n_tokens}, {1 + top_k}] but got {token_slots.dtype} "
@@ -64,7 +68,9 @@ def _routing(expert_affinities_masked, block_to_expert, block_size, tp2id, n_tok
         kernel_assert(False, f"expert_affinities_masked must be bfloat16 or float32 but got {aff.dtype}")
     if aff.dim() != 2 or aff.shape[0] < n_tokens or aff.shape[1] < 1:
         kernel_assert(False, f"expert_affinities_masked must be [{n_tokens} or more, E] but got {tuple(aff.shape)}")
-    b2e = nv.require_device_tensor(block_to_expert, "block_to_expert").reshape(-1)
+    b2e = nv.require_device_tensor(block_to_expert, "block_to_expert")
+    if b2e.dim() != 1:
+        b2e = b2e.reshape(-1)
     if b2e.dtype != torch.int32:
         kernel_assert(False, f"block_to_expert must be int32 but got {b2e.dtype}")
     B = int(block_size)
@@ -99,7 +105,7 @@ def permute_tokens(hidden_states: torch.Tensor, token_position_to_id: torch.Tens
     x = _rows(hidden_states, "hidden_states")
     t = _table(token_position_to_id)
     dev = _same_device(x, t)
-    out = torch.empty((t.numel(), x.shape[1]), dtype=x.dtype, device=dev)
+    out = x.new_empty((t.numel(), x.shape[1]))
     if out.numel() == 0:
         return out
     if x.shape[0] == 0:
@@ -122,7 +128,7 @@ def permute_tokens_bwd(d_permuted: torch.Tensor, token_position_to_id: torch.Ten
     dt = nv.dtype_code(d, "d_permuted")
     slots, build = _slots(t, n_tokens, top_k, token_slots)
     _same_device(d, slots)
-    out = torch.empty((n_tokens, d.shape[1]), dtype=d.dtype, device=dev)
+    out = d.new_empty((n_tokens, d.shape[1]))
     if out.numel() == 0 or t.numel() == 0:
         return out.zero_()
     with nv.on_device(dev):
@@ -146,7 +152,7 @@ def combine_tokens(permuted: torch.Tensor, expert_affinities_masked: torch.Tenso
     dt = nv.dtype_code(y, "permuted")
     slots, build = _slots(t, n_tokens, top_k, token_slots)
     _same_device(y, slots)
-    out = torch.empty((n_tokens, y.shape[1]), dtype=y.dtype, device=dev)
+    out = y.new_empty((n_tokens, y.shape[1]))
     if out.numel() == 0 or t.numel() == 0:
         return out.zero_()
     with nv.on_device(dev):

@@ -13,7 +13,7 @@ DTYPES = ["bfloat16", "float16", "float32"]
 # T, H, E, k, B: one token, one slot per block, rows of odd length (2- and 4-byte pieces, none at all), more than eight slots per
 # token, more than a group of tokens per workgroup, an expert without tokens
 SHAPES = [(1, 64, 4, 1, 1), (1, 7168, 256, 8, 1), (5, 3, 4, 2, 4), (33, 130, 8, 3, 16), (300, 1029, 60, 4, 32), (129, 2056, 16, 2, 128),
-          (70, 515, 24, 17, 8), (40, 96, 64, 64, 1), (700, 256, 3, 3, 512)]
+          (70, 515, 24, 17, 8), (40, 96, 64, 64, 1), (700, 256, 3, 3, 512), (32, 1500, 64, 64, 1), (600, 128, 3, 3, 1)]
 
 
 def _case(shape, dtype, seed, skip_token=False):
