@@ -126,31 +126,40 @@ struct SlotTables {
   uint32_t B, N;
   int64_t E, S;          // S: rows of y
 };
-// Eight neighbours of a token's list: rows and weights.  A slot of a block without an expert counts for nothing and is
-// not read (row -1), nor is one that lies outside of y (a list made of another table).
+// Eight neighbours of a token's list: rows (-1: none; one outside of y, of a list made of another table, is none either), weights.
+// A slot of a block without an expert counts for nothing: `on` is false, its weight 0.  Its row is asked for all the same: the
+// rows of y do not wait for the chain of expert and affinity.
 struct SlotGroup {
   int64_t row[8];
   float w[8];
   int e[8];
+  bool on[8];
 };
 template <class SLOT>
-__device__ __forceinline__ void load_group(const SlotTables& a, SLOT&& slot, int64_t t, int j0, int n, SlotGroup& g) {
+__device__ __forceinline__ void load_rows(const SlotTables& a, SLOT&& slot, int j0, int n, SlotGroup& g) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     g.row[j] = j0 + j < n ? slot(j0 + j) : -1;
     if (g.row[j] >= a.S) g.row[j] = -1;
+  }
+}
+__device__ __forceinline__ void load_weights(const SlotTables& a, int64_t t, SlotGroup& g) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
     g.w[j] = 1.f;
     g.e[j] = 0;
+    g.on[j] = g.row[j] >= 0;
+    if (a.b2e && g.on[j]) {
+      const uint32_t b = (uint32_t)g.row[j] / a.B;
+      g.e[j] = b < a.N ? a.b2e[b] : -1;
+    }
   }
   if (!a.b2e) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    if (g.row[j] >= 0) {
-      const uint32_t b = (uint32_t)g.row[j] / a.B;
-      const int e = b < a.N ? a.b2e[b] : -1;
-      g.e[j] = e;
-      if (e < 0 || e >= a.E) g.row[j] = -1;
-      else g.w[j] = load_as_f32(a.aff, a.aff_dtype, t * a.E + e);
+    if (g.on[j]) {
+      g.on[j] = g.e[j] >= 0 && g.e[j] < a.E;
+      g.w[j] = g.on[j] ? load_as_f32(a.aff, a.aff_dtype, t * a.E + g.e[j]) : 0.f;
     }
 }
 
@@ -205,7 +214,8 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
     const int n = cut ? 0 : count;
     const float start = cut ? __builtin_nanf("") : 0.f;
     SlotGroup g;
-    load_group(a, slot, t, 0, n, g);
+    load_rows(a, slot, 0, n, g);
+    bool weighted = false;  // (the first eight's weights, once; more than eight slots: each time)
     // (the last piece of a row that is no whole number of them begins early and writes what its neighbour writes)
     for (int64_t c0 = (int64_t)lane * N; c0 < H && H >= N; c0 += (int64_t)step * N) {
       const int64_t c = c0 < H - N ? c0 : H - N;
@@ -213,14 +223,16 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = start;
       for (int j0 = 0; j0 < n; j0 += 8) {
-        if (n > 8) load_group(a, slot, t, j0, n, g);
+        if (n > 8) load_rows(a, slot, j0, n, g);
         u32x4 d[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (g.row[j] >= 0) d[j] = load_piece<DT>(y + (g.row[j] * H + c) * EL::SIZE);
+        if (n > 8 || !weighted) load_weights(a, t, g);
+        weighted = true;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (g.row[j] >= 0) {
+          if (g.on[j]) {
             float v[N];
             unpack<DT>(d[j], v);
 #pragma unroll
@@ -232,10 +244,11 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
     for (int64_t c = lane; c < H && H < N; c += step) {
       float acc = start;
       for (int j0 = 0; j0 < n; j0 += 8) {
-        if (n > 8) load_group(a, slot, t, j0, n, g);
+        load_rows(a, slot, j0, n, g);
+        load_weights(a, t, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (g.row[j] >= 0) acc = fmaf(g.w[j], elem_to_f32<DT>(((const raw*)y)[g.row[j] * H + c]), acc);
+          if (g.on[j]) acc = fmaf(g.w[j], elem_to_f32<DT>(((const raw*)y)[g.row[j] * H + c]), acc);
       }
       ((raw*)out)[t * H + c] = f32_to_elem<DT>(acc);
     }
@@ -293,7 +306,8 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
     }
     for (int j0 = 0; j0 < n; j0 += 8) {
       SlotGroup g;
-      load_group(a, [&](int j) { return list[1 + j]; }, t, j0, n, g);
+      load_rows(a, [&](int j) { return list[1 + j]; }, j0, n, g);
+      load_weights(a, t, g);
       float dot[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) dot[j] = 0.f;
@@ -302,12 +316,12 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
         const u32x4 dg = load_piece_kept<DT>(dout + (t * H + c) * EL::SIZE);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (g.row[j] >= 0) d[j] = load_piece<DT>(y + (g.row[j] * H + c) * EL::SIZE);
+          if (g.on[j]) d[j] = load_piece<DT>(y + (g.row[j] * H + c) * EL::SIZE);
         float gv[N];
         unpack<DT>(dg, gv);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (g.row[j] >= 0) {
+          if (g.on[j]) {
             float v[N];
             unpack<DT>(d[j], v);
 #pragma unroll
@@ -322,7 +336,7 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
         const float gv = elem_to_f32<DT>(((const raw*)dout)[t * H + c]);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (g.row[j] >= 0) {
+          if (g.on[j]) {
             dot[j] = fmaf(gv, elem_to_f32<DT>(((const raw*)y)[g.row[j] * H + c]), dot[j]);
             ((raw*)dy)[g.row[j] * H + c] = f32_to_elem<DT>(g.w[j] * gv);
           }
@@ -332,7 +346,7 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
       for (int j = 0; j < 8; ++j) {
         const float v = wave_sum(dot[j]);
         if ((tid & 63) == 0) s_part[tid >> 6][j] = v;
-        if (tid == 0 && j0 + j < n) s_e[j0 + j] = g.row[j] >= 0 ? g.e[j] : -1;
+        if (tid == 0 && j0 + j < n) s_e[j0 + j] = g.on[j] ? g.e[j] : -1;
       }
       __syncthreads();
       if (tid < 8 && j0 + tid < n) s_dot[j0 + tid] = (s_part[0][tid] + s_part[1][tid]) + (s_part[2][tid] + s_part[3][tid]);
