@@ -71,6 +71,12 @@ __device__ __forceinline__ float max8(float v) {
 }
 
 template <int KS>
+struct GradW {
+  static constexpr int NQ = KS > 8 ? KS / 8 : 1;  // column blocks of 256 experts
+  static constexpr int NT = KS > 8 ? 4 : KS / 2;  // 16-expert tiles per wave
+};
+
+template <int KS>
 __global__ __launch_bounds__(256) void router_dlogits_kernel(const RouterBwdArgs a) {
   constexpr int EP = 32 * KS, PITCH = EP + 4;
   extern __shared__ __attribute__((aligned(16))) float s_dl[];  // [32][PITCH]
@@ -216,8 +222,9 @@ __global__ __launch_bounds__(256) void router_dlogits_kernel(const RouterBwdArgs
     dst[0] = h;
     dst[64] = lo;
   }
-  for (int i = wave; i < 2 * KS; i += 4) {  // dw: 16 experts i
-    const float* col = s_dl + 8 * g * PITCH + 16 * i + c;
+  for (int i = wave; i < 2 * KS; i += 4) {  // dw: tile i % NT of a wave's NT; its column c is expert NT c + i % NT of theirs
+    constexpr int NT = GradW<KS>::NT;
+    const float* col = s_dl + 8 * g * PITCH + i / NT * (16 * NT) + NT * c + i % NT;
     u32x4 h, lo;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -249,11 +256,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t token_rows(const uint16_t* bas
 // each) go through LDS.  Lane (r, g) reads 8 tokens x 8 columns of them and turns them in registers: they are the fragments of
 // eight row tiles whose row r is column 8 r + j.  A step goes over them twice, for dl's hi and for its lo parts, so that the
 // fragments of either part arrive in registers that the other half step has no use for; the rows are asked for two steps ahead.
-template <int KS>
-struct GradW {
-  static constexpr int NQ = KS > 8 ? KS / 8 : 1;  // column blocks of 256 experts
-  static constexpr int NT = KS > 8 ? 4 : KS / 2;  // 16-expert tiles per wave
-};
 template <int KS>
 __global__ __launch_bounds__(DW_THREADS) void router_dw_kernel(const RouterBwdArgs a) {
   constexpr int NQ = GradW<KS>::NQ, NT = GradW<KS>::NT;
@@ -340,21 +342,39 @@ __global__ __launch_bounds__(DW_THREADS) void router_dw_kernel(const RouterBwdAr
     __syncthreads();
   }
   if (kg == 1) return;
+  // a lane's NT tiles are neighbours along the experts
   const bool whole = a.splits == 1;
+  const int64_t e0 = n0 * 16 + NT * r;
+  typedef float parts_any __attribute__((ext_vector_type(NT), aligned(4)));
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int64_t e = (n0 + n) * 16 + r;
-    if (e < a.E) {
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 8; ++j) {
+      const int64_t at = (hb * 128 + 8 * (4 * g + i) + j) * a.E + e0;
+      if (!whole && e0 + NT <= a.E) {
+        float* dst = a.dwp + sp * a.H * a.E + at;
+        if constexpr (NT == 1) *dst = acc[j][0][i];
+        else {
+          parts_any v;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int64_t at = (hb * 128 + 8 * (4 * g + i) + j) * a.E + e;
-          if (whole) a.dw[at] = f32_to_bf16_bits(acc[j][n][i]);
-          else a.dwp[sp * a.H * a.E + at] = acc[j][n][i];
+          for (int n = 0; n < NT; ++n) v[n] = acc[j][n][i];
+          *(parts_any*)dst = v;
+        }
+        continue;
+      }
+      if (NT == 4 && whole && e0 + NT <= a.E) {
+        typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+        *(u32x2_any*)(a.dw + at) = u32x2_any{pack2_bf16(acc[j][0][i], acc[j][NT > 1 ? 1 : 0][i]),
+                                             pack2_bf16(acc[j][NT > 2 ? 2 : 0][i], acc[j][NT > 3 ? 3 : 0][i])};
+        continue;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (e0 + n < a.E) {
+          if (whole) a.dw[at + n] = f32_to_bf16_bits(acc[j][n][i]);
+          else a.dwp[sp * a.H * a.E + at + n] = acc[j][n][i];
         }
     }
-  }
 }
 
 // The parts of dw and db added up, by the workgroups that have written dx.
