@@ -18,8 +18,12 @@
 //   1. router_dlogits_kernel   a workgroup takes 32 tokens: dl in LDS, then hi / lo fragments of 16 bytes per lane in the order in
 //                              which the products read them, each token's list of (expert, dl), and the tokens' part of db;
 //                              further workgroups transpose w (dense: bring it into fragment order);
-//   2. router_dw_kernel        bound by the matrix pipes at the clock that they leave (1.6 to 1.7 GHz of 2.4);
-//   3. router_dx_list_kernel   dx (router_dx_kernel: dense), then the sums of the parts of dw and of db.
+//   2. router_grad_kernel      dw and dx (large calls: router_dw_kernel, bound by the matrix pipes at the 1.64 GHz of 2.4 that their
+//                              power leaves, and router_dx_list_kernel, by the vector ALU: 75 instructions a token and 256
+//                              columns, half of them to unpack w);
+//   3. router_reduce_kernel    the sums of the parts of dw and of db (large calls: the workgroups of dx, when done).
+// T = 8192, H = 7168, E = 256, top-8: 8.4 + 56 + 50 us of 52 for its bytes at the rate of a copy and 50 for 2 x 2 x 30 GFLOP at
+// that of a large product.
 #include <type_traits>
 
 #include "common.hpp"
@@ -49,7 +53,7 @@ struct RouterBwdArgs {
   void* db;
   int db_dtype;
   int64_t steps, splits;  // steps of 32 tokens; parts of them for dw
-  int64_t x_splits;          // parts of the tokens for dx
+  int64_t n_dw, x_splits;    // jobs of dw; parts of the tokens for dx
 };
 
 __device__ __forceinline__ uint32_t hi_lo(float a, float b, uint32_t& lo) {
@@ -242,7 +246,7 @@ __device__ __forceinline__ v4f mfma(const u32x4& x, const u32x4& y, const v4f& c
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x), __builtin_bit_cast(v8bf, y), c, 0, 0, 0);
 }
 
-constexpr int DW_THREADS = 512, DX_THREADS = 256, DX_LIST_THREADS = 1024;
+constexpr int GRAD_THREADS = 512, DX_THREADS = 1024;
 
 // Rows [t0, t0 + 32) of x or dx, as a buffer: what lies behind the last token reads as zeros and is not written.  No branch
 // stands around a load or store then, and the waits count the operations that are really out.
@@ -256,13 +260,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t token_rows(const uint16_t* bas
 // each) go through LDS.  Lane (r, g) reads 8 tokens x 8 columns of them and turns them in registers: they are the fragments of
 // eight row tiles whose row r is column 8 r + j.  A step goes over them twice, for dl's hi and for its lo parts, so that the
 // fragments of either part arrive in registers that the other half step has no use for; the rows are asked for two steps ahead.
+constexpr int DW_LDS = 32768;
 template <int KS>
-__global__ __launch_bounds__(DW_THREADS) void router_dw_kernel(const RouterBwdArgs a) {
+__device__ __forceinline__ void grad_w(const RouterBwdArgs& a, int64_t job, uint8_t* smem) {
   constexpr int NQ = GradW<KS>::NQ, NT = GradW<KS>::NT;
-  __shared__ __attribute__((aligned(16))) u32x4 s_x[2][2][512];  // [group][buffer][32 tokens][16]; at the end the sums of a quarter
+  u32x4(*s_x)[2][512] = (u32x4(*)[2][512])smem;  // [group][buffer][32 tokens][16]; at the end the sums of a quarter
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int tid = threadIdx.x & 255, kg = wave >> 2, nq = wave & 3, r = lane & 15, g = lane >> 4;
-  const int64_t job = blockIdx.x;
   const int64_t nb = job % NQ, hb = job / NQ % (a.H / 128), sp = job / NQ / (a.H / 128);
   const int64_t s0 = a.steps * sp / a.splits, s1 = a.steps * (sp + 1) / a.splits;
   const int n0 = (int)nb * 16 + nq * NT;  // first of the wave's 16-expert tiles
@@ -377,41 +381,17 @@ __global__ __launch_bounds__(DW_THREADS) void router_dw_kernel(const RouterBwdAr
     }
 }
 
-// The parts of dw and db added up, by the workgroups that have written dx.
-__device__ __forceinline__ void reduce_parts(const RouterBwdArgs& a, int threads) {
-  const int64_t first = (int64_t)blockIdx.x * threads + threadIdx.x, step = (int64_t)gridDim.x * threads;
-  if (a.splits > 1) {
-    const int64_t n = a.H * a.E;  // (H is a multiple of 128: whole pieces of four)
-    for (int64_t i = first; i < n / 4; i += step) {
-      v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
-      for (int64_t s = 0; s < a.splits; ++s) v += ((const v4f*)(a.dwp + s * n))[i];
-      typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
-      *(u32x2_any*)(a.dw + 4 * i) = u32x2_any{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3])};
-    }
-  }
-  if (a.db)
-    for (int64_t e = first >> 6; e < a.E; e += step >> 6) {
-      float v = 0.f;
-      for (int64_t s = threadIdx.x & 63; s < a.steps; s += 64) v += a.dbp[s * a.E + e];
-      v = wave_sum(v);
-      if ((threadIdx.x & 63) == 0) {
-        if (a.db_dtype == MOE_DT_FP32) ((float*)a.db)[e] = v;
-        else ((uint16_t*)a.db)[e] = f32_to_bf16_bits(v);
-      }
-    }
-}
-
-// dx of k experts per token: a workgroup keeps the slice of w of 64 * CPL columns in LDS, a wave takes a token at a time, CPL
+// dx of k experts per token: a workgroup keeps the slice of w of 64 * CPL columns in LDS, a wave takes two tokens at a time, CPL
 // columns per lane: k reads of LDS and k multiply-adds per value, expert and dl in scalar registers.
-template <int CPL, int KP>
-__global__ __launch_bounds__(DX_LIST_THREADS) void router_dx_list_kernel(const RouterBwdArgs a) {
+template <int CPL, int KP, int THREADS>
+__device__ __forceinline__ void grad_x_list(const RouterBwdArgs& a, int64_t job, uint8_t* smem) {
   constexpr int COLS = 64 * CPL, W = CPL / 2;  // words of a lane
-  extern __shared__ __attribute__((aligned(16))) uint32_t s_w[];  // [E][COLS / 2]
+  uint32_t* s_w = (uint32_t*)smem;             // [E][COLS / 2]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int64_t slices = (a.H + COLS - 1) / COLS, c0 = blockIdx.x % slices * COLS, sp = blockIdx.x / slices;
+  const int64_t slices = (a.H + COLS - 1) / COLS, c0 = job % slices * COLS, sp = job / slices;
   const int cols = (int)(a.H - c0 < COLS ? a.H - c0 : COLS);  // (H is a multiple of 128)
   const int pieces = cols / 8;
-  for (int i = threadIdx.x; i < (int)a.E * pieces; i += DX_LIST_THREADS) {
+  for (int i = threadIdx.x; i < (int)a.E * pieces; i += THREADS) {
     const int e = i / pieces, p = i - e * pieces;
     *(u32x4*)(s_w + e * (COLS / 2) + 4 * p) = *(const u32x4*)(a.wt + e * a.H + c0 + 8 * p);
   }
@@ -419,48 +399,57 @@ __global__ __launch_bounds__(DX_LIST_THREADS) void router_dx_list_kernel(const R
   const int64_t t0 = a.T * sp / a.x_splits, t1 = a.T * (sp + 1) / a.x_splits;
   const bool mine = lane * CPL < cols;
   // (address space 4: read-only for the launch, uniform over the wave.  The lists come by scalar loads, which no store is waited
-  // for ahead of, a token early)
+  // for ahead of, a turn early)
   typedef const __attribute__((address_space(4))) uint32_t* list_ptr;
   auto fetch = [&](int64_t t, uint32_t(&l)[2 * KP]) {
     const list_ptr src = (list_ptr)(uintptr_t)(a.list + (t < t1 ? t : t1 - 1) * KP);
 #pragma unroll
     for (int i = 0; i < 2 * KP; ++i) l[i] = src[i];
   };
-  constexpr int WAVES = DX_LIST_THREADS / 64;
-  uint32_t now[2 * KP], next[2 * KP];
-  if (t0 + wave < t1) fetch(t0 + wave, now);
-  for (int64_t t = t0 + wave; t < t1; t += WAVES) {
-    fetch(t + WAVES, next);
-    float acc[CPL];
-#pragma unroll
-    for (int i = 0; i < CPL; ++i) acc[i] = 0.f;
-    uint32_t v[KP][W];
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-#pragma unroll
-      for (int q = 0; q < W; ++q) v[j][q] = s_w[now[2 * j] * (COLS / 2) + lane * W + q];
-#pragma unroll
-    for (int j = 0; j < KP; ++j) {
-      const float dl = __uint_as_float(now[2 * j + 1]);
-#pragma unroll
-      for (int q = 0; q < W; ++q) {
-        acc[2 * q] = fmaf(dl, bf16_lo(v[j][q]), acc[2 * q]);
-        acc[2 * q + 1] = fmaf(dl, bf16_hi(v[j][q]), acc[2 * q + 1]);
-      }
-    }
-    if (mine) {
-      uint32_t* dst = (uint32_t*)(a.dx + t * a.H + c0) + lane * W;
-      if constexpr (W == 2) {
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        __builtin_nontemporal_store((u32x2{pack2_bf16(acc[0], acc[1]), pack2_bf16(acc[2], acc[3])}), (u32x2*)dst);
-      } else {
-        __builtin_nontemporal_store(pack2_bf16(acc[0], acc[1]), dst);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * KP; ++i) now[i] = next[i];
+  constexpr int STEP = 2 * THREADS / 64;
+  uint32_t now[2][2 * KP], next[2][2 * KP];
+  int64_t t = t0 + 2 * wave;
+  if (t < t1) {
+    fetch(t, now[0]);
+    fetch(t + 1, now[1]);
   }
-  reduce_parts(a, DX_LIST_THREADS);
+  for (; t < t1; t += STEP) {
+    fetch(t + STEP, next[0]);
+    fetch(t + STEP + 1, next[1]);
+    uint32_t v[2][KP][W];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < KP; ++j)
+#pragma unroll
+        for (int q = 0; q < W; ++q) v[u][j][q] = s_w[now[u][2 * j] * (COLS / 2) + lane * W + q];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float acc[CPL];
+#pragma unroll
+      for (int i = 0; i < CPL; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KP; ++j) {
+        const float dl = __uint_as_float(now[u][2 * j + 1]);
+#pragma unroll
+        for (int q = 0; q < W; ++q) {
+          acc[2 * q] = fmaf(dl, bf16_lo(v[u][j][q]), acc[2 * q]);
+          acc[2 * q + 1] = fmaf(dl, bf16_hi(v[u][j][q]), acc[2 * q + 1]);
+        }
+      }
+      if (mine && t + u < t1) {
+        uint32_t* dst = (uint32_t*)(a.dx + (t + u) * a.H + c0) + lane * W;
+        if constexpr (W == 2) {
+          typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+          __builtin_nontemporal_store((u32x2{pack2_bf16(acc[0], acc[1]), pack2_bf16(acc[2], acc[3])}), (u32x2*)dst);
+        } else {
+          __builtin_nontemporal_store(pack2_bf16(acc[0], acc[1]), dst);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * KP; ++i) now[u][i] = next[u][i];
+    }
+  }
 }
 
 // Dense dx: each wave keeps the w of 64 columns (32 beyond 256 experts) in registers and multiplies 16 tokens after 16 tokens of a
@@ -468,18 +457,17 @@ __global__ __launch_bounds__(DX_LIST_THREADS) void router_dx_list_kernel(const R
 template <int KS>
 struct GradX {
   static constexpr int NM = KS > 8 ? 2 : 4;         // row tiles of 16 columns per wave
-  static constexpr int COLS = NM * 16 * 4;          // columns of a workgroup
+  static constexpr int COLS = NM * 16 * 8;          // columns of a workgroup
 };
 template <int KS>
-__global__ __launch_bounds__(DX_THREADS, 2) void router_dx_kernel(const RouterBwdArgs a) {
-  __shared__ __attribute__((aligned(16))) u32x4 s_dl[2 * KS * 128];  // [2][KS][2][64]
-  const int64_t job = blockIdx.x;
-  constexpr int NM = GradX<KS>::NM, PIECES = KS * 128 / DX_THREADS;
+__device__ __forceinline__ void grad_x(const RouterBwdArgs& a, int64_t job, uint8_t* smem) {
+  u32x4* s_dl = (u32x4*)smem;  // [2][KS][2][64]
+  constexpr int NM = GradX<KS>::NM, PIECES = KS * 128 / GRAD_THREADS > 0 ? KS * 128 / GRAD_THREADS : 1;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int64_t groups = (a.H + GradX<KS>::COLS - 1) / GradX<KS>::COLS, hg = job % groups, sp = job / groups;
   const int64_t tiles = (a.T + 15) / 16, i0 = tiles * sp / a.x_splits, i1 = tiles * (sp + 1) / a.x_splits;
-  const int64_t unit = hg * 4 + wave;  // of 16 NM columns
+  const int64_t unit = hg * 8 + wave;  // of 16 NM columns
   const bool mine = unit * NM / 4 < a.H / 64;  // (the others multiply the last block once more and keep nothing)
   const int64_t hb = mine ? unit * NM / 4 : a.H / 64 - 1, m0 = unit * NM % 4;
   u32x4 w[NM][KS];
@@ -491,11 +479,13 @@ __global__ __launch_bounds__(DX_THREADS, 2) void router_dx_kernel(const RouterBw
   auto fetch = [&](int64_t i) {
     const u32x4* src = a.dlx + (i < i1 ? i : i1 - 1) * (KS * 128) + tid;
 #pragma unroll
-    for (int q = 0; q < PIECES; ++q) in[q] = src[q * DX_THREADS];
+    for (int q = 0; q < PIECES; ++q)
+      if (q * GRAD_THREADS + tid < KS * 128) in[q] = src[q * GRAD_THREADS];
   };
   auto store = [&](u32x4* buf) {
 #pragma unroll
-    for (int q = 0; q < PIECES; ++q) buf[q * DX_THREADS + tid] = in[q];
+    for (int q = 0; q < PIECES; ++q)
+      if (q * GRAD_THREADS + tid < KS * 128) buf[q * GRAD_THREADS + tid] = in[q];
   };
   fetch(i0);
   store(s_dl);
@@ -536,6 +526,57 @@ __global__ __launch_bounds__(DX_THREADS, 2) void router_dx_kernel(const RouterBw
     }
     __syncthreads();
   }
+}
+
+// The parts of dw and db added up, by all workgroups of a launch.
+__device__ __forceinline__ void reduce_parts(const RouterBwdArgs& a, int threads) {
+  const int64_t first = (int64_t)blockIdx.x * threads + threadIdx.x, step = (int64_t)gridDim.x * threads;
+  if (a.splits > 1) {
+    const int64_t n = a.H * a.E;  // (H is a multiple of 128: whole pieces of four)
+    for (int64_t i = first; i < n / 4; i += step) {
+      v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
+      for (int64_t s = 0; s < a.splits; ++s) v += ((const v4f*)(a.dwp + s * n))[i];
+      typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+      *(u32x2_any*)(a.dw + 4 * i) = u32x2_any{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3])};
+    }
+  }
+  if (a.db)
+    for (int64_t e = first >> 6; e < a.E; e += step >> 6) {
+      float v = 0.f;
+      for (int64_t s = threadIdx.x & 63; s < a.steps; s += 64) v += a.dbp[s * a.E + e];
+      v = wave_sum(v);
+      if ((threadIdx.x & 63) == 0) {
+        if (a.db_dtype == MOE_DT_FP32) ((float*)a.db)[e] = v;
+        else ((uint16_t*)a.db)[e] = f32_to_bf16_bits(v);
+      }
+    }
+}
+
+// dw and dx in one launch, then the sums: jobs of dw, then jobs of dx, which need nothing of each other.  KP: the places of a token's
+// list; 0: dense.  (Slices of 256 columns of w in LDS, of 128 beyond 256 experts.)
+template <int KS, int KP>
+__global__ __launch_bounds__(GRAD_THREADS) void router_grad_kernel(const RouterBwdArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int64_t job = blockIdx.x;
+  if (job < a.n_dw) grad_w<KS>(a, job, smem);
+  else if constexpr (KP == 0) grad_x<KS>(a, job - a.n_dw, smem);
+  else grad_x_list<(KS > 8 ? 2 : 4), KP, GRAD_THREADS>(a, job - a.n_dw, smem);
+}
+__global__ __launch_bounds__(256) void router_reduce_kernel(const RouterBwdArgs a) { reduce_parts(a, 256); }
+
+// Or dw, and then dx with the sums behind it: dx by lists needs a quarter of dw's registers, so that a CU has 16 waves of it instead
+// of 8.  In one launch | two, us of a call: 128 tokens, top-8 of 128, H = 2048 15.6 | 19.3; 1999, top-4 of 60, 4096 24 |
+// 26; 8192, top-8 of 256, 7168 128 | 112.
+constexpr int64_t ONE_LAUNCH_VALUES = (int64_t)1 << 24;  // of x
+template <int KS>
+__global__ __launch_bounds__(GRAD_THREADS) void router_dw_kernel(const RouterBwdArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[DW_LDS];
+  grad_w<KS>(a, blockIdx.x, smem);
+}
+template <int CPL, int KP>
+__global__ __launch_bounds__(DX_THREADS) void router_dx_list_kernel(const RouterBwdArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  grad_x_list<CPL, KP, DX_THREADS>(a, blockIdx.x, smem);
   reduce_parts(a, DX_THREADS);
 }
 
@@ -568,30 +609,36 @@ static RouterBwdPlan router_bwd_plan(int64_t T, int64_t H, int64_t E) {
   return p;
 }
 
-// Parts of the tokens for dx: a workgroup per CU of `slices` slices of columns, `least` tokens each at least.
-static int64_t dx_splits(int64_t slices, int64_t T, int64_t least) {
-  int64_t n = 256 / slices;
-  if (n > (T + least - 1) / least) n = (T + least - 1) / least;
-  return n < 1 ? 1 : n;
-}
-template <int CPL, int KP>
-static int launch_dx_list(RouterBwdArgs& a, hipStream_t s) {
-  constexpr int LDS = 128 * 1024;
-  if (allow_lds<router_dx_list_kernel<CPL, KP>>(LDS) != hipSuccess) return MOE_E_LAUNCH;
-  const int64_t slices = (a.H + 64 * CPL - 1) / (64 * CPL);
-  a.x_splits = dx_splits(slices, a.T, DX_LIST_THREADS / 64);
-  hipLaunchKernelGGL((router_dx_list_kernel<CPL, KP>), dim3((unsigned)(slices * a.x_splits)), dim3(DX_LIST_THREADS), (size_t)a.E * 128 * CPL, s, a);
-  MOE_CHECK_LAUNCH();
-  return MOE_OK;
-}
-template <int CPL>
-static int launch_dx_list_k(RouterBwdArgs& a, hipStream_t s) {
-  switch (a.kp) {
-    case 1: return launch_dx_list<CPL, 1>(a, s);
-    case 2: return launch_dx_list<CPL, 2>(a, s);
-    case 4: return launch_dx_list<CPL, 4>(a, s);
-    default: return launch_dx_list<CPL, 8>(a, s);
+constexpr int GRAD_LDS = 128 * 1024;  // 256 experts by 256 columns of w, or 512 by 128
+template <int KS, int KP>
+static int launch_grad(RouterBwdArgs& a, hipStream_t s) {
+  const int64_t cols = KP == 0 ? GradX<KS>::COLS : KS > 8 ? 128 : 256, groups = (a.H + cols - 1) / cols;
+  // dx: a job per CU, of 16 tokens at least
+  a.x_splits = 256 / groups;
+  if (a.x_splits > (a.T + 15) / 16) a.x_splits = (a.T + 15) / 16;
+  if (a.x_splits < 1) a.x_splits = 1;
+  const int64_t n_dx = groups * a.x_splits;
+  if constexpr (KP > 0) {
+    if (a.T * a.H > ONE_LAUNCH_VALUES) {
+      constexpr int CPL = KS > 8 ? 2 : 4;
+      if (allow_lds<router_dx_list_kernel<CPL, KP>>(GRAD_LDS) != hipSuccess) return MOE_E_LAUNCH;
+      hipLaunchKernelGGL(router_dw_kernel<KS>, dim3((unsigned)a.n_dw), dim3(GRAD_THREADS), 0, s, a);
+      MOE_CHECK_LAUNCH();
+      hipLaunchKernelGGL((router_dx_list_kernel<CPL, KP>), dim3((unsigned)n_dx), dim3(DX_THREADS), (size_t)(a.E * cols * 2), s, a);
+      MOE_CHECK_LAUNCH();
+      return MOE_OK;
+    }
   }
+  const int dx = KP == 0 ? 2 * KS * 2048 : (int)(a.E * cols * 2);
+  if (allow_lds<router_grad_kernel<KS, KP>>(GRAD_LDS) != hipSuccess) return MOE_E_LAUNCH;
+  hipLaunchKernelGGL((router_grad_kernel<KS, KP>), dim3((unsigned)(a.n_dw + n_dx)), dim3(GRAD_THREADS), dx > DW_LDS ? dx : DW_LDS, s, a);
+  MOE_CHECK_LAUNCH();
+  if (a.splits > 1 || a.db) {
+    const int64_t wgs = a.splits > 1 ? a.H * a.E / 1024 : 0, least = a.db ? (a.E + 3) / 4 : 1;
+    hipLaunchKernelGGL(router_reduce_kernel, dim3((unsigned)(wgs > least ? wgs : least)), dim3(256), 0, s, a);
+    MOE_CHECK_LAUNCH();
+  }
+  return MOE_OK;
 }
 template <int KS>
 static int launch_router_bwd(RouterBwdArgs& a, const RouterBwdPlan& p, hipStream_t s) {
@@ -599,20 +646,12 @@ static int launch_router_bwd(RouterBwdArgs& a, const RouterBwdPlan& p, hipStream
   if (allow_lds<router_dlogits_kernel<KS>>(LDS) != hipSuccess) return MOE_E_LAUNCH;
   hipLaunchKernelGGL(router_dlogits_kernel<KS>, dim3((unsigned)(p.steps + a.H / 64)), dim3(256), LDS, s, a);
   MOE_CHECK_LAUNCH();
-  hipLaunchKernelGGL(router_dw_kernel<KS>, dim3((unsigned)p.n_dw), dim3(DW_THREADS), 0, s, a);
-  MOE_CHECK_LAUNCH();
-  // (256 experts by 256 columns of w, or 512 by 128, are the 128 KB of LDS that a slice may take)
-  if (!a.dense) return a.E <= 256 ? launch_dx_list_k<4>(a, s) : launch_dx_list_k<2>(a, s);
-  const int64_t groups = (a.H + GradX<KS>::COLS - 1) / GradX<KS>::COLS;
-  a.x_splits = dx_splits(groups, a.T, 16);
-  hipLaunchKernelGGL(router_dx_kernel<KS>, dim3((unsigned)(groups * a.x_splits)), dim3(DX_THREADS), 0, s, a);
-  MOE_CHECK_LAUNCH();
-  return MOE_OK;
+  return a.dense ? launch_grad<KS, 0>(a, s) : a.kp == 2 ? launch_grad<KS, 2>(a, s) : a.kp == 4 ? launch_grad<KS, 4>(a, s) : launch_grad<KS, 8>(a, s);
 }
 
 static int router_bwd_shape(int64_t T, int64_t H, int64_t E) {
   if (T < 1 || H < 1 || E < 1) return MOE_E_BAD_ARG;
-  // (every launch stays below 2^32 threads: at these limits 2^21 + 2^14 workgroups of 256, 2^14 of 512, 2^13 of 1024)
+  // (every launch stays below 2^32 threads: at these limits 2^21 + 2^14 workgroups of 256, 2^14 + 2^13 of 512)
   if (E > 512 || H % 128 != 0 || H > (int64_t)1 << 20 || T > (int64_t)1 << 26) return MOE_E_BAD_SHAPE;
   return MOE_OK;
 }
@@ -655,7 +694,7 @@ extern "C" int moe_router_topk_bwd(const void* d_affinities, int aff_dtype, cons
   a.norm = router_pre_norm && norm_topk_prob;
   a.full = router_pre_norm && !norm_topk_prob && !mask_to_topk;
   a.dense = a.full || (a.softmax && !a.chosen && !a.norm);
-  a.kp = k > 4 ? 8 : k > 2 ? 4 : k;
+  a.kp = k > 4 ? 8 : k > 2 ? 4 : 2;
   a.dlx = (u32x4*)(ws + p.dlx);
   a.dlw = (u32x4*)(ws + p.dlw);
   a.wp = (u32x4*)(ws + p.w);
@@ -667,7 +706,7 @@ extern "C" int moe_router_topk_bwd(const void* d_affinities, int aff_dtype, cons
   a.dwp = (float*)(ws + p.dwp);
   a.db = d_bias;
   a.db_dtype = bias_dtype;
-  a.steps = p.steps; a.splits = p.splits;
+  a.steps = p.steps; a.splits = p.splits; a.n_dw = p.n_dw;
   const hipStream_t s = (hipStream_t)stream;
   switch (p.ks) {
     case 2: return launch_router_bwd<2>(a, p, s);

@@ -37,5 +37,6 @@ Modules
   rmsnorm    RMSNorm + fp8 ROW / STATIC quantise, RMSNorm -> MXFP8
   moe        blockwise MoE goldens (bf16, fp8-weight, fp8-row, MXFP8)
   router     router top-k (logits, top-k selection, affinities)
+  train      permute / combine / 8-bit activation checkpoints / router gradient, in 64 bits
   compare    the reference comparator (max-abs-rel "maxAllClose")
 """

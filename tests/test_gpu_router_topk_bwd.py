@@ -98,19 +98,21 @@ def test_gradients(shape, mode):
     _check(got, want, err, values(x), values(w), f"{shape} {mode}", bias)
 
 
-@pytest.mark.parametrize("T,H,E,k", [(8192, 7168, 256, 8), (4096, 2048, 128, 8), (1999, 4096, 60, 4), (3000, 1024, 300, 8)])
-def test_large_shapes_on_the_device(T, H, E, k):
-    """The token axis in many parts, against products in 64 bits on the GPU."""
+@pytest.mark.parametrize("T,H,E,k,softmax", [(8192, 7168, 256, 8, False), (4096, 2048, 128, 8, False), (1999, 4096, 60, 4, False),
+                                             (3000, 1024, 300, 8, False), (17001, 1024, 300, 3, False), (16500, 1152, 70, 1, False),
+                                             (8200, 2176, 512, 2, False), (9000, 2048, 200, 4, True)])
+def test_large_shapes_on_the_device(T, H, E, k, softmax):
+    """The token axis in many parts, dw and dx in one launch and in two, against products in 64 bits on the GPU."""
     import torch
     from nkilib.core.router_topk import router_topk_bwd
     from nkilib.core.utils.common_types import RouterActFnType
 
     rng, l, ids, g, x, w = _case(T, H, E, k, 9)
-    mode = (False, True, True, True)
+    mode = (softmax, True, not softmax, True)
     want, err = _dl_limits(g[:T].astype(np.float64), l, ids, mode)
     bias = torch.zeros(E, device="cuda")
-    d_x, d_w, d_b = router_topk_bwd(tensor(g), x, w, bias, tensor(l), tensor(ids, "int32"), RouterActFnType.SIGMOID,
-                                    norm_topk_prob=True)
+    d_x, d_w, d_b = router_topk_bwd(tensor(g), x, w, bias, tensor(l), tensor(ids, "int32"),
+                                    RouterActFnType.SOFTMAX if softmax else RouterActFnType.SIGMOID, norm_topk_prob=not softmax)
     dl, er = torch.from_numpy(want).cuda(), torch.from_numpy(err).cuda()
     xd, wd = x.double(), w.double()
 
