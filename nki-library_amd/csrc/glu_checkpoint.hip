@@ -16,6 +16,9 @@
 // All of it moves bytes: a pair of values costs 4 + 2 + 2 + 1/16 bytes forward in bf16, 2 + 1/16 + 2 + 4 + 2 backward.  Four lanes
 // share a group of 32, eight values each (16 bytes of bf16), so that a group's maximum is two exchanges between neighbours.
 // Rows of padding slots are neither read nor computed: their outputs are zero.
+// Measured: forward, fp16, 9088 rows (8192 of tokens) of I = 14336 174 us = 5.7 TB/s; backward, bf16, 98048 rows (65536) of 2048
+// 311 us = 5.6 TB/s, 330 with stores that stay in the caches, 321 with such loads; pack of 1408 rows (512) of 1024 8.7 us, of which the
+// bytes are 2 (with 2-byte loads and a lookup of the row's id for each 14).  A copy moves 4.9 TB/s, a fill 6.9.
 #include <type_traits>
 
 #include "rows.hpp"

@@ -9,6 +9,9 @@
 // hardly compute: their bound is memory.  Sums run over the slots in ascending order in 32 bits and are rounded once, so
 // that a result depends on its inputs alone.  (The layer's own combine, combine.hip, adds in bf16 as the reference does.)
 //
+// T = 8192 tokens of 14 KB in 8 of 98048 slots: combine 202 us with its list (5.2 TB/s), its backward pass 500 (4.9; 5.3 without
+// list and launches); T = 8192, 4 KB, 8 of 81792 52 us = 5.8 TB/s.  A copy moves 4.9.
+//
 // All but permute work by token: a token's row is read or written once whatever k is.  They go by a list of every token's slots,
 // which token_slots_kernel inverts the table into.
 #include <type_traits>
