@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void router_dlogits_kernel(const RouterBwdArgs
       if (a.norm) {
         const float total = sum8(s);
         const float mean = sum8(on ? g * s : 0.f) / total;
-        dl = (g - mean) / total * slope;
+        dl = (g - mean) * (slope / total);  // (a_j (1 - s_j), at most one: scores near zero do not overflow on the way)
       }
     }
     if (on) s_dl[tl * PITCH + id] = dl;

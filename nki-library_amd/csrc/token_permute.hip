@@ -166,10 +166,10 @@ __device__ __forceinline__ void load_weights(const SlotTables& a, int64_t t, Slo
     }
 }
 
-// TPR threads per token; where the tokens are few, gridDim.y groups of them side by side along the row.  tp2id: the table
-// itself, of at most COMBINE_SCAN_SLOTS slots for tokens of a single round of the launch, that every group looks its token up in:
-// a launch less, which at such sizes takes as long as the sums (8 tokens, 64 slots of 14 KB: kernels 6.1 + 3.0 us by the list, 6.8 so; a call 17.6 and
-// 13.0).  Null: by the lists.
+// TPR threads per token; where the tokens are few, gridDim.y groups of them side by side along the row.  SCAN: every group looks
+// its token up in the table itself, of at most COMBINE_SCAN_SLOTS slots, for tokens of a single round of the launch: a launch
+// less, which at such sizes takes as long as the sums (8 tokens, 64 slots of 14 KB: kernels 6.1 + 3.0 us by the list, 6.8 so; a
+// call 17.6 and 13.0).
 constexpr int64_t COMBINE_SCAN_SLOTS = 2048;
 template <int DT, int TPR, bool SCAN>
 __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __restrict__ y, const SlotTables a,

@@ -180,6 +180,21 @@ def test_extreme_logits():
         _check((d_x, d_w, None), want, err, values(x), values(w), str(mode), None)
 
 
+def test_scores_near_zero_divided_by_their_sum():
+    """Sigmoid scores of 1e-37 divided by their sum are ordinary affinities with ordinary gradients."""
+    from nkilib.core.router_topk import router_topk_bwd
+    from nkilib.core.utils.common_types import RouterActFnType
+
+    T, H, E, k = 20, 128, 12, 4
+    rng, l, ids, g, x, w = _case(T, H, E, k, 6)
+    l = (l / 4 - 85).astype(np.float32)
+    g *= 100
+    mode = (False, True, True, True)
+    got = router_topk_bwd(tensor(g), x, w, None, tensor(l), tensor(ids, "int32"), RouterActFnType.SIGMOID, norm_topk_prob=True)
+    want, err = _dl_limits(g[:T].astype(np.float64), l, ids, mode)
+    _check(got, want, err, values(x), values(w), str(mode), None)
+
+
 def test_route_for_moe_hands_out_the_logits():
     import torch
     from nkilib.core.router_topk import route_for_moe
