@@ -326,59 +326,57 @@ __device__ __forceinline__ void grad_w(const RouterBwdArgs& a, int64_t job, uint
     multiply(buf, bl);
     __syncthreads();
   }
-  // the second group's sums to the first by way of LDS, two row tiles of 16 columns at a time
-  v4f* s_acc = (v4f*)s_x + nq * (2 * NT * 64) + lane;
+  // both groups' sums by way of LDS, JC of the eight columns of a lane's 8 r + j at a time, and from there to memory in pieces of
+  // four experts: in a loop, since code that runs once is fetched cold (written out as stores of accumulators, this launch took
+  // 11.3 us for 128 tokens, now 8.2)
+  constexpr int JC = 8 / NT;
+  float* s_sum = (float*)smem;  // [4 waves][JC][NT][64 lanes][4]
+  v4f* s_acc = (v4f*)smem + nq * (JC * NT * 64) + lane;
+  const bool whole = a.splits == 1;
+  const int64_t e_base = nb * 256;
 #pragma unroll
-  for (int j0 = 0; j0 < 8; j0 += 2) {
+  for (int j0 = 0; j0 < 8; j0 += JC) {
     if (kg == 1) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < JC; ++j)
 #pragma unroll
         for (int n = 0; n < NT; ++n) s_acc[(j * NT + n) * 64] = acc[j0 + j][n];
     }
     __syncthreads();
     if (kg == 0) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < JC; ++j)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[j0 + j][n] += s_acc[(j * NT + n) * 64];
+        for (int n = 0; n < NT; ++n) s_acc[(j * NT + n) * 64] += acc[j0 + j][n];
+    }
+    __syncthreads();
+    // piece p: row p / (16 NT) of 16 JC, experts 4 (p % (16 NT)) ..
+#pragma unroll 1
+    for (int p = threadIdx.x; p < 2048; p += GRAD_THREADS) {
+      const int row = p / (16 * NT), e4 = 4 * (p % (16 * NT)), j = row % JC, gi = row / JC;  // gi = 4 g + i of the accumulators
+      const int64_t e = e_base + e4, at = (hb * 128 + 8 * gi + j0 + j) * a.E + e;
+      v4f v;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // expert (wave, NT r + n)
+        const int ee = e4 + q, wv = ee / (16 * NT), in = ee % (16 * NT), r2 = in / NT, n = in % NT;
+        v[q] = s_sum[(((wv * JC + j) * NT + n) * 64 + 16 * (gi >> 2) + r2) * 4 + (gi & 3)];
+      }
+      if (e + 4 <= a.E) {
+        typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+        typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+        if (whole) *(u32x2_any*)(a.dw + at) = u32x2_any{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3])};
+        else *(v4f_any*)(a.dwp + sp * a.H * a.E + at) = v4f_any{v[0], v[1], v[2], v[3]};
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (e + q < a.E) {
+            if (whole) a.dw[at + q] = f32_to_bf16_bits(v[q]);
+            else a.dwp[sp * a.H * a.E + at + q] = v[q];
+          }
+      }
     }
     __syncthreads();
   }
-  if (kg == 1) return;
-  // a lane's NT tiles are neighbours along the experts
-  const bool whole = a.splits == 1;
-  const int64_t e0 = n0 * 16 + NT * r;
-  typedef float parts_any __attribute__((ext_vector_type(NT), aligned(4)));
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t at = (hb * 128 + 8 * (4 * g + i) + j) * a.E + e0;
-      if (!whole && e0 + NT <= a.E) {
-        float* dst = a.dwp + sp * a.H * a.E + at;
-        if constexpr (NT == 1) *dst = acc[j][0][i];
-        else {
-          parts_any v;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) v[n] = acc[j][n][i];
-          *(parts_any*)dst = v;
-        }
-        continue;
-      }
-      if (NT == 4 && whole && e0 + NT <= a.E) {
-        typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
-        *(u32x2_any*)(a.dw + at) = u32x2_any{pack2_bf16(acc[j][0][i], acc[j][NT > 1 ? 1 : 0][i]),
-                                             pack2_bf16(acc[j][NT > 2 ? 2 : 0][i], acc[j][NT > 3 ? 3 : 0][i])};
-        continue;
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-        if (e0 + n < a.E) {
-          if (whole) a.dw[at + n] = f32_to_bf16_bits(acc[j][n][i]);
-          else a.dwp[sp * a.H * a.E + at + n] = acc[j][n][i];
-        }
-    }
 }
 
 // dx of k experts per token: a workgroup keeps the slice of w of 64 * CPL columns in LDS, a wave takes two tokens at a time, CPL
