@@ -90,7 +90,10 @@ __global__ __launch_bounds__(256) void router_dlogits_kernel(const RouterBwdArgs
     if (!a.dense) {
       uint16_t* s_w = (uint16_t*)s_dl;  // [64][E]
       const uint16_t* src = a.w + hb * 64 * a.E;
-      for (int i = tid; i < 64 * (int)a.E; i += 256) s_w[i] = src[i];
+      for (int i = tid; i < 8 * (int)a.E; i += 256) {
+        const u32x4_any d = *(const u32x4_any*)(src + 8 * i);
+        *(u32x4*)(s_w + 8 * i) = u32x4{d[0], d[1], d[2], d[3]};
+      }
       __syncthreads();
       for (int i = tid; i < 8 * (int)a.E; i += 256) {
         const int e = i >> 3, p = i & 7;

@@ -27,9 +27,12 @@ from ...utils.kernel_assert import kernel_assert
 def _ids(token_position_to_id, n_tokens, R, device):
     if token_position_to_id is None:
         return None, 0
-    t = nv.require_device_tensor(token_position_to_id, "token_position_to_id").reshape(-1)
+    t = nv.require_device_tensor(token_position_to_id, "token_position_to_id")
+    if t.dim() != 1:
+        t = t.reshape(-1)
     if t.dtype != torch.int32 or t.numel() != R or t.device != device:
-        kernel_assert(False, f"token_position_to_id must be int32 of {R} rows on {device} but is {t.dtype} of {t.numel()} on {t.device}")
+        kernel_assert(False, f"token_position_to_id must be int32 of {R} rows on {device} but is {t.dtype} of {t.numel()} on "
+                             f"{t.device}")
     if n_tokens is None or int(n_tokens) < 0:
         kernel_assert(False, "token_position_to_id needs n_tokens")
     return t, int(n_tokens)

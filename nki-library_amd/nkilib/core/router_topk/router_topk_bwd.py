@@ -49,8 +49,9 @@ def router_topk_bwd(d_expert_affinities, x, w, w_bias, router_logits, expert_ind
         if bias.numel() != E or bias.dtype not in (torch.bfloat16, torch.float32):
             kernel_assert(False, f"w_bias must hold E = {E} bfloat16 or float32 values but is {bias.dtype} {tuple(bias.shape)}")
         d_bias = torch.empty_like(bias)
-    if any(t is not None and t.device != dev for t in (w, g, logits, ids, bias)):
-        kernel_assert(False, f"all tensors must be on {dev}")
+    for t in (w, g, logits, ids, bias):
+        if t is not None and t.device != dev:
+            kernel_assert(False, f"all tensors must be on {dev} but one is on {t.device}")
     act = act_fn if isinstance(act_fn, RouterActFnType) else RouterActFnType(act_fn)
     d_x, d_w = torch.empty_like(x), torch.empty_like(w)
     if T == 0:
