@@ -84,6 +84,7 @@ __global__ __launch_bounds__(1024) void token_slots_kernel(const int32_t* __rest
 
 typedef uint32_t bytes16 __attribute__((ext_vector_type(4), aligned(1)));
 
+constexpr int64_t SHORT_ROW = 4096;  // bytes of a row that is a wave's work
 // TPR threads per row or part of a row (a whole number of waves, so that everything about a row is uniform).
 template <int TPR>
 __device__ __forceinline__ int64_t row_of_group() {
@@ -93,6 +94,8 @@ __device__ __forceinline__ int64_t row_of_group() {
 // as often as they have slots, from the Infinity Cache if the output leaves them there.  T = 8192 tokens of 14 KB in 8 of 98048
 // slots, x in no cache, us: 306; a piece at a time 319, with ordinary stores 359, a workgroup per 512 pieces 361; token by token,
 // each row read once and written to 8 places, 301 with the list of the slots that this takes.  The writes alone, in order: 205.
+// A wave or a workgroup per row, us: 8192 tokens of 1 KB 29 and 49, 3 KB 67 and 82, 5.6 KB 129 and 127, 8 KB 180 and 172; 1024 of
+// 3 KB 18 and 24, 5.6 KB 32 and 32.
 template <int TPR>
 __global__ __launch_bounds__(256) void permute_kernel(const uint8_t* __restrict__ x, const int32_t* __restrict__ tp2id, int64_t S,
                                                       int64_t T, int64_t row_bytes, uint8_t* __restrict__ out) {
@@ -178,11 +181,11 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
   typedef Elem<DT> EL;
   typedef typename EL::raw raw;
   constexpr int N = EL::N;
-  __shared__ int s_found[SCAN ? 256 / TPR : 1][1 + SLOTS_MAX_K], s_sorted[SCAN ? 256 / TPR : 1][SLOTS_MAX_K];
+  static_assert(TPR == 256 || !SCAN, "the scan is the workgroup's");
+  __shared__ int found[SCAN ? 1 + SLOTS_MAX_K : 1], sorted[SCAN ? SLOTS_MAX_K : 1];
   const int lane = blockIdx.y * TPR + threadIdx.x % TPR, step = gridDim.y * TPR;
   if constexpr (SCAN) {
-    int *found = s_found[threadIdx.x / TPR], *sorted = s_sorted[threadIdx.x / TPR];
-    const int i0 = threadIdx.x % TPR, S = (int)a.S;
+    const int i0 = threadIdx.x, S = (int)a.S;
     const int t = (int)row_of_group<TPR>();
     if (i0 == 0) found[0] = 0;
     __syncthreads();
@@ -209,10 +212,10 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
   for (int64_t t = row_of_group<TPR>(); t < T; t += (int64_t)gridDim.x * (256 / TPR)) {
     const int32_t* list = SCAN ? nullptr : a.lists + t * (1 + a.k);
     auto slot = [&](int j) {
-      if constexpr (SCAN) return __builtin_amdgcn_readfirstlane(s_sorted[threadIdx.x / TPR][j]);
+      if constexpr (SCAN) return __builtin_amdgcn_readfirstlane(sorted[j]);
       else return list[1 + j];
     };
-    const int count = SCAN ? __builtin_amdgcn_readfirstlane(s_found[SCAN ? threadIdx.x / TPR : 0][0]) : list[0];
+    const int count = SCAN ? __builtin_amdgcn_readfirstlane(found[0]) : list[0];
     const bool cut = count > a.k;  // the table lists the token more often than its caller said: no sum of a part
     const int n = cut ? 0 : count;
     const float start = cut ? __builtin_nanf("") : 0.f;
@@ -263,8 +266,12 @@ __global__ __launch_bounds__(256) void combine_tokens_kernel(const uint8_t* __re
 // Jobs [0, T) take a token each: its row of dout is read once per eight slots, eight rows of y and dy beside it.  The next
 // ceil(S / PAD_SLOTS) write the rows of slots that no token's list holds (few slots each: padding comes in runs, at an expert's
 // end; with 64 the kernel took 480 us instead of 465 at T = 8192, 98048 slots of 14 KB), the last one the rows of da behind T.
+// A job has TPR threads: a workgroup, or a wave where rows are short, which shares nothing with the others of its workgroup.
+// The kernel with workgroups and with waves, us: 3855 tokens in 3 slots of 130 bytes 48 and 16, 8192 in 8 of 1.5 KB 160 and 60,
+// 3 KB 175 and 100, 5.6 KB 222 and 180, 8 KB 262 and 263, 14 KB 467 and 482.  (Calls for 1024 tokens: 3 KB 43 and 35, 5.6 KB 54
+// and 54; for 128: 20 and 21, 23 and 27.)
 constexpr int PAD_SLOTS = 8;
-template <int DT>
+template <int DT, int TPR>
 __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* __restrict__ dout, const uint8_t* __restrict__ y,
                                                                  const SlotTables a, const int32_t* __restrict__ tp2id,
                                                                  int64_t S, int64_t T, int64_t T1, int64_t H,
@@ -272,13 +279,15 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
   typedef Elem<DT> EL;
   typedef typename EL::raw raw;
   constexpr int N = EL::N;
+  constexpr bool WAVE_JOB = TPR == 64;
+  static_assert(TPR == 64 || TPR == 256, "a wave or the workgroup");
   __shared__ float s_part[4][8], s_dot[SLOTS_MAX_K];
   __shared__ int s_e[SLOTS_MAX_K];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x % TPR;
   const int64_t whole = H / N * N, n_pad = (S + PAD_SLOTS - 1) / PAD_SLOTS;
-  for (int64_t job = blockIdx.x; job < T + n_pad + 1; job += gridDim.x) {
+  for (int64_t job = row_of_group<TPR>(); job < T + n_pad + 1; job += (int64_t)gridDim.x * (256 / TPR)) {
     if (job == T + n_pad) {
-      for (int64_t i = T * a.E + tid; i < T1 * a.E; i += 256) daff[i] = 0.f;
+      for (int64_t i = T * a.E + tid; i < T1 * a.E; i += TPR) daff[i] = 0.f;
       continue;
     }
     if (job >= T) {
@@ -295,18 +304,21 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
         float v[N];
 #pragma unroll
         for (int q = 0; q < N; ++q) v[q] = (nans >> i) & 1 ? __builtin_nanf("") : 0.f;
-        for (int64_t c = (int64_t)tid * N; c < whole; c += 256 * N) store_piece<DT>(dy + (s * H + c) * EL::SIZE, pack<DT>(v));
-        for (int64_t c = whole + tid; c < H; c += 256) ((raw*)dy)[s * H + c] = f32_to_elem<DT>(v[0]);
+        for (int64_t c = (int64_t)tid * N; c < whole; c += TPR * N) store_piece<DT>(dy + (s * H + c) * EL::SIZE, pack<DT>(v));
+        for (int64_t c = whole + tid; c < H; c += TPR) ((raw*)dy)[s * H + c] = f32_to_elem<DT>(v[0]);
       }
       continue;
     }
     const int64_t t = job;
     const int32_t* list = a.lists + t * (1 + a.k);
     const int n = list[0];
+    float* drow = daff + t * a.E;
     if (n > a.k) {
-      for (int64_t e = tid; e < a.E; e += 256) daff[t * a.E + e] = __builtin_nanf("");
+      for (int64_t e = tid; e < a.E; e += TPR) drow[e] = __builtin_nanf("");
       continue;
     }
+    if (WAVE_JOB && n <= 0)
+      for (int64_t e = tid; e < a.E; e += TPR) drow[e] = 0.f;
     for (int j0 = 0; j0 < n; j0 += 8) {
       SlotGroup g;
       load_rows(a, [&](int j) { return list[1 + j]; }, j0, n, g);
@@ -314,7 +326,7 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
       float dot[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) dot[j] = 0.f;
-      for (int64_t c = (int64_t)tid * N; c < whole; c += 256 * N) {
+      for (int64_t c = (int64_t)tid * N; c < whole; c += TPR * N) {
         u32x4 d[8];
         const u32x4 dg = load_piece_kept<DT>(dout + (t * H + c) * EL::SIZE);
 #pragma unroll
@@ -335,7 +347,7 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
             store_piece<DT>(dy + (g.row[j] * H + c) * EL::SIZE, pack<DT>(v));
           }
       }
-      for (int64_t c = whole + tid; c < H; c += 256) {
+      for (int64_t c = whole + tid; c < H; c += TPR) {
         const float gv = elem_to_f32<DT>(((const raw*)dout)[t * H + c]);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -344,22 +356,37 @@ __global__ __launch_bounds__(256) void combine_tokens_bwd_kernel(const uint8_t* 
             ((raw*)dy)[g.row[j] * H + c] = f32_to_elem<DT>(g.w[j] * gv);
           }
       }
-      __syncthreads();  // (the sums of the group before, and of the token before, have been read)
+      if constexpr (WAVE_JOB) {
+        // every lane has the sums: each adds up the entries of da that are its own, group by group
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = wave_sum(dot[j]);
-        if ((tid & 63) == 0) s_part[tid >> 6][j] = v;
-        if (tid == 0 && j0 + j < n) s_e[j0 + j] = g.on[j] ? g.e[j] : -1;
+        for (int j = 0; j < 8; ++j) dot[j] = wave_sum(dot[j]);
+        for (int64_t e = tid; e < a.E; e += TPR) {
+          float v = j0 ? drow[e] : 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (g.on[j] && g.e[j] == e) v += dot[j];
+          drow[e] = v;
+        }
+      } else {
+        __syncthreads();  // (the sums of the group before, and of the token before, have been read)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float v = wave_sum(dot[j]);
+          if ((tid & 63) == 0) s_part[tid >> 6][j] = v;
+          if (tid == 0 && j0 + j < n) s_e[j0 + j] = g.on[j] ? g.e[j] : -1;
+        }
+        __syncthreads();
+        if (tid < 8 && j0 + tid < n) s_dot[j0 + tid] = (s_part[0][tid] + s_part[1][tid]) + (s_part[2][tid] + s_part[3][tid]);
       }
-      __syncthreads();
-      if (tid < 8 && j0 + tid < n) s_dot[j0 + tid] = (s_part[0][tid] + s_part[1][tid]) + (s_part[2][tid] + s_part[3][tid]);
     }
-    __syncthreads();
-    for (int64_t e = tid; e < a.E; e += 256) {
-      float v = 0.f;
-      for (int j = 0; j < n; ++j)
-        if (s_e[j] == e) v += s_dot[j];
-      daff[t * a.E + e] = v;
+    if constexpr (!WAVE_JOB) {
+      __syncthreads();
+      for (int64_t e = tid; e < a.E; e += TPR) {
+        float v = 0.f;
+        for (int j = 0; j < n; ++j)
+          if (s_e[j] == e) v += s_dot[j];
+        drow[e] = v;
+      }
     }
   }
 }
@@ -396,7 +423,7 @@ extern "C" int moe_permute_tokens(const void* x, const int32_t* token_position_t
   if (S >= (int64_t)1 << 31 || T >= (int64_t)1 << 31 || row_bytes >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
   if (S == 0 || row_bytes == 0) return MOE_OK;
   const hipStream_t s = (hipStream_t)stream;
-  if (row_bytes > 2048)
+  if (row_bytes > SHORT_ROW)
     hipLaunchKernelGGL(permute_kernel<256>, dim3(grid_of(S)), dim3(256), 0, s, (const uint8_t*)x, token_position_to_id, S, T,
                        row_bytes, (uint8_t*)out);
   else
@@ -410,8 +437,10 @@ extern "C" int moe_permute_tokens(const void* x, const int32_t* token_position_t
 template <int DT>
 static void launch_combine_tokens(const void* y, const SlotTables& a, const int32_t* tp2id, int64_t T, int64_t H, void* out,
                                   hipStream_t s) {
-  // a workgroup per token, or a wave where rows are short; few tokens (decode): several per token, a piece per thread
-  const bool wide = H * Elem<DT>::SIZE > 2048;
+  // a workgroup per token, or a wave where rows are short and tokens many (us a call, top-8 of 128 experts, caches cold, wave and
+  // workgroup: 1024 tokens of 1 KB 15.6 and 15.6, 3 KB 19.6 and 18.3; 8192 of 1 KB 35 and 37, 3 KB 59 and 68, 8 KB 130 and 125);
+  // few tokens (decode): several per token, a piece per thread
+  const bool wide = H * Elem<DT>::SIZE > SHORT_ROW || T < 2048;
   const int64_t groups = wide ? T : (T + 3) / 4;
   int64_t parts = 1;
   if (wide && groups < 512) {
@@ -423,7 +452,6 @@ static void launch_combine_tokens(const void* y, const SlotTables& a, const int3
   hipLaunchKernelGGL((combine_tokens_kernel<DT, TPR, SCAN>), grid, dim3(256), 0, s, (const uint8_t*)y, a, tp2id, T, H, (uint8_t*)out)
   if (wide && tp2id) MOE_COMBINE(256, true);
   else if (wide) MOE_COMBINE(256, false);
-  else if (tp2id) MOE_COMBINE(64, true);
   else MOE_COMBINE(64, false);
 #undef MOE_COMBINE
 }
@@ -477,16 +505,24 @@ extern "C" int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtyp
   const hipStream_t s = (hipStream_t)stream;
   const int rc = begin_by_list(a, T, T1, token_position_to_id, build_token_slots, true, s);
   if (rc != MOE_OK) return rc;
-  const unsigned grid = grid_of(T + (S + PAD_SLOTS - 1) / PAD_SLOTS + 1);
-  switch (dtype) {
+  const int64_t jobs = T + (S + PAD_SLOTS - 1) / PAD_SLOTS + 1;
+  const int64_t row_bytes = H * (dtype == MOE_DT_FP32 ? 4 : 2);
 #define MOE_BWD(DT)                                                                                                             \
-  hipLaunchKernelGGL(combine_tokens_bwd_kernel<DT>, dim3(grid), dim3(256), 0, s, (const uint8_t*)d_out, (const uint8_t*)y, a,   \
-                     token_position_to_id, S, T, T1, H, (uint8_t*)d_y, d_affinities)
+  do {                                                                                                                          \
+    if (row_bytes > SHORT_ROW)                                                                                                  \
+      hipLaunchKernelGGL((combine_tokens_bwd_kernel<DT, 256>), dim3(grid_of(jobs)), dim3(256), 0, s, (const uint8_t*)d_out,     \
+                         (const uint8_t*)y, a, token_position_to_id, S, T, T1, H, (uint8_t*)d_y, d_affinities);                 \
+    else                                                                                                                        \
+      hipLaunchKernelGGL((combine_tokens_bwd_kernel<DT, 64>), dim3(grid_of((jobs + 3) / 4)), dim3(256), 0, s,                   \
+                         (const uint8_t*)d_out, (const uint8_t*)y, a, token_position_to_id, S, T, T1, H, (uint8_t*)d_y,         \
+                         d_affinities);                                                                                         \
+  } while (0)
+  switch (dtype) {
     case MOE_DT_BF16: MOE_BWD(MOE_DT_BF16); break;
     case MOE_DT_FP16: MOE_BWD(MOE_DT_FP16); break;
     default: MOE_BWD(MOE_DT_FP32); break;
-#undef MOE_BWD
   }
+#undef MOE_BWD
   MOE_CHECK_LAUNCH();
   return MOE_OK;
 }

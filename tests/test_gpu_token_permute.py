@@ -117,6 +117,41 @@ def test_combine_and_gradient(shape, dtype):
     assert_within(d_aff, want_a, bound(want_a, mag_a, "float32", H / 64 + 16), f"d_aff {shape} {dtype}")
 
 
+# many tokens: rows of a wave each up to 4096 bytes, of a workgroup each beyond; more than eight slots; no token in the last ones
+@pytest.mark.parametrize("shape", [(3855, 65, 128, 3, 16), (2048, 3, 8, 2, 16), (2047, 1024, 16, 4, 32), (2100, 1025, 24, 9, 32),
+                                   (2500, 2048, 16, 2, 64), (2048, 2049, 16, 2, 64)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_tokens_with_short_rows(shape, dtype):
+    import torch
+    from nkilib.core.moe.token_permute import combine_tokens, combine_tokens_bwd, permute_tokens, permute_tokens_bwd
+
+    T, H, E, k, B = shape
+    rng, tp2id, b2e, tp, be, aff, y = _case(shape, dtype, T + H, skip_token=True)
+    a, yv = values(aff), values(y)
+    d = tensor(rng.standard_normal((T, H)), dtype)
+    assert np.array_equal(values(permute_tokens(d, tp)), ot.permute(values(d), tp2id))
+    want, mag = ot.combine(yv, a, tp2id, b2e, B, T)
+    assert_within(combine_tokens(y, aff, tp, be, B, T, k), want, bound(want, mag, dtype, k + 1), f"{shape} {dtype}")
+    want, mag = ot.combine(yv, None, tp2id, b2e, B, T)
+    assert_within(permute_tokens_bwd(y, tp, T, k), want, bound(want, mag, dtype, k + 1), f"{shape} {dtype}")
+    want_y, want_a, mag_a = ot.combine_bwd(values(d), yv, a, tp2id, b2e, B)
+    d_y, d_aff = combine_tokens_bwd(d, y, aff, tp, be, B, k)
+    assert_within(d_y, want_y, bound(want_y, np.abs(want_y), dtype, 1), f"d_y {shape} {dtype}")
+    assert_within(d_aff, want_a, bound(want_a, mag_a, "float32", H / 64 + 16), f"d_aff {shape} {dtype}")
+    # a token listed more often than the caller said: NaN for it, in each of the three, and for no other
+    often = torch.zeros(T, dtype=torch.int32)
+    ids = torch.from_numpy(tp2id).long()
+    often.index_add_(0, ids[(ids >= 0) & (ids < T)], torch.ones(int(((ids >= 0) & (ids < T)).sum()), dtype=torch.int32))
+    cut = (often > k - 1).numpy()
+    got = values(combine_tokens(y, aff, tp, be, B, T, k - 1))
+    assert np.array_equal(np.isnan(got).all(1), cut) and np.array_equal(np.isnan(got).any(1), cut)
+    cut_y, cut_a = combine_tokens_bwd(d, y, aff, tp, be, B, k - 1)
+    assert np.array_equal(np.isnan(values(cut_a)).all(1)[:T], cut) and not np.isnan(values(cut_a)[T:]).any()
+    held = (tp2id >= 0) & (tp2id < T)
+    want_nan = held & cut[np.where(held, tp2id, 0)]
+    assert np.array_equal(np.isnan(values(cut_y)).all(1), want_nan) and np.array_equal(np.isnan(values(cut_y)).any(1), want_nan)
+
+
 def test_padding_rows_are_not_read_and_bad_experts_count_for_nothing():
     """NaN in padding rows of y and in rows behind the tokens of the affinities; a block whose expert is -1, or E."""
     import torch
