@@ -22,7 +22,7 @@
 //                              power leaves, and router_dx_list_kernel, by the vector ALU: 75 instructions a token and 256
 //                              columns, half of them to unpack w);
 //   3. router_reduce_kernel    the sums of the parts of dw and of db (large calls: the workgroups of dx, when done).
-// T = 8192, H = 7168, E = 256, top-8: 8.4 + 56 + 50 us of 52 for its bytes at the rate of a copy and 50 for 2 x 2 x 30 GFLOP at
+// T = 8192, H = 7168, E = 256, top-8: 9 + 57 + 50 us; 52 for its bytes at the rate of a copy and 50 for 2 x 2 x 30 GFLOP at
 // that of a large product.
 #include <type_traits>
 

@@ -438,9 +438,10 @@ template <int DT>
 static void launch_combine_tokens(const void* y, const SlotTables& a, const int32_t* tp2id, int64_t T, int64_t H, void* out,
                                   hipStream_t s) {
   // a workgroup per token, or a wave where rows are short and tokens many (us a call, top-8 of 128 experts, caches cold, wave and
-  // workgroup: 1024 tokens of 1 KB 15.6 and 15.6, 3 KB 19.6 and 18.3; 8192 of 1 KB 35 and 37, 3 KB 59 and 68, 8 KB 130 and 125);
-  // few tokens (decode): several per token, a piece per thread
-  const bool wide = H * Elem<DT>::SIZE > SHORT_ROW || T < 2048;
+  // workgroup: 1024 tokens of 1 KB 15.6 and 15.6, 3 KB 19.6 and 18.3; 8192 of 1 KB 35 and 37, 3 KB 59 and 68, 8 KB 130 and 125;
+  // the kernel for 8192 of 4 KB, whose pieces a workgroup has one of per thread, weighted 62 and 64, else 59 and 52); few tokens
+  // (decode): several per token, a piece per thread
+  const bool wide = H * Elem<DT>::SIZE >= SHORT_ROW || T < 2048;
   const int64_t groups = wide ? T : (T + 3) / 4;
   int64_t parts = 1;
   if (wide && groups < 512) {
