@@ -413,7 +413,9 @@ int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtype, const vo
  * moe_glu_checkpoint: gate_up [R, 2, I] -> intermediate [R, I] = act(gate) * up and the record of the clamped values.
  * moe_pack_gate_up_checkpoint: the same record of what moe_blockwise left in gate_up_activations_T (bf16 [N, 2, I, B]; R = N*B).
  * moe_glu_checkpoint_bwd: the record and d_intermediate [R, I] -> d_gate_up [R, 2, I] (zero where the recorded value lies at or
- * beyond its clamp) and, unless NULL, intermediate [R, I] of the recorded values (what the down weights' gradient needs).
+ * beyond its limit as the record holds that: rounded to e4m3 as a clamped value is, from fp32 or by way of the checkpoint's bf16.
+ * Values up to half a step inside are recorded alike and count as clamped) and, unless NULL, intermediate [R, I] of the recorded
+ * values (what the down weights' gradient needs).
  * moe_dequantize_checkpoint: `rows` rows of I codes with ceil(I/32) scales each -> values (bf16 holds them exactly, down to 2^-133). */
 int moe_glu_checkpoint(const void* gate_up, int dtype, int64_t R, int64_t I, int act_fn, int clamp_mask,
                        const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens, void* intermediate,

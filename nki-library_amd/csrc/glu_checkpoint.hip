@@ -12,6 +12,10 @@
 //   backward   record, dh -> du = dh act(g), dg = dh u act'(g) (0 at and beyond a clamp), and h again for the down weights'
 //              gradient
 //
+// A clamped value is recorded as its limit rounded to e4m3 (7.2 as 7.0 or as 7.5, as the scale has it), so a record's value is at its
+// clamp where it reaches what the record makes of the limit in its group, not the limit itself.  Values that were not clamped but
+// round to the same code, up to half a step inside, cannot be told from those and count as clamped.
+//
 // act(x) = x s(x) for every kind: SiLU and Swish s = sigmoid(a x); GELU s = Phi(x); its tanh form 0.5 (1 + tanh z) = sigmoid(2 z).
 // All of it moves bytes: a pair of values costs 4 + 2 + 2 + 1/16 bytes forward in bf16, 2 + 1/16 + 2 + 4 + 2 backward.  Four lanes
 // share a group of 32, eight values each (16 bytes of bf16), so that a group's maximum is two exchanges between neighbours.
@@ -32,6 +36,7 @@ struct GluArgs {
   uint32_t v_magic;      // ceil(2^32 / V)
   int act_fn, clamp_mask;
   float clamp[4];        // gate upper, gate lower, up upper, up lower
+  float clamp16[4];      // the same as bf16 holds them: what the layer's checkpoint has of a clamped value
 };
 
 // s(x) and x s'(x).  EXACT (fp32 rows): the exponent's rounding is made good; it costs up to |z| / 2 units of the last place, which
@@ -116,6 +121,21 @@ __device__ __forceinline__ void decode8(const uint2& c, uint32_t byte, float (&v
     v[4 * h + 2] = b[0] * s;
     v[4 * h + 3] = b[1] * s;
   }
+}
+// The limits of a gate or up group as its record holds them.  The value recorded is the limit itself or, by way of moe_cte's checkpoint,
+// its bf16, which may round to another code (7.2503 to 7.5, its bf16 7.25 to 7.0): the one further inside.  A limit above 448 times the
+// scale is above every value of the group and stays what it is.
+__device__ __forceinline__ void recorded_limits(const GluArgs& a, int upper, uint32_t byte, float& hi, float& lo) {
+  const float inv = mx_inv_scale(byte), s = scale_value(byte);
+  const float v[4] = {a.clamp[upper], a.clamp16[upper], a.clamp[upper + 1], a.clamp16[upper + 1]};
+  const int w = (int)pack4_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+  const v2f h = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), l = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+  const float r[4] = {h[0] * s, h[1] * s, l[0] * s, l[1] * s};
+  float q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = fabsf(v[i] * inv) <= 448.f ? r[i] : v[i];
+  hi = fminf(q[0], q[1]);
+  lo = fmaxf(q[2], q[3]);
 }
 
 // n of eight values of a row at p (n = 8 except at the end of a row whose length is no multiple of eight)
@@ -258,6 +278,11 @@ __global__ __launch_bounds__(256) void glu_checkpoint_bwd_kernel(const GluArgs a
     load8<DT>(dh + (p.row * a.I + 8 * p.v) * ES, p.n, d);
     decode8(cg, sg, g);
     decode8(cu, su, u);
+    float g_hi = 0.f, g_lo = 0.f, u_hi = 0.f, u_lo = 0.f;
+    if (a.clamp_mask) {
+      recorded_limits(a, 0, sg, g_hi, g_lo);
+      recorded_limits(a, 2, su, u_hi, u_lo);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       bool in_g = true, in_u = true;
@@ -265,9 +290,8 @@ __global__ __launch_bounds__(256) void glu_checkpoint_bwd_kernel(const GluArgs a
         const float g0 = g[i], u0 = u[i];
         g[i] = clamp_value(g0, a.clamp_mask, MOE_CLAMP_GATE_HI, MOE_CLAMP_GATE_LO, a.clamp[0], a.clamp[1]);
         u[i] = clamp_value(u0, a.clamp_mask, MOE_CLAMP_UP_HI, MOE_CLAMP_UP_LO, a.clamp[2], a.clamp[3]);
-        // a recorded value at its limit is one that the forward pass clamped
-        in_g = !(((a.clamp_mask & MOE_CLAMP_GATE_HI) && g0 >= a.clamp[0]) || ((a.clamp_mask & MOE_CLAMP_GATE_LO) && g0 <= a.clamp[1]));
-        in_u = !(((a.clamp_mask & MOE_CLAMP_UP_HI) && u0 >= a.clamp[2]) || ((a.clamp_mask & MOE_CLAMP_UP_LO) && u0 <= a.clamp[3]));
+        in_g = !(((a.clamp_mask & MOE_CLAMP_GATE_HI) && g0 >= g_hi) || ((a.clamp_mask & MOE_CLAMP_GATE_LO) && g0 <= g_lo));
+        in_u = !(((a.clamp_mask & MOE_CLAMP_UP_HI) && u0 >= u_hi) || ((a.clamp_mask & MOE_CLAMP_UP_LO) && u0 <= u_lo));
       }
       float s, xds;
       act_parts<ACT, DT == MOE_DT_FP32>(g[i], s, xds);
@@ -375,6 +399,15 @@ __global__ __launch_bounds__(256) void pack_checkpoint_kernel(const uint16_t* __
 
 using namespace moe;
 
+// bf16 of a value, rounded to the nearest even.
+static float as_bf16(float f) {
+  uint32_t u;
+  __builtin_memcpy(&u, &f, 4);
+  if ((u & 0x7fffffffu) < 0x7f800000u) u += 0x7fffu + ((u >> 16) & 1u);
+  u &= 0xffff0000u;
+  __builtin_memcpy(&f, &u, 4);
+  return f;
+}
 static int glu_args(GluArgs& a, int64_t R, int64_t I, int act_fn, int clamp_mask, const float* clamps, const int32_t* tp2id,
                     int64_t n_tokens) {
   if (R < 0 || I < 1 || n_tokens < 0) return MOE_E_BAD_ARG;
@@ -389,7 +422,10 @@ static int glu_args(GluArgs& a, int64_t R, int64_t I, int act_fn, int clamp_mask
   a.v_magic = (uint32_t)((((uint64_t)1 << 32) + a.V - 1) / a.V);
   a.act_fn = act_fn;
   a.clamp_mask = clamp_mask;
-  for (int i = 0; i < 4; ++i) a.clamp[i] = clamp_mask ? clamps[i] : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    a.clamp[i] = clamp_mask ? clamps[i] : 0.f;
+    a.clamp16[i] = as_bf16(a.clamp[i]);
+  }
   return MOE_OK;
 }
 // Rows per launch: fewer than 2^32 threads, and at least one row.

@@ -122,8 +122,10 @@ def glu_checkpoint_bwd(codes: torch.Tensor, scales: torch.Tensor, d_intermediate
                        n_tokens: Optional[int] = None, return_intermediate: bool = True):
     """Gradient of ``act(gate) * up`` at the recorded values: ``d_intermediate`` ``[R, I]`` -> ``d_gate_up`` ``[R, 2, I]`` of its
     type and, with ``return_intermediate``, the recomputed ``intermediate`` ``[R, I]`` (the other factor of the down weights'
-    gradient; ``None`` without).  Where a recorded value lies at its clamp or beyond, the forward pass clamped it and its
-    gradient is zero."""
+    gradient; ``None`` without).  Where a recorded value lies at or beyond its limit, its gradient is zero.  A clamped value
+    is recorded as its limit rounded to e4m3 (7.2 as 7.0, or 7.5, as the group's scale has it), so the limit is taken as the record
+    holds it: no clamped value passes a gradient.  Values that were not clamped but are recorded alike, up to half a step (1/16)
+    inside the limit, pass none either."""
     codes, scales, R, I = _record(codes, scales)
     d = nv.require_device_tensor(d_intermediate, "d_intermediate")
     if d.shape != (R, I) or d.device != codes.device:

@@ -126,12 +126,37 @@ def clamp_glu(gate, up, clamps):
     return gate, up
 
 
-def glu_bwd(gate, up, d, kind, clamps=(None,) * 4):
-    """(d_gate, d_up, h) at the recorded values; zero at and beyond a clamp."""
+def recorded_limit(limit, scales, I):
+    """What the record of a clamped value holds, per value of rows [..., I] with `scales` [..., ceil(I/32)]: the limit as one of its
+    group's e4m3 values; the limit itself where it lies beyond all of them (no value of the group met it)."""
+    s = np.exp2(np.repeat(scales.astype(np.float64) - 127, 32, axis=-1)[..., :I])
+    v = limit / s
+    code = e4m3fn_encode(np.clip(v, -448, 448).astype(np.float32))
+    return np.where(np.abs(v) <= 448, E4M3FN_TABLE[code].astype(np.float64) * s, limit)
+
+
+def bf16_value(x):
+    u = np.asarray(x, np.float32).reshape(1).view(np.uint32).astype(np.uint64)
+    u = (u + 0x7FFF + ((u >> np.uint64(16)) & np.uint64(1))) & np.uint64(0xFFFF0000)
+    return float(u.astype(np.uint32).view(np.float32)[0])
+
+
+def reaches(v, limit, upper, scales=None):
+    """Where recorded values are at their clamp or beyond.  With `scales`, at what the record holds of it: of the limit or of its
+    bf16 (the layer's checkpoint), whichever lies further inside.  Without, limits that every group holds."""
+    if limit is None:
+        return np.zeros(v.shape, bool)
+    at = [limit] if scales is None else [recorded_limit(l, scales, v.shape[-1]) for l in (limit, bf16_value(limit))]
+    return v >= np.minimum.reduce(at) if upper else v <= np.maximum.reduce(at)
+
+
+def glu_bwd(gate, up, d, kind, clamps=(None,) * 4, scales=None):
+    """(d_gate, d_up, h) at the recorded values; zero at and beyond a clamp.  scales: the record's, [..., 2, ceil(I/32)]."""
     g, u = clamp_glu(gate, up, clamps)
     gh, gl, uh, ul = clamps
-    in_g = np.ones(gate.shape, bool) & (True if gh is None else ~(gate >= gh)) & (True if gl is None else ~(gate <= gl))
-    in_u = np.ones(up.shape, bool) & (True if uh is None else ~(up >= uh)) & (True if ul is None else ~(up <= ul))
+    sg, su = (None, None) if scales is None else (scales[..., 0, :], scales[..., 1, :])
+    in_g = ~(reaches(gate, gh, True, sg) | reaches(gate, gl, False, sg))
+    in_u = ~(reaches(up, uh, True, su) | reaches(up, ul, False, su))
     a, da = act(g, kind)
     return np.where(in_g, d * u * da, 0.0), np.where(in_u, d * a, 0.0), a * u
 

@@ -76,6 +76,26 @@ def test_record_takes_the_smallest_scale_and_the_nearest_value():
             assert abs(v[r, c] - x[r, c]) == np.abs(finite * s - x[r, c]).min()
 
 
+@pytest.mark.parametrize("limit", [7.0, 7.2, 10.5, 20.6, 6.2, 1.1, 0.9, -0.7, 7.2503, 0.0, 1e-3, 500.0])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_clamped_values_are_clamped_in_the_record(limit, bf16):
+    """Values clamped at the limit (kept as bf16 between, or not) lie at their clamp in the record, those far inside do not."""
+    rng = np.random.default_rng(6)
+    x = (rng.standard_normal((50, 160)) * np.exp2(rng.integers(-4, 9, (50, 1)))).astype(np.float32)
+    for upper in (True, False):
+        v = np.minimum(x, np.float32(limit)) if upper else np.maximum(x, np.float32(limit))
+        if bf16:
+            v = np.vectorize(ot.bf16_value, otypes=[np.float32])(v)
+        codes, scales = ot.record(v)
+        rec = ot.record_values(codes, scales)
+        got = ot.reaches(rec, float(np.float32(limit)), upper, scales)
+        out = x >= np.float32(limit) if upper else x <= np.float32(limit)
+        assert got[out].all()
+        far = abs(limit) / 8 + np.repeat(np.exp2(scales.astype(np.float64) - 127), 32, axis=1)[:, : x.shape[1]] / 512
+        inside = x < limit - far if upper else x > limit + far
+        assert inside.any() and not got[inside].any()
+
+
 @pytest.mark.parametrize("softmax", [True, False])
 @pytest.mark.parametrize("pre_norm,norm", [(True, True), (True, False), (False, False)])
 def test_router_gradient_against_differences(softmax, pre_norm, norm):
