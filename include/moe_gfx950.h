@@ -416,6 +416,9 @@ int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtype, const vo
  * beyond its limit as the record holds that: rounded to e4m3 as a clamped value is, from fp32 or by way of the checkpoint's bf16.
  * Values up to half a step inside are recorded alike and count as clamped) and, unless NULL, intermediate [R, I] of the recorded
  * values (what the down weights' gradient needs).
+ * moe_..._clamped: the same with clamped uint8 [R, 2, ceil(I/8)] (nullable), bit i of byte v for value 8 v + i of a row, written by
+ * the first two: set where a value lay at or beyond its limit ahead of the clamp (pack: where the checkpoint holds its limit, as bf16,
+ * or more; clamp_mask and clamps have no other use there).  moe_glu_checkpoint_bwd_clamped passes a gradient where it is not set.
  * moe_dequantize_checkpoint: `rows` rows of I codes with ceil(I/32) scales each -> values (bf16 holds them exactly, down to 2^-133). */
 int moe_glu_checkpoint(const void* gate_up, int dtype, int64_t R, int64_t I, int act_fn, int clamp_mask,
                        const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens, void* intermediate,
@@ -427,6 +430,16 @@ int moe_glu_checkpoint_bwd(const uint8_t* codes, const uint8_t* scales, const vo
                            int64_t I, int act_fn, int clamp_mask, const float* clamps,
                            const int32_t* token_position_to_id, int64_t n_tokens, void* d_gate_up, void* intermediate,
                            void* stream);
+int moe_glu_checkpoint_clamped(const void* gate_up, int dtype, int64_t R, int64_t I, int act_fn, int clamp_mask,
+                               const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens,
+                               void* intermediate, uint8_t* codes, uint8_t* scales, uint8_t* clamped, void* stream);
+int moe_pack_gate_up_checkpoint_clamped(const void* gate_up_activations_T, int64_t N, int64_t I, int64_t B, int clamp_mask,
+                                        const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens,
+                                        uint8_t* codes, uint8_t* scales, uint8_t* clamped, void* stream);
+int moe_glu_checkpoint_bwd_clamped(const uint8_t* codes, const uint8_t* scales, const uint8_t* clamped,
+                                   const void* d_intermediate, int dtype, int64_t R, int64_t I, int act_fn, int clamp_mask,
+                                   const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens,
+                                   void* d_gate_up, void* intermediate, void* stream);
 int moe_dequantize_checkpoint(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t I, void* out, int dtype,
                               void* stream);
 

@@ -14,7 +14,8 @@
 //
 // A clamped value is recorded as its limit rounded to e4m3 (7.2 as 7.0 or as 7.5, as the scale has it), so a record's value is at its
 // clamp where it reaches what the record makes of the limit in its group, not the limit itself.  Values that were not clamped but
-// round to the same code, up to half a step inside, cannot be told from those and count as clamped.
+// round to the same code, up to half a step inside, cannot be told from those and count as clamped, unless the forward pass also keeps a
+// bit per value (`clamped`, an eighth of a record's bytes, one for the eight values of a lane) and the backward pass goes by those.
 //
 // act(x) = x s(x) for every kind: SiLU and Swish s = sigmoid(a x); GELU s = Phi(x); its tanh form 0.5 (1 + tanh z) = sigmoid(2 z).
 // All of it moves bytes: a pair of values costs 4 + 2 + 2 + 1/16 bytes forward in bf16, 2 + 1/16 + 2 + 4 + 2 backward.  Four lanes
@@ -37,6 +38,7 @@ struct GluArgs {
   int act_fn, clamp_mask;
   float clamp[4];        // gate upper, gate lower, up upper, up lower
   float clamp16[4];      // the same as bf16 holds them: what the layer's checkpoint has of a clamped value
+  uint8_t* clamped;      // [R][2][ceil(I/8)] or null: bit i of byte v for value 8 v + i
 };
 
 // s(x) and x s'(x).  EXACT (fp32 rows): the exponent's rounding is made good; it costs up to |z| / 2 units of the last place, which
@@ -75,6 +77,11 @@ __device__ __forceinline__ float clamp_value(float x, int mask, int hi_bit, int 
   if ((mask & hi_bit) && x > hi) x = hi;
   if ((mask & lo_bit) && x < lo) x = lo;
   return x;
+}
+
+// (NaN is at no limit)
+__device__ __forceinline__ bool at_limit(float x, int mask, int hi_bit, int lo_bit, float hi, float lo) {
+  return ((mask & hi_bit) && x >= hi) || ((mask & lo_bit) && x <= lo);
 }
 
 __device__ __forceinline__ uint32_t max_finite(uint32_t m, float v) {
@@ -236,12 +243,16 @@ __global__ __launch_bounds__(256) void glu_checkpoint_kernel(const GluArgs a, co
     load8<DT>(gate_up + off * ES, p.n, g);
     load8<DT>(gate_up + (off + a.I) * ES, p.n, u);
   }
+  uint32_t at_g = 0, at_u = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (a.clamp_mask) {
+      const bool real = p.on && i < p.n;
+      if (real && at_limit(g[i], a.clamp_mask, MOE_CLAMP_GATE_HI, MOE_CLAMP_GATE_LO, a.clamp[0], a.clamp[1])) at_g |= 1u << i;
+      if (real && at_limit(u[i], a.clamp_mask, MOE_CLAMP_UP_HI, MOE_CLAMP_UP_LO, a.clamp[2], a.clamp[3])) at_u |= 1u << i;
       g[i] = clamp_value(g[i], a.clamp_mask, MOE_CLAMP_GATE_HI, MOE_CLAMP_GATE_LO, a.clamp[0], a.clamp[1]);
       u[i] = clamp_value(u[i], a.clamp_mask, MOE_CLAMP_UP_HI, MOE_CLAMP_UP_LO, a.clamp[2], a.clamp[3]);
-      if (!p.on || i >= p.n) g[i] = u[i] = 0.f;
+      if (!real) g[i] = u[i] = 0.f;
     }
     float s, xds;
     act_parts<ACT, DT == MOE_DT_FP32>(g[i], s, xds);
@@ -252,6 +263,11 @@ __global__ __launch_bounds__(256) void glu_checkpoint_kernel(const GluArgs a, co
     store8<DT>(h + (p.row * a.I + 8 * p.v) * ES, p.n, r);
     store_codes(codes + off, p.n, encode8(g, sg));
     store_codes(codes + off + a.I, p.n, encode8(u, su));
+    if (a.clamped) {
+      const int64_t G8 = (a.I + 7) / 8;
+      a.clamped[p.row * 2 * G8 + p.v] = (uint8_t)at_g;
+      a.clamped[p.row * 2 * G8 + G8 + p.v] = (uint8_t)at_u;
+    }
   }
   if ((p.v & 3) == 0) {
     scales[p.row * 2 * G + p.v / 4] = (uint8_t)sg;
@@ -279,19 +295,26 @@ __global__ __launch_bounds__(256) void glu_checkpoint_bwd_kernel(const GluArgs a
     decode8(cg, sg, g);
     decode8(cu, su, u);
     float g_hi = 0.f, g_lo = 0.f, u_hi = 0.f, u_lo = 0.f;
-    if (a.clamp_mask) {
+    uint32_t at_g = 0, at_u = 0;
+    if (a.clamped) {
+      const int64_t G8 = (a.I + 7) / 8;
+      at_g = a.clamped[p.row * 2 * G8 + p.v];
+      at_u = a.clamped[p.row * 2 * G8 + G8 + p.v];
+    } else if (a.clamp_mask) {
       recorded_limits(a, 0, sg, g_hi, g_lo);
       recorded_limits(a, 2, su, u_hi, u_lo);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      bool in_g = true, in_u = true;
+      bool in_g = !(at_g >> i & 1), in_u = !(at_u >> i & 1);
       if (a.clamp_mask) {
         const float g0 = g[i], u0 = u[i];
         g[i] = clamp_value(g0, a.clamp_mask, MOE_CLAMP_GATE_HI, MOE_CLAMP_GATE_LO, a.clamp[0], a.clamp[1]);
         u[i] = clamp_value(u0, a.clamp_mask, MOE_CLAMP_UP_HI, MOE_CLAMP_UP_LO, a.clamp[2], a.clamp[3]);
-        in_g = !(((a.clamp_mask & MOE_CLAMP_GATE_HI) && g0 >= g_hi) || ((a.clamp_mask & MOE_CLAMP_GATE_LO) && g0 <= g_lo));
-        in_u = !(((a.clamp_mask & MOE_CLAMP_UP_HI) && u0 >= u_hi) || ((a.clamp_mask & MOE_CLAMP_UP_LO) && u0 <= u_lo));
+        if (!a.clamped) {
+          in_g = !at_limit(g0, a.clamp_mask, MOE_CLAMP_GATE_HI, MOE_CLAMP_GATE_LO, g_hi, g_lo);
+          in_u = !at_limit(u0, a.clamp_mask, MOE_CLAMP_UP_HI, MOE_CLAMP_UP_LO, u_hi, u_lo);
+        }
       }
       float s, xds;
       act_parts<ACT, DT == MOE_DT_FP32>(g[i], s, xds);
@@ -325,8 +348,13 @@ __global__ __launch_bounds__(256) void dequantize_checkpoint_kernel(const GluArg
 // a row and a group of 32 columns per thread.  Two bytes per value from LDS: neighbouring lanes hold neighbouring rows.
 // (Groups lie max(8, tb) values apart beyond their length, so that lanes of several groups do not meet in a bank.)
 constexpr int PACK_TILE = 8192;
+// The limits of gate and of up as the checkpoint holds them (bf16; NaN, which nothing reaches, where there is none), for `out`: which values lie there.
+struct PackClamps {
+  float hi[2], lo[2];
+  uint8_t* out;  // [N B][2][ceil(I/8)] or null
+};
 __global__ __launch_bounds__(256) void pack_checkpoint_kernel(const uint16_t* __restrict__ x, const int32_t* __restrict__ tp2id,
-                                                              int64_t n_tokens, int64_t I, int64_t B, int ltb,
+                                                              int64_t n_tokens, int64_t I, int64_t B, int ltb, const PackClamps at,
                                                               uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   __shared__ __attribute__((aligned(16))) uint16_t s_x[PACK_TILE + PACK_TILE / 32 * 8];
   const int tid = threadIdx.x, tb = 1 << ltb, tc = PACK_TILE >> ltb, pad = tb > 8 ? tb : 8;
@@ -348,7 +376,7 @@ __global__ __launch_bounds__(256) void pack_checkpoint_kernel(const uint16_t* __
   }
   const bool any = __syncthreads_or(on);
   const uint16_t* src = x + ((blk * 2 + z) * I + c0) * B + r0;
-  auto at = [&](int c, int row) { return c / 32 * (32 * tb + pad) + (c % 32) * tb + row; };
+  auto place = [&](int c, int row) { return c / 32 * (32 * tb + pad) + (c % 32) * tb + row; };
   if (any) {
     if (((B % 8 == 0 && tb >= 8) || B == tb) && ((uintptr_t)src & 15) == 0 && nc * tb % 8 == 0) {
       u32x4 d[4];
@@ -361,12 +389,12 @@ __global__ __launch_bounds__(256) void pack_checkpoint_kernel(const uint16_t* __
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int e = 8 * (tid + 256 * q);
-        *(u32x4*)(s_x + at(e >> ltb, e & (tb - 1))) = d[q];
+        *(u32x4*)(s_x + place(e >> ltb, e & (tb - 1))) = d[q];
       }
     } else {
       for (int e = tid; e < PACK_TILE; e += 256) {
         const int c = e >> ltb, row = e & (tb - 1);
-        s_x[at(c, row)] = c < nc && row < nr ? src[(int64_t)c * B + row] : (uint16_t)0;
+        s_x[place(c, row)] = c < nc && row < nr ? src[(int64_t)c * B + row] : (uint16_t)0;
       }
     }
   }
@@ -393,6 +421,18 @@ __global__ __launch_bounds__(256) void pack_checkpoint_kernel(const uint16_t* __
     if (n > 0) store_codes<false>(dst + 8 * q, n > 8 ? 8 : n, encode8(part, s));
   }
   scales[row * G + c0 / 32 + cg] = (uint8_t)s;
+  if (at.out) {
+    const float hi = z ? at.hi[1] : at.hi[0], lo = z ? at.lo[1] : at.lo[0];
+    uint8_t* bytes = at.out + row * ((I + 7) / 8) + c0 / 8 + 4 * cg;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (on && 8 * q + e < left && (v[8 * q + e] >= hi || v[8 * q + e] <= lo)) m |= 1u << e;
+      if (8 * q < left) bytes[q] = (uint8_t)m;
+    }
+  }
 }
 
 }  // namespace moe
@@ -422,6 +462,7 @@ static int glu_args(GluArgs& a, int64_t R, int64_t I, int act_fn, int clamp_mask
   a.v_magic = (uint32_t)((((uint64_t)1 << 32) + a.V - 1) / a.V);
   a.act_fn = act_fn;
   a.clamp_mask = clamp_mask;
+  a.clamped = nullptr;
   for (int i = 0; i < 4; ++i) {
     a.clamp[i] = clamp_mask ? clamps[i] : 0.f;
     a.clamp16[i] = as_bf16(a.clamp[i]);
@@ -450,9 +491,9 @@ static int by_dtype(int dtype, F&& f) {
   }
 }
 
-extern "C" int moe_glu_checkpoint(const void* gate_up, int dtype, int64_t R, int64_t I, int act_fn, int clamp_mask,
-                                  const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens,
-                                  void* intermediate, uint8_t* codes, uint8_t* scales, void* stream) {
+extern "C" int moe_glu_checkpoint_clamped(const void* gate_up, int dtype, int64_t R, int64_t I, int act_fn, int clamp_mask,
+                                          const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens,
+                                          void* intermediate, uint8_t* codes, uint8_t* scales, uint8_t* clamped, void* stream) {
   if (!gate_up || !intermediate || !codes || !scales) return MOE_E_BAD_ARG;
   GluArgs a;
   const int rc = glu_args(a, R, I, act_fn, clamp_mask, clamps, token_position_to_id, n_tokens);
@@ -465,6 +506,7 @@ extern "C" int moe_glu_checkpoint(const void* gate_up, int dtype, int64_t R, int
         GluArgs p = a;
         p.R = R - r0 < per ? R - r0 : per;
         if (p.tp2id) p.tp2id += r0;
+        if (clamped) p.clamped = clamped + r0 * 2 * ((I + 7) / 8);
         hipLaunchKernelGGL((glu_checkpoint_kernel<DT, decltype(act)::value>), dim3((unsigned)((p.R * p.V + 255) / 256)), dim3(256),
                            0, (hipStream_t)stream, p, (const uint8_t*)gate_up + r0 * 2 * I * ES,
                            (uint8_t*)intermediate + r0 * I * ES, codes + r0 * 2 * I, scales + r0 * (p.V / 2));
@@ -475,10 +517,17 @@ extern "C" int moe_glu_checkpoint(const void* gate_up, int dtype, int64_t R, int
   });
 }
 
-extern "C" int moe_glu_checkpoint_bwd(const uint8_t* codes, const uint8_t* scales, const void* d_intermediate, int dtype, int64_t R,
-                                      int64_t I, int act_fn, int clamp_mask, const float* clamps,
-                                      const int32_t* token_position_to_id, int64_t n_tokens, void* d_gate_up,
-                                      void* intermediate, void* stream) {
+extern "C" int moe_glu_checkpoint(const void* gate_up, int dtype, int64_t R, int64_t I, int act_fn, int clamp_mask,
+                                  const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens,
+                                  void* intermediate, uint8_t* codes, uint8_t* scales, void* stream) {
+  return moe_glu_checkpoint_clamped(gate_up, dtype, R, I, act_fn, clamp_mask, clamps, token_position_to_id, n_tokens, intermediate,
+                                    codes, scales, nullptr, stream);
+}
+
+extern "C" int moe_glu_checkpoint_bwd_clamped(const uint8_t* codes, const uint8_t* scales, const uint8_t* clamped,
+                                              const void* d_intermediate, int dtype, int64_t R, int64_t I, int act_fn,
+                                              int clamp_mask, const float* clamps, const int32_t* token_position_to_id,
+                                              int64_t n_tokens, void* d_gate_up, void* intermediate, void* stream) {
   if (!codes || !scales || !d_intermediate || !d_gate_up) return MOE_E_BAD_ARG;
   GluArgs a;
   const int rc = glu_args(a, R, I, act_fn, clamp_mask, clamps, token_position_to_id, n_tokens);
@@ -491,6 +540,7 @@ extern "C" int moe_glu_checkpoint_bwd(const uint8_t* codes, const uint8_t* scale
         GluArgs p = a;
         p.R = R - r0 < per ? R - r0 : per;
         if (p.tp2id) p.tp2id += r0;
+        if (clamped) p.clamped = const_cast<uint8_t*>(clamped) + r0 * 2 * ((I + 7) / 8);
         hipLaunchKernelGGL((glu_checkpoint_bwd_kernel<DT, decltype(act)::value>), dim3((unsigned)((p.R * p.V + 255) / 256)),
                            dim3(256), 0, (hipStream_t)stream, p, codes + r0 * 2 * I, scales + r0 * (p.V / 2),
                            (const uint8_t*)d_intermediate + r0 * I * ES, (uint8_t*)d_gate_up + r0 * 2 * I * ES,
@@ -500,6 +550,14 @@ extern "C" int moe_glu_checkpoint_bwd(const uint8_t* codes, const uint8_t* scale
       return MOE_OK;
     });
   });
+}
+
+extern "C" int moe_glu_checkpoint_bwd(const uint8_t* codes, const uint8_t* scales, const void* d_intermediate, int dtype, int64_t R,
+                                      int64_t I, int act_fn, int clamp_mask, const float* clamps,
+                                      const int32_t* token_position_to_id, int64_t n_tokens, void* d_gate_up,
+                                      void* intermediate, void* stream) {
+  return moe_glu_checkpoint_bwd_clamped(codes, scales, nullptr, d_intermediate, dtype, R, I, act_fn, clamp_mask, clamps,
+                                        token_position_to_id, n_tokens, d_gate_up, intermediate, stream);
 }
 
 extern "C" int moe_dequantize_checkpoint(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t I, void* out, int dtype,
@@ -522,10 +580,11 @@ extern "C" int moe_dequantize_checkpoint(const uint8_t* codes, const uint8_t* sc
   });
 }
 
-extern "C" int moe_pack_gate_up_checkpoint(const void* gate_up_activations_T, int64_t N, int64_t I, int64_t B,
-                                           const int32_t* token_position_to_id, int64_t n_tokens, uint8_t* codes, uint8_t* scales,
-                                           void* stream) {
+extern "C" int moe_pack_gate_up_checkpoint_clamped(const void* gate_up_activations_T, int64_t N, int64_t I, int64_t B, int clamp_mask,
+                                                   const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens,
+                                                   uint8_t* codes, uint8_t* scales, uint8_t* clamped, void* stream) {
   if (!gate_up_activations_T || !codes || !scales || N < 0 || I < 1 || B < 1 || n_tokens < 0) return MOE_E_BAD_ARG;
+  if ((clamp_mask & ~15) || (clamp_mask && !clamps)) return MOE_E_BAD_ARG;
   if (I > 1 << 17 || N * B >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
   int ltb = 0;
   while (ltb < 6 && (1 << ltb) < B) ++ltb;
@@ -534,13 +593,27 @@ extern "C" int moe_pack_gate_up_checkpoint(const void* gate_up_activations_T, in
   const int64_t blocks = (((int64_t)1 << 24) - 1) / per_block;  // (of a launch: fewer than 2^32 threads)
   if (blocks < 1) return MOE_E_BAD_SHAPE;
   const int64_t G = (I + 31) / 32;
+  constexpr int HI[2] = {MOE_CLAMP_GATE_HI, MOE_CLAMP_UP_HI}, LO[2] = {MOE_CLAMP_GATE_LO, MOE_CLAMP_UP_LO};
+  PackClamps at;
+  for (int z = 0; z < 2; ++z) {
+    at.hi[z] = clamp_mask & HI[z] ? as_bf16(clamps[2 * z]) : __builtin_nanf("");
+    at.lo[z] = clamp_mask & LO[z] ? as_bf16(clamps[2 * z + 1]) : __builtin_nanf("");
+  }
   for (int64_t n0 = 0; n0 < N; n0 += blocks) {
     const int64_t n = N - n0 < blocks ? N - n0 : blocks;
+    at.out = clamped ? clamped + n0 * B * 2 * ((I + 7) / 8) : nullptr;
     hipLaunchKernelGGL(pack_checkpoint_kernel, dim3((unsigned)(n * per_block)), dim3(256), 0, (hipStream_t)stream,
                        (const uint16_t*)gate_up_activations_T + n0 * 2 * I * B,
-                       token_position_to_id ? token_position_to_id + n0 * B : nullptr, n_tokens, I, B, ltb,
+                       token_position_to_id ? token_position_to_id + n0 * B : nullptr, n_tokens, I, B, ltb, at,
                        codes + n0 * B * 2 * I, scales + n0 * B * 2 * G);
     MOE_CHECK_LAUNCH();
   }
   return MOE_OK;
+}
+
+extern "C" int moe_pack_gate_up_checkpoint(const void* gate_up_activations_T, int64_t N, int64_t I, int64_t B,
+                                           const int32_t* token_position_to_id, int64_t n_tokens, uint8_t* codes, uint8_t* scales,
+                                           void* stream) {
+  return moe_pack_gate_up_checkpoint_clamped(gate_up_activations_T, N, I, B, 0, nullptr, token_position_to_id, n_tokens, codes, scales,
+                                             nullptr, stream);
 }

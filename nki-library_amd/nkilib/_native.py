@@ -57,6 +57,9 @@ EXPORTED_SYMBOLS = (
     "moe_glu_checkpoint",
     "moe_pack_gate_up_checkpoint",
     "moe_glu_checkpoint_bwd",
+    "moe_glu_checkpoint_clamped",
+    "moe_pack_gate_up_checkpoint_clamped",
+    "moe_glu_checkpoint_bwd_clamped",
     "moe_dequantize_checkpoint",
     "moe_router_topk_bwd_workspace_bytes",
     "moe_router_topk_bwd",
@@ -205,6 +208,12 @@ def lib():
                                         c_void_p],
         "moe_glu_checkpoint_bwd": [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p,
                                    c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
+        "moe_glu_checkpoint_clamped": [c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p,
+                                       c_void_p, c_void_p, c_void_p, c_void_p],
+        "moe_pack_gate_up_checkpoint_clamped": [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p,
+                                                c_void_p, c_void_p, c_void_p],
+        "moe_glu_checkpoint_bwd_clamped": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_void_p,
+                                           c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
         "moe_dequantize_checkpoint": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p],
         "moe_router_topk_bwd": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int,
                                 c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p],

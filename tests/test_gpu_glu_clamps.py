@@ -157,3 +157,110 @@ def test_a_clamped_layer_and_its_gradient():
             assert got[rows, half][both].all()
             seen += out.sum()
     assert seen > 1000
+
+
+def _bits(clamped, I):
+    return np.unpackbits(clamped.cpu().numpy(), axis=-1, bitorder="little")[..., :I].astype(bool)
+
+
+def _near_limits(rng, R, I, clamps):
+    """Rows [R, 2, I] with values around, at and far beyond their limits."""
+    x = rng.standard_normal((R, 2, I)) * np.exp2(rng.integers(-2, 5, (R, 2, 1)))
+    for half in (0, 1):
+        for limit in clamps[2 * half : 2 * half + 2]:
+            if limit is not None:
+                at = rng.random((R, I))
+                x[:, half][at < 0.2] = limit * (1 + rng.uniform(-0.1, 0.1, np.count_nonzero(at < 0.2)))
+                x[:, half][(at > 0.2) & (at < 0.25)] = limit
+                x[:, half][(at > 0.25) & (at < 0.27)] = limit * 100
+    return x
+
+
+@pytest.mark.parametrize("clamps", LIMITS)
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("I", [1, 37, 200])
+def test_kept_bits_tell_clamped_values_from_all_others(clamps, dtype, I):
+    import torch
+    from nkilib.core.moe.glu_checkpoint import glu_checkpoint, glu_checkpoint_bwd
+
+    rng = np.random.default_rng(I)
+    R, T = 50, 20
+    t = tensor(_near_limits(rng, R, I, clamps), dtype)
+    v = values(t)
+    h, codes, scales, clamped = glu_checkpoint(t, **_kwargs(clamps), return_clamped=True)
+    assert all(torch.equal(a, b) for a, b in zip((h, codes, scales), glu_checkpoint(t, **_kwargs(clamps))))
+    out = np.stack([_sides(v[:, half], *clamps[2 * half : 2 * half + 2])[0] for half in (0, 1)], 1)
+    assert clamped.shape == (R, 2, -(-I // 8)) and np.array_equal(_bits(clamped, I), out)
+    assert not (np.unpackbits(clamped.cpu().numpy(), axis=-1, bitorder="little")[..., I:]).any()
+    d = torch.ones((R, I), device="cuda")
+    d_gu, h2 = glu_checkpoint_bwd(codes, scales, d, **_kwargs(clamps), clamped=clamped)
+    plain, h3 = glu_checkpoint_bwd(codes, scales, d, **_kwargs(clamps))
+    got, was = values(d_gu), values(plain)
+    assert torch.equal(h2, h3) and not got[out].any() and np.array_equal(got[was != 0], was[was != 0])
+    rec = ot.record_values(codes.cpu().numpy(), scales.cpu().numpy())
+    g, u = ot.clamp_glu(rec[:, 0], rec[:, 1], [None if l is None else float(np.float32(l)) for l in clamps])
+    act, slope = ot.act(g, "silu")
+    for half, factor in ((0, u * slope), (1, act)):
+        assert got[:, half][~out[:, half] & (np.abs(factor) > 2.0**-100)].all()
+    # padding rows: no bit, none looked at
+    ids = rng.integers(-1, T + 2, R).astype(np.int32)
+    on = (ids >= 0) & (ids < T)
+    table = dict(token_position_to_id=tensor(ids, "int32"), n_tokens=T)
+    got = glu_checkpoint(t, **_kwargs(clamps), **table, return_clamped=True)[3]
+    assert np.array_equal(got.cpu().numpy(), clamped.cpu().numpy() * on[:, None, None])
+
+
+@pytest.mark.parametrize("clamps", LIMITS)
+@pytest.mark.parametrize("N,I,B", [(2, 96, 40), (3, 37, 1), (1, 130, 64), (2, 9, 200), (1, 1000, 3)])
+def test_bits_of_a_layers_checkpoint(clamps, N, I, B):
+    """Set where the checkpoint holds the limit's bf16 or more: for every clamped value, and for none further than a step of bf16 inside."""
+    import torch
+    from nkilib.core.moe.glu_checkpoint import glu_checkpoint_bwd, pack_gate_up_checkpoint
+
+    rng = np.random.default_rng(N + I + B)
+    x = _near_limits(rng, N * B, I, clamps).astype(np.float32)
+    f32 = [None if l is None else float(np.float32(l)) for l in clamps]
+    g, u = ot.clamp_glu(x[:, 0], x[:, 1], [None if l is None else np.float32(l) for l in clamps])
+    kept = tensor(np.stack((g, u), 1).reshape(N, B, 2, I).transpose(0, 2, 3, 1), "bfloat16")
+    codes, scales, clamped = pack_gate_up_checkpoint(kept, **_kwargs(clamps), return_clamped=True)
+    assert all(torch.equal(a, b) for a, b in zip((codes, scales), pack_gate_up_checkpoint(kept)))
+    got = _bits(clamped, I)
+    rows = values(kept).transpose(0, 3, 1, 2).reshape(N * B, 2, I)
+    for half in (0, 1):
+        hi, lo = f32[2 * half : 2 * half + 2]
+        want = (rows[:, half] >= (np.inf if hi is None else ot.bf16_value(hi))) | (rows[:, half] <= (-np.inf if lo is None else ot.bf16_value(lo)))
+        assert np.array_equal(got[:, half], want)
+        assert got[:, half][_sides(x[:, half].astype(np.float64), hi, lo)[0]].all()
+    d_gu, _ = glu_checkpoint_bwd(codes, scales, torch.ones((N * B, I), device="cuda"), **_kwargs(clamps), clamped=clamped)
+    assert not values(d_gu)[got].any()
+    ids = rng.integers(-1, 3, N * B).astype(np.int32)
+    on = (ids >= 0) & (ids < 2)
+    got = pack_gate_up_checkpoint(kept, tensor(ids, "int32"), 2, **_kwargs(clamps), return_clamped=True)[2]
+    assert np.array_equal(got.cpu().numpy(), clamped.cpu().numpy() * on[:, None, None])
+
+
+def test_bits_of_infinities_and_nan_and_without_limits():
+    import torch
+    from nkilib.core.moe.glu_checkpoint import glu_checkpoint, pack_gate_up_checkpoint
+
+    x = torch.tensor([[[float("inf"), float("-inf"), float("nan"), 2.0, 1.0]] * 2], device="cuda").bfloat16()
+    for kw, want in (({}, [[0] * 5] * 2), (dict(gate_clamp_upper_limit=2.0), [[1, 0, 0, 1, 0], [0] * 5]),
+                     (dict(up_clamp_lower_limit=-3.0, up_clamp_upper_limit=1.0), [[0] * 5, [1, 1, 0, 1, 1]])):
+        assert _bits(glu_checkpoint(x, **kw, return_clamped=True)[3], 5)[0].tolist() == want
+        assert _bits(pack_gate_up_checkpoint(x.view(1, 2, 5, 1), **kw, return_clamped=True)[2], 5)[0].tolist() == want
+
+
+def test_refusals():
+    import torch
+    from nkilib.core.moe.glu_checkpoint import glu_checkpoint, glu_checkpoint_bwd, pack_gate_up_checkpoint
+
+    x = torch.zeros((4, 2, 36), device="cuda")
+    _, c, s, m = glu_checkpoint(x, return_clamped=True)
+    d = torch.zeros((4, 36), device="cuda")
+    for bad in (m[:3], m[:, :, :4], m.int(), m[:, 0], m.bool()):
+        with pytest.raises(AssertionError, match="NCC_INKI016"):
+            glu_checkpoint_bwd(c, s, d, clamped=bad)
+    with pytest.raises(AssertionError, match="NCC_INKI016"):
+        pack_gate_up_checkpoint(torch.zeros((1, 2, 8, 4), device="cuda").bfloat16(), gate_clamp_upper_limit=7.0)
+    h, c, s, m = glu_checkpoint(x[:0], return_clamped=True)
+    assert m.shape == (0, 2, 5) and glu_checkpoint_bwd(c, s, d[:0], clamped=m)[0].shape == (0, 2, 36)

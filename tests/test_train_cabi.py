@@ -93,6 +93,17 @@ def test_glu_refusals(L):
     assert L.moe_dequantize_checkpoint(P, P, 0, 64, P, 0, None) == 0
 
 
+def test_glu_with_kept_bits_refusals(L):
+    f = (ctypes.c_float * 4)()
+    fwd = lambda R=4, mask=0, clamps=None: L.moe_glu_checkpoint_clamped(P, 0, R, 64, 0, mask, clamps, None, 0, P, P, P, P, None)
+    bwd = lambda R=4, mask=0, clamps=None: L.moe_glu_checkpoint_bwd_clamped(P, P, P, P, 0, R, 64, 0, mask, clamps, None, 0, P, None, None)
+    pack = lambda R=4, mask=0, clamps=None: L.moe_pack_gate_up_checkpoint_clamped(P, R, 64, 4, mask, clamps, None, 0, P, P, P, None)
+    for call in (fwd, bwd, pack):
+        assert call(R=0) == 0 and call(R=0, mask=15, clamps=f) == 0
+        assert call(mask=16, clamps=f) == BAD_ARG and call(mask=1) == BAD_ARG and call(R=-1) == BAD_ARG
+    assert L.moe_glu_checkpoint_bwd_clamped(None, P, P, P, 0, 4, 64, 0, 0, None, None, 0, P, None, None) == BAD_ARG
+
+
 def test_host_tensors_are_refused():
     """There is no CPU path: the operators say so."""
     import torch
