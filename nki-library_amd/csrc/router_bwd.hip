@@ -62,7 +62,7 @@ __device__ __forceinline__ uint32_t hi_lo(float a, float b, uint32_t& lo) {
   return h;
 }
 
-// sum / max over the eight lanes that share a token
+// sum / max over the eight lanes that share a token, all of which have to be there: a lane that a branch leaves out hands over anything
 __device__ __forceinline__ float sum8(float v) {
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) v += __shfl_xor(v, o, 64);
@@ -143,7 +143,8 @@ __global__ __launch_bounds__(256) void router_dlogits_kernel(const RouterBwdArgs
     if (a.dense) {
       dl = g;  // below
     } else if (a.softmax) {
-      const float p = on ? expf(l - max8(on ? l : -__builtin_inff())) : 0.f;
+      const float mx = max8(l);  // (all eight lanes take part; l of one that is off is -inf)
+      const float p = on ? expf(l - mx) : 0.f;
       const float q = p / sum8(p);
       const float mean = sum8(on ? g * q : 0.f);
       dl = q * (g - mean);

@@ -1,0 +1,73 @@
+"""The router's gradient where logits, gradients and repeats are at their worst (tolerances: test_gpu_router_topk_bwd)."""
+
+import numpy as np
+import pytest
+
+from test_gpu_router_topk_bwd import MODES, _case, _check, _dl_limits
+from train_helpers import tensor, values
+
+pytestmark = pytest.mark.gpu
+
+
+def _call(g, x, w, l, ids, mode, bias=None):
+    from nkilib.core.router_topk import router_topk_bwd
+    from nkilib.core.utils.common_types import RouterActFnType
+
+    return router_topk_bwd(tensor(g), x, w, bias, tensor(l), tensor(ids, "int32"), RouterActFnType.SOFTMAX if mode[0] else RouterActFnType.SIGMOID,
+                           router_pre_norm=mode[1], norm_topk_prob=mode[2], mask_to_topk=mode[3])
+
+
+@pytest.mark.parametrize("mode", [m for m in MODES if m[0]])
+@pytest.mark.parametrize("shift", [-90.0, -150.0, -1e4, 90.0, 1e4])
+@pytest.mark.parametrize("k", [1, 3, 5, 8])
+def test_softmax_of_shifted_logits(mode, shift, k):
+    """A softmax does not change when every logit is shifted; its gradient neither."""
+    import torch
+
+    T, H, E = 37, 128, 12
+    rng, l, ids, g, x, w = _case(T, H, E, k, int(abs(shift)) + k)
+    l = (l + np.float32(shift)).astype(np.float32)
+    ids = np.argsort(-l, 1, kind="stable")[:, :k].astype(np.int32)
+    want, err = _dl_limits(g[:T].astype(np.float64), l, ids, mode)
+    got = _call(g, x, w, l, ids, mode, torch.zeros(E, device="cuda"))
+    _check(got, want, err, values(x), values(w), f"{mode} {shift} {k}", "float32")
+
+
+@pytest.mark.parametrize("mode", [m for m in MODES if m[0] and (m[2] or not m[1])])
+@pytest.mark.parametrize("shift", [-90.0, -150.0])
+def test_repeats_and_wrong_indices_beside_small_logits(mode, shift):
+    """Lanes of repeated and wrong indices have no part in a token's maximum."""
+    T, H, E = 3, 128, 10
+    rng, l, _, g, x, w = _case(T, H, E, 3, 2)
+    l = (l + np.float32(shift)).astype(np.float32)
+    ids = np.array([[4, 2, 4], [-1, 10, 7], [9, 9, 9]], np.int32)
+    want, err = np.zeros((T, E)), np.zeros((T, E))
+    for t, mine in enumerate(([4, 2], [7], [9])):
+        want[t : t + 1], err[t : t + 1] = _dl_limits(g[t : t + 1].astype(np.float64), l[t : t + 1], np.array([mine]), mode)
+    _check(_call(g, x, w, l, ids, mode), want, err, values(x), values(w), str(mode), None)
+
+
+@pytest.mark.parametrize("E,k", [(64, 8), (256, 8), (300, 5)])
+def test_what_cancels_over_all_experts_does(E, k):
+    """The softmax over all experts, whose dx is a product on the matrix cores: a part of w that all experts share leaves nothing."""
+    import torch
+
+    T, H = 40, 128
+    mode = (True, True, False, False)
+    rng, l, ids, g, x, w = _case(T, H, E, k, 1)
+    small = (rng.integers(-8, 9, (H, E)) / 8).astype(np.float32)
+    w = tensor(16.0 + small, "bfloat16")
+    for m in (mode, (True, True, False, True)):
+        want, err = _dl_limits(g[:T].astype(np.float64), l, ids, m)
+        assert np.abs(want.sum(1)).max() < 1e-12
+        _check(_call(g, x, w, l, ids, m), want, err, values(x), values(w), "cancels", None)
+
+
+def test_the_same_call_gives_the_same_bits():
+    import torch
+
+    for T, H, E, k, mode in ((1999, 512, 60, 4, MODES[3]), (8192, 2176, 256, 8, MODES[3]), (3000, 256, 300, 3, MODES[1])):
+        rng, l, ids, g, x, w = _case(T, H, E, k, 5)
+        first = _call(g, x, w, l, ids, mode, torch.zeros(E, device="cuda"))
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(first, _call(g, x, w, l, ids, mode, torch.zeros(E, device="cuda"))))
