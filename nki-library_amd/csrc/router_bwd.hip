@@ -56,9 +56,12 @@ struct RouterBwdArgs {
   int64_t n_dw, x_splits;    // jobs of dw; parts of the tokens for dx
 };
 
+// (An infinite value is its own hi part, with nothing behind it: inf - inf would make a NaN of what a sum in fp32 leaves infinite.  A
+// finite dl is at most half of the largest fp32, whose bf16 is finite too.)
 __device__ __forceinline__ uint32_t hi_lo(float a, float b, uint32_t& lo) {
   const uint32_t h = pack2_bf16(a, b);
-  lo = pack2_bf16(a - bf16_lo(h), b - bf16_hi(h));
+  const float ra = fabsf(a) < __builtin_inff() ? a - bf16_lo(h) : 0.f, rb = fabsf(b) < __builtin_inff() ? b - bf16_hi(h) : 0.f;
+  lo = pack2_bf16(ra, rb);
   return h;
 }
 
@@ -290,10 +293,12 @@ __device__ __forceinline__ void grad_w(const RouterBwdArgs& a, int64_t job, uint
     buf[tid] = in[0];
     buf[256 + tid] = in[1];
   };
-  auto fetch_dl = [&](int64_t s, int part, u32x4(&d)[NT]) {
-    const u32x4* src = a.dlw + (((s < s1 ? s : s1 - 1) * 2 * KS + n0) * 2 + part) * 64 + lane;
+  auto fetch_dl = [&](int64_t s, int part, u32x4(&d)[NT]) {  // (as a buffer too: zeros behind the last step)
+    const __amdgpu_buffer_rsrc_t step =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(a.dlw + s * (2 * KS * 128)), 0, s < s1 ? 2 * KS * 2048 : 0, 0x00020000);
+    const int at = ((n0 * 2 + part) * 64 + lane) * 16;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) d[n] = src[n * 128];
+    for (int n = 0; n < NT; ++n) d[n] = __builtin_amdgcn_raw_buffer_load_b128(step, at + n * 2048, 0, 0);
   };
   auto multiply = [&](const u32x4* buf, const u32x4(&d)[NT]) {
     u32x4 x[8];
@@ -309,7 +314,7 @@ __device__ __forceinline__ void grad_w(const RouterBwdArgs& a, int64_t job, uint
       for (int n = 0; n < NT; ++n) acc[j][n] = mfma(f, d[n], acc[j][n]);
     }
   };
-  // both groups take as many turns: in one without a step the rows are zeros (and dl some step's, which they leave at zero)
+  // both groups take as many turns: in one without a step the rows and dl are zeros (another step's dl would do, were it finite)
   const int64_t turns = (s1 - s0 + 1) / 2;
   fetch_x(s0 + kg);
   store_x(s_x[kg][0]);

@@ -47,6 +47,40 @@ def test_repeats_and_wrong_indices_beside_small_logits(mode, shift):
     _check(_call(g, x, w, l, ids, mode), want, err, values(x), values(w), str(mode), None)
 
 
+@pytest.mark.parametrize("T,E,k", [(5, 12, 3), (33, 60, 8), (70, 300, 2), (600, 64, 4)])
+@pytest.mark.parametrize("mode", [(False, True, False, True), (False, False, False, True), (False, True, False, False)])
+def test_infinite_gradients_stay_infinite(T, E, k, mode):
+    """An affinity's gradient that is infinite: dx of its token and dw of its expert are infinite with the sign of their factors, as a
+    sum in fp32 has them, and the rest is as without it, another one of the largest magnitude included."""
+    import torch
+
+    H = 128
+    rng, l, ids, g, x, w = _case(T, H, E, k, T + E)
+    e, t, e2, t2 = int(ids[1, 0]), 1, int(ids[T - 1, k - 1]), T - 1
+    if e2 == e:
+        e2 = int(ids[T - 1, 0])
+    assert e2 != e
+    l[t2, e2] = 0.0  # (the slope's largest value, 1/4)
+    g[t, e], g[t2, e2] = np.inf, -3.4e38
+    xv, wv = values(x), values(w)
+    assert (xv[t] != 0).all() and (wv[:, e] != 0).all()
+    clean = g.copy()
+    clean[t, e] = 0
+    want, err = _dl_limits(clean[:T].astype(np.float64), l, ids, mode)
+    d_x, d_w, d_b = _call(g, x, w, l, ids, mode, torch.zeros(E, device="cuda"))
+    got_x, got_w, got_b = values(d_x), values(d_w), values(d_b)
+    assert np.array_equal(got_x[t], np.sign(wv[:, e]) * np.inf) and np.array_equal(got_w[:, e], np.sign(xv[t]) * np.inf)
+    assert np.isposinf(got_b[e])
+    rows, cols = np.arange(T) != t, np.arange(E) != e
+    fits = lambda a: np.where(np.abs(a) < 3.3e38, a, np.nan)
+    wx, ww = want @ wv.T, xv.T @ want
+    mx = 2.0**-8 * np.abs(wx) * (1 + 2.0**-7) + (E + 2) * 2.0**-24 * (np.abs(want) @ np.abs(wv.T)) + err @ np.abs(wv.T) + 2.0**-134
+    mw = 2.0**-8 * np.abs(ww) * (1 + 2.0**-7) + (T + 2) * 2.0**-24 * (np.abs(xv.T) @ np.abs(want)) + np.abs(xv.T) @ err + 2.0**-134
+    okx, okw = np.isfinite(fits(wx))[rows], np.isfinite(fits(ww))[:, cols]
+    assert (np.abs(got_x - wx)[rows] <= mx[rows])[okx].all()
+    assert (np.abs(got_w - ww)[:, cols] <= mw[:, cols])[okw].all()
+
+
 @pytest.mark.parametrize("E,k", [(64, 8), (256, 8), (300, 5)])
 def test_what_cancels_over_all_experts_does(E, k):
     """The softmax over all experts, whose dx is a product on the matrix cores: a part of w that all experts share leaves nothing."""
