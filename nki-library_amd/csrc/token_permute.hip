@@ -479,7 +479,7 @@ extern "C" int moe_combine_tokens(const void* y, int dtype, const void* expert_a
   if (block_to_expert && (B <= 0 || N < 0 || B >= (int64_t)1 << 31 || N >= (int64_t)1 << 31 || S != B * N)) return MOE_E_BAD_SHAPE;
   const SlotTables a{token_slots, block_to_expert, expert_affinities, aff_dtype, top_k, (uint32_t)B, (uint32_t)N, E, S};
   const hipStream_t s = (hipStream_t)stream;
-  const bool scan = build_token_slots && combine_scans(S, T);
+  const bool scan = build_token_slots && token_position_to_id && combine_scans(S, T);  // (no table, no slots: the list of none)
   const int rc = begin_by_list(a, T, T1, token_position_to_id, build_token_slots, !scan, s);
   if (rc != MOE_OK) return rc;
   if (T == 0 || H == 0) return MOE_OK;
