@@ -22,8 +22,31 @@ namespace moe {
 
 constexpr int SLOTS_MAX_K = 64;        // most slots a list holds per token
 constexpr int SLOTS_LDS_WORDS = 12288;  // 48 KB of lists per workgroup
+// Entries that the workgroups of token_slots_kernel read in all, at most: as many as slots times workgroups, which grow with the tokens
+// from 256 * SLOTS_LDS_WORDS / (1 + k) on.  The whole table in every workgroup | global counters, us: 8192 tokens in 8 of 98 k slots
+// 8.0 | 10.9 (2^24.6 entries), 262 k in 8 of 2.1 M 85 | 68 (2^29), 131 k in 16 of 2.2 M 92 | 122 (2^29.1), 400 k in 8 of 3.3 M
+// 244 | 151 (2^29.9), 131 k in 32 of 4.3 M 323 | 365, 262 k in 16 of 4.3 M 313 | 254 (2^30.5 both), 80 k in 64 of 5.2 M 393 | 377 (2^31).
+constexpr int64_t LISTS_WHOLE_TABLE = (int64_t)1 << 30;
 
 // lists [T][1 + k]: how many slots the token has (more than k: the list is cut), its slots ascending, -1 behind them.
+// The lists of nt tokens from t0 on, whose slots were taken in any order into s_list: each goes to the place that its rank names.
+__device__ __forceinline__ void write_ranked(const int* s_list, int nt, int64_t t0, int k, int32_t* __restrict__ lists) {
+  const int w = 1 + k;
+  for (int i = threadIdx.x; i < nt * w; i += 1024) {
+    const int t = i / w, j = i - t * w, n = s_list[t * w], held = n < k ? n : k;
+    int32_t* out = lists + (t0 + t) * w;
+    if (j == 0) {
+      out[0] = n;
+    } else if (j > held) {
+      out[j] = -1;
+    } else {
+      const int mine = s_list[t * w + j];
+      int rank = 1;
+      for (int o = 1; o <= held; ++o) rank += s_list[t * w + o] < mine;
+      out[rank] = mine;
+    }
+  }
+}
 // A workgroup owns `range` tokens and reads the whole table, which the L2 hands out: a table of 98 k slots is 0.4 MB, and
 // one launch without global atomics or cleared counters is shorter than the two that those would take.
 __global__ __launch_bounds__(1024) void token_slots_kernel(const int32_t* __restrict__ tp2id, int64_t S, int64_t T, int k,
@@ -63,20 +86,37 @@ __global__ __launch_bounds__(1024) void token_slots_kernel(const int32_t* __rest
   }
   for (int64_t s = 4 * n4 + threadIdx.x; s < S; s += 1024) take(s, tp2id[s]);
   __syncthreads();
-  // the slots were taken in any order: each goes to the place that its rank names
-  for (int i = threadIdx.x; i < nt * w; i += 1024) {
-    const int t = i / w, j = i - t * w, n = s_list[t * w], held = n < k ? n : k;
-    int32_t* out = lists + (t0 + t) * w;
-    if (j == 0) {
-      out[0] = n;
-    } else if (j > held) {
-      out[j] = -1;
-    } else {
-      const int mine = s_list[t * w + j];
-      int rank = 1;
-      for (int o = 1; o <= held; ++o) rank += s_list[t * w + o] < mine;
-      out[rank] = mine;
-    }
+  write_ranked(s_list, nt, t0, k, lists);
+}
+
+// Long tables (every workgroup's reading of the whole would grow with their square): counts cleared, each slot put behind its token's
+// others by a global counter, the lists ranked by way of LDS.  Which slots of a token with more than k are kept is left open.
+__global__ __launch_bounds__(256) void clear_counts_kernel(int64_t T, int w, int32_t* __restrict__ lists) {
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < T; t += (int64_t)gridDim.x * 256) lists[t * w] = 0;
+}
+__global__ __launch_bounds__(256) void place_slots_kernel(const int32_t* __restrict__ tp2id, int64_t S, int64_t T, int k,
+                                                          int32_t* __restrict__ lists) {
+  constexpr int U = 4;
+  const int64_t threads = (int64_t)gridDim.x * 256;
+  for (int64_t s0 = (int64_t)blockIdx.x * 256 + threadIdx.x; s0 < S; s0 += threads * U) {
+    int id[U], p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = s0 + u * threads < S ? tp2id[s0 + u * threads] : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) p[u] = id[u] >= 0 && id[u] < T ? atomicAdd(&lists[(int64_t)id[u] * (1 + k)], 1) : k;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p[u] < k) lists[(int64_t)id[u] * (1 + k) + 1 + p[u]] = (int)(s0 + u * threads);
+  }
+}
+__global__ __launch_bounds__(1024) void rank_slots_kernel(int64_t T, int k, int range, int32_t* __restrict__ lists) {
+  __shared__ int s_list[SLOTS_LDS_WORDS];
+  for (int64_t t0 = (int64_t)blockIdx.x * range; t0 < T; t0 += (int64_t)gridDim.x * range) {
+    const int nt = (int)(T - t0 < range ? T - t0 : range);
+    __syncthreads();  // (the lists of the round before have been read)
+    for (int i = threadIdx.x; i < nt * (1 + k); i += 1024) s_list[i] = lists[t0 * (1 + k) + i];
+    __syncthreads();
+    write_ranked(s_list, nt, t0, k, lists);
   }
 }
 
@@ -404,8 +444,17 @@ static int launch_token_slots(const int32_t* tp2id, int64_t S, int64_t T, int k,
   if (T == 0) return MOE_OK;
   int64_t range = (T + 255) / 256;  // a workgroup per CU
   if (range > SLOTS_LDS_WORDS / (1 + k)) range = SLOTS_LDS_WORDS / (1 + k);
-  hipLaunchKernelGGL(token_slots_kernel, dim3((unsigned)((T + range - 1) / range)), dim3(1024), 0, s, tp2id, S, T, k, (int)range,
-                     lists);
+  const int64_t groups = (T + range - 1) / range;
+  if (groups * S <= LISTS_WHOLE_TABLE) {
+    hipLaunchKernelGGL(token_slots_kernel, dim3((unsigned)groups), dim3(1024), 0, s, tp2id, S, T, k, (int)range, lists);
+    MOE_CHECK_LAUNCH();
+    return MOE_OK;
+  }
+  hipLaunchKernelGGL(clear_counts_kernel, dim3(grid_of((T + 255) / 256)), dim3(256), 0, s, T, 1 + k, lists);
+  MOE_CHECK_LAUNCH();
+  hipLaunchKernelGGL(place_slots_kernel, dim3(grid_of((S + 1023) / 1024)), dim3(256), 0, s, tp2id, S, T, k, lists);
+  MOE_CHECK_LAUNCH();
+  hipLaunchKernelGGL(rank_slots_kernel, dim3(grid_of(groups)), dim3(1024), 0, s, T, k, (int)range, lists);
   MOE_CHECK_LAUNCH();
   return MOE_OK;
 }

@@ -1,8 +1,128 @@
-"""Tables without slots (operators and tolerances: test_gpu_token_permute)."""
+"""Lists of long tables, tables without slots (operators and tolerances: test_gpu_token_permute).
+
+Long tables are looked at on the device: their oracle is torch's, in whole numbers for the lists and in 64 bits for the sums.
+"""
 
 import pytest
 
 pytestmark = pytest.mark.gpu
+
+
+def _lists(tp, T, k):
+    """[T, 1 + k] of a table on the device: counts, the first k slots in ascending order, -1."""
+    import torch
+
+    ids = torch.where((tp >= 0) & (tp < T), tp.long(), T)
+    order = torch.argsort(ids, stable=True)
+    counts = torch.bincount(ids, minlength=T + 1)[:T]
+    first = torch.cumsum(counts, 0) - counts
+    j = torch.arange(k, device=tp.device)
+    at = (first[:, None] + j).clamp(max=max(tp.numel() - 1, 0))
+    out = torch.where(j < counts[:, None], order[at], -1)
+    return torch.cat((counts[:, None], out), 1).int()
+
+
+# tokens, slots, most slots of a token: tables on either side of 2^30 entries read by the workgroups that own the tokens, tokens without
+# slots in most lists, a last workgroup with few tokens
+@pytest.mark.parametrize("T,S,k", [(1, 300_000, 64), (70_000, 600_000, 8), (12, 262_145, 3), (4001, 5_000_000, 64), (600_001, 5_000_002, 8),
+                                   (1_000_003, 4_300_001, 1), (200_000, 4_300_003, 2), (3_000_000, 1_000_000, 5), (1_048_576, 8_600_000, 7)])
+def test_lists_of_long_tables(T, S, k):
+    import torch
+    from nkilib.core.moe.token_permute import build_token_slots
+
+    g = torch.Generator(device="cuda").manual_seed(T + S)
+    # every token up to k times, at places in any order; the rest padding of any kind
+    most = min(k * T, S - S // 10)
+    tp = torch.tensor([T, -1, 2**31 - 1, -(2**31)], dtype=torch.int32, device="cuda")[torch.randint(0, 4, (S,), generator=g, device="cuda")]
+    tokens = torch.arange(k * T, device="cuda", dtype=torch.int64)[torch.randperm(k * T, generator=g, device="cuda")[:most]] % T
+    tp[torch.randperm(S, generator=g, device="cuda")[:most]] = tokens.int()
+    want = _lists(tp, T, k)
+    assert int(want[:, 0].max()) <= k
+    assert torch.equal(build_token_slots(tp, T, k), want)
+    odd = torch.cat((tp[:3], tp))  # a table that begins at a 4-byte address
+    assert torch.equal(build_token_slots(odd[3:], T, k), want)
+    if k > 1:  # lists that are cut: the true count, slots that are the token's, each once
+        cut = build_token_slots(tp, T, k - 1)
+        assert torch.equal(cut[:, 0], want[:, 0])
+        whole = want[:, 0] < k
+        assert torch.equal(cut[whole], want[whole][:, :k])
+        long = cut[~whole][:, 1:]
+        if long.numel():
+            assert bool((tp[long.long()] == torch.nonzero(~whole).int()).all()) and bool((long[:, 1:] > long[:, :-1]).all())
+
+
+def test_sums_over_a_long_table():
+    """permute and combine, both ways, with lists that the calls make themselves."""
+    import torch
+    from nkilib.core.moe.token_permute import combine_tokens, combine_tokens_bwd, permute_tokens, permute_tokens_bwd
+
+    T, H, E, k, B = 1_050_000, 20, 16, 4, 16
+    g = torch.Generator(device="cuda").manual_seed(0)
+    ids = torch.rand((T, E), generator=g, device="cuda").topk(k, dim=1).indices
+    order = torch.argsort(ids.reshape(-1), stable=True)
+    counts = torch.bincount(ids.reshape(-1), minlength=E)
+    blocks = (counts + B - 1) // B
+    first, rank = (torch.cumsum(blocks, 0) - blocks) * B, torch.arange(T * k, device="cuda") - (torch.cumsum(counts, 0) - counts)[ids.reshape(-1)[order]]
+    N = int(blocks.sum())
+    tp = torch.full((N * B,), T, dtype=torch.int32, device="cuda")
+    at = first[ids.reshape(-1)[order]] + rank
+    tp[at] = (order // k).int()
+    be = torch.repeat_interleave(torch.arange(E, dtype=torch.int32, device="cuda"), blocks)
+    S = N * B
+    x, d = (torch.randn((T, H), generator=g, device="cuda") for _ in range(2))
+    aff = torch.rand((T, E), generator=g, device="cuda")
+    on = tp < T
+    xs = permute_tokens(x, tp)
+    assert torch.equal(xs[on], x[tp[on].long()]) and not xs[~on].any()
+    e = be.long().repeat_interleave(B)[on]
+    t = tp[on].long()
+    w = aff.double()[t, e]
+    want = torch.zeros((T, H), dtype=torch.float64, device="cuda").index_add_(0, t, xs[on].double())
+    mag = torch.zeros_like(want).index_add_(0, t, xs[on].double().abs())
+    near = lambda got, want, mag, steps: bool(((got.double() - want).abs() <= 2.0**-24 * (want.abs() + steps * mag)).all())
+    assert near(permute_tokens_bwd(xs, tp, T, k), want, mag, k + 1)
+    want = torch.zeros_like(want).index_add_(0, t, xs[on].double() * w[:, None])
+    assert near(combine_tokens(xs, aff, tp, be, B, T, k), want, torch.zeros_like(want).index_add_(0, t, (xs[on].double() * w[:, None]).abs()), k + 2)
+    d_y, d_aff = combine_tokens_bwd(d, xs, aff, tp, be, B, k)
+    assert near(d_y[on], d.double()[t] * w[:, None], torch.zeros((), device="cuda"), 0) and not d_y[~on].any()
+    terms = d.double()[t] * xs[on].double()
+    want = torch.zeros((T, E), dtype=torch.float64, device="cuda").index_put_((t, e), terms.sum(1))
+    mag = torch.zeros_like(want).index_put_((t, e), terms.abs().sum(1))
+    assert near(d_aff, want, mag, H / 64 + 16)
+
+
+def test_a_long_tables_lists_in_a_graph_and_on_two_streams():
+    import torch
+    from nkilib.core.moe.token_permute import build_token_slots
+
+    T, S, k = 400_000, 4_500_000, 40  # (no token lies in 40 slots)
+    tables = [torch.randint(-1, T + 2, (S,), generator=torch.Generator(device="cuda").manual_seed(i), device="cuda").int() for i in range(4)]
+    want = [_lists(t, T, k) for t in tables]
+    assert max(int(w[:, 0].max()) for w in want) <= k
+    buf = tables[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        build_token_slots(buf, T, k)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = build_token_slots(buf, T, k)
+    for i in (1, 2, 3, 1):
+        buf.copy_(tables[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i]), i
+        assert torch.equal(build_token_slots(tables[0], T, k), want[0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(4):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(build_token_slots(tables[i], T, k))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_no_slots_and_no_table():
