@@ -1,9 +1,13 @@
-"""Lists of long tables, tables without slots (operators and tolerances: test_gpu_token_permute).
+"""Lists of long tables, launches that go round more than once, tables without slots (operators and tolerances: test_gpu_token_permute).
 
 Long tables are looked at on the device: their oracle is torch's, in whole numbers for the lists and in 64 bits for the sums.
 """
 
+import numpy as np
 import pytest
+
+from oracle import train as ot
+from train_helpers import tensor
 
 pytestmark = pytest.mark.gpu
 
@@ -145,3 +149,60 @@ def test_no_slots_and_no_table():
                 rc = L.moe_combine_tokens(y.data_ptr(), nv.DT_FP32, aff.data_ptr(), nv.DT_FP32, 4, 3, None, be.data_ptr(), 4, 0,
                                           slots.data_ptr(), 2, 1, 0, T, 16, out.data_ptr(), nv.stream_ptr(y.device))
                 assert rc == 0 and not out.any(), (T, fill)
+
+
+# A launch holds at most 2^20 workgroups, which take their next job 2^20 further on: rows of more than 4 KB are a workgroup's job,
+# shorter ones a wave's, four to a workgroup.
+@pytest.mark.parametrize("T,H,dtype", [((1 << 20) + 77, 2051, "bfloat16"), ((1 << 22) + 77, 9, "float16"), ((1 << 22) + 77, 3, "float32")])
+def test_more_rows_than_a_launch_has_workgroups(T, H, dtype):
+    import torch
+    from nkilib.core.moe.token_permute import build_token_slots, combine_tokens, combine_tokens_bwd, permute_tokens
+
+    dt = getattr(torch, dtype)
+    g = torch.Generator(device="cuda").manual_seed(H)
+    B, E = 64, 3
+    N = (T + 5 + B - 1) // B
+    S = N * B
+    tp = torch.full((S,), -1, dtype=torch.int32, device="cuda")
+    at = torch.randperm(S, generator=g, device="cuda")[:T]
+    tp[at] = torch.arange(T, dtype=torch.int32, device="cuda")
+    be = torch.randint(0, E, (N,), generator=g, device="cuda").int()
+    # values of few bits: every product is exact in fp32, so that the results are known to the bit
+    x = torch.randint(-8, 9, (T, H), generator=g, device="cuda", dtype=torch.int8).to(dt)
+    aff = torch.randint(1, 9, (T + 2, E), generator=g, device="cuda").float() / 8
+    xs = permute_tokens(x, tp)
+    parts = [slice(i, min(i + (1 << 18), T)) for i in range(0, T, 1 << 18)]
+    for p in parts:
+        assert torch.equal(xs[at[p]], x[p])
+    pad = torch.nonzero(tp < 0)[:, 0]
+    assert not xs[pad].any()
+    slots = build_token_slots(tp, T, 1)
+    assert torch.equal(slots[:, 1], at.int()) and bool((slots[:, 0] == 1).all())
+    w = aff[torch.arange(T, device="cuda"), be.long()[at // B]]
+    out = combine_tokens(xs, aff, tp, be, B, T, 1, token_slots=slots)
+    for p in parts:
+        assert torch.equal(out[p], (w[p, None] * x[p].float()).to(dt))
+    del out
+    d_y, d_aff = combine_tokens_bwd(x, xs, aff, tp, be, B, 1, token_slots=slots)
+    assert not d_y[pad].any()
+    total = 0.0
+    for p in parts:
+        assert torch.equal(d_y[at[p]], (w[p, None] * x[p].float()).to(dt))
+        sums = (x[p].float() ** 2).sum(1)
+        assert torch.equal(d_aff[p].gather(1, be.long()[at[p] // B][:, None])[:, 0], sums)
+        total += float(sums.double().sum())
+    assert float(d_aff.double().sum()) == total
+
+
+def test_more_blocks_of_a_checkpoint_than_a_launch_takes():
+    import torch
+    from nkilib.core.moe.glu_checkpoint import pack_gate_up_checkpoint
+
+    N = (1 << 23) + 300  # (two tiles a block, fewer than 2^24 a launch)
+    x = torch.ones((N, 2, 1, 1), dtype=torch.bfloat16, device="cuda")
+    x[-1000:] = torch.randn((1000, 2, 1, 1), generator=torch.Generator(device="cuda").manual_seed(0), device="cuda").bfloat16()
+    c, s = pack_gate_up_checkpoint(x)
+    c1, s1 = pack_gate_up_checkpoint(x[-1000:].contiguous())
+    assert torch.equal(c[-1000:], c1) and torch.equal(s[-1000:], s1)
+    assert bool((c[:-1000] == c[0]).all()) and bool((s[:-1000] == s[0]).all())
+    assert np.array_equal(c1.cpu().numpy(), ot.record(x[-1000:, :, :, 0].float().cpu().numpy())[0])
