@@ -406,7 +406,7 @@ int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtype, const vo
 /* No counterpart in the reference (its checkpoints are bf16, moe_cte.py:145-150).  A record of R rows of I gate and I up values:
  * codes uint8 [R, 2, I] (OCP e4m3) and scales uint8 [R, 2, ceil(I/32)], one E8M0 byte per 32 neighbours; a value is
  * code * 2^(byte - 127).  The scale is the smallest power of two with amax / scale <= 448 over the group's finite values;
- * infinities and NaN are kept as NaN codes.  I <= 131072.  clamp_mask: MOE_CLAMP_*; clamps: host, gate upper, gate lower, up
+ * infinities and NaN are kept as NaN codes.  I <= 131072, R < 2^31.  clamp_mask: MOE_CLAMP_*; clamps: host, gate upper, gate lower, up
  * upper, up lower (NULL when clamp_mask is 0).  token_position_to_id int32 [R] (nullable): rows of padding slots (outside
  * [0, n_tokens)) are not read, and zero in every output.
  *
@@ -419,7 +419,7 @@ int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtype, const vo
  * moe_..._clamped: the same with clamped uint8 [R, 2, ceil(I/8)] (nullable), bit i of byte v for value 8 v + i of a row, written by
  * the first two: set where a value lay at or beyond its limit ahead of the clamp (pack: where the checkpoint holds its limit, as bf16,
  * or more; clamp_mask and clamps have no other use there).  moe_glu_checkpoint_bwd_clamped passes a gradient where it is not set.
- * moe_dequantize_checkpoint: `rows` rows of I codes with ceil(I/32) scales each -> values (bf16 holds them exactly, down to 2^-133). */
+ * moe_dequantize_checkpoint: `rows` < 2^32 rows of I codes with ceil(I/32) scales each -> values (bf16 holds them exactly, down to 2^-133). */
 int moe_glu_checkpoint(const void* gate_up, int dtype, int64_t R, int64_t I, int act_fn, int clamp_mask,
                        const float* clamps, const int32_t* token_position_to_id, int64_t n_tokens, void* intermediate,
                        uint8_t* codes, uint8_t* scales, void* stream);

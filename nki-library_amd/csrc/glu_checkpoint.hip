@@ -449,11 +449,11 @@ static float as_bf16(float f) {
   return f;
 }
 static int glu_args(GluArgs& a, int64_t R, int64_t I, int act_fn, int clamp_mask, const float* clamps, const int32_t* tp2id,
-                    int64_t n_tokens) {
+                    int64_t n_tokens, int64_t rows = (int64_t)1 << 31) {
   if (R < 0 || I < 1 || n_tokens < 0) return MOE_E_BAD_ARG;
   if (act_fn < MOE_ACT_SILU || act_fn > MOE_ACT_SWISH || (clamp_mask & ~15) || (clamp_mask && !clamps)) return MOE_E_BAD_ARG;
   // (the place of a piece within its workgroup's rows is found by a 32-bit multiplication, exact up to here)
-  if (I > 1 << 17 || R >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
+  if (I > 1 << 17 || R >= rows) return MOE_E_BAD_SHAPE;
   a.tp2id = tp2id;
   a.n_tokens = n_tokens;
   a.R = R;
@@ -564,7 +564,7 @@ extern "C" int moe_dequantize_checkpoint(const uint8_t* codes, const uint8_t* sc
                                          void* stream) {
   if (!codes || !scales || !out) return MOE_E_BAD_ARG;
   GluArgs a;
-  const int rc = glu_args(a, rows, I, MOE_ACT_SILU, 0, nullptr, nullptr, 0);
+  const int rc = glu_args(a, rows, I, MOE_ACT_SILU, 0, nullptr, nullptr, 0, (int64_t)1 << 32);  // (a record of R rows has 2 R here)
   if (rc != MOE_OK) return rc;
   return by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;

@@ -194,6 +194,28 @@ def test_more_rows_than_a_launch_has_workgroups(T, H, dtype):
     assert float(d_aff.double().sum()) == total
 
 
+def test_more_rows_of_a_record_than_a_launch_has_threads():
+    """Rows of one value: four pieces each, 2^32 of them past 2^30 rows."""
+    import torch
+    from nkilib.core.moe.glu_checkpoint import dequantize_checkpoint, glu_checkpoint, glu_checkpoint_bwd
+
+    R, far = (1 << 30) + 300, 1 << 30
+    x = torch.ones((R, 2, 1), dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x[-1000:] = torch.randn((1000, 2, 1), generator=g, device="cuda").bfloat16()
+    h, c, s = glu_checkpoint(x)
+    h1, c1, s1 = glu_checkpoint(x[-1000:].contiguous())
+    assert torch.equal(h[-1000:], h1) and torch.equal(c[-1000:], c1) and torch.equal(s[-1000:], s1)
+    assert bool((h[: far - 1000 : 4099] == h[0]).all()) and bool((c[: far - 1000 : 4099] == c[0]).all())
+    del x
+    v = dequantize_checkpoint(c, s)
+    assert torch.equal(v[-1000:], dequantize_checkpoint(c1, s1)) and bool((v[: far - 1000 : 4099] == 1).all())
+    del v
+    d_gu, h2 = glu_checkpoint_bwd(c, s, h)
+    d1, h3 = glu_checkpoint_bwd(c1, s1, h1)
+    assert torch.equal(d_gu[-1000:], d1) and torch.equal(h2[-1000:], h3) and bool((d_gu[: far - 1000 : 4099] == d_gu[0]).all())
+
+
 def test_more_blocks_of_a_checkpoint_than_a_launch_takes():
     import torch
     from nkilib.core.moe.glu_checkpoint import pack_gate_up_checkpoint

@@ -104,6 +104,12 @@ def test_glu_with_kept_bits_refusals(L):
     assert L.moe_glu_checkpoint_bwd_clamped(None, P, P, P, 0, 4, 64, 0, 0, None, None, 0, P, None, None) == BAD_ARG
 
 
+def test_rows_of_a_record_as_its_values(L):
+    """A record of R < 2^31 rows is one of 2 R rows of codes."""
+    assert L.moe_dequantize_checkpoint(P, P, 2**32, 64, P, 0, None) == BAD_SHAPE
+    assert L.moe_glu_checkpoint(P, 0, 2**31, 1, 0, 0, None, None, 0, P, P, P, None) == BAD_SHAPE
+
+
 def test_host_tensors_are_refused():
     """There is no CPU path: the operators say so."""
     import torch
