@@ -22,8 +22,9 @@ def _cumsum(x, axis=-1):
     y = torch.empty_like(x)
     if x.numel() == 0:
         return y
-    rc = nv.lib().moe_cumsum(nv.ptr(x), nv.ptr(y), nv.index_dtype_code(x, "x"), x.numel() // H, H,
-                             nv.stream_ptr(x.device))
+    with nv.on_device(x.device):
+        rc = nv.lib().moe_cumsum(nv.ptr(x), nv.ptr(y), nv.index_dtype_code(x, "x"), x.numel() // H, H,
+                                 nv.stream_ptr(x.device))
     nv.check(rc, "cumsum")
     return y
 

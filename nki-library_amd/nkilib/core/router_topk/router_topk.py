@@ -65,14 +65,15 @@ def _router_topk(x, w, w_bias, router_logits, expert_affinities, expert_index, a
     L = nv.lib()
     # (its size follows T: from the caching allocator, which knows the stream, not from the scratch that only grows)
     ws = torch.empty(L.moe_router_topk_workspace_bytes_for(T, H, E), dtype=torch.uint8, device=dev)
-    rc = L.moe_router_topk(
-        nv.ptr(x), nv.ptr(w), nv.ptr(bias), nv.dtype_code(bias, "w_bias") if bias is not None else 0, T, H, E, int(k),
-        act.value, int(bool(router_pre_norm)), int(bool(norm_topk_prob)), int(bool(_mask_to_topk)), int(bool(_pad_row)),
-        None if skip_store_router_logits else nv.ptr(router_logits),
-        nv.dtype_code(router_logits, "router_logits") if router_logits is not None else 0,
-        None if skip_store_expert_index else nv.ptr(expert_index), nv.ptr(expert_affinities),
-        nv.dtype_code(expert_affinities, "expert_affinities"), nv.ptr(topk_aff), nv.ptr(ws), ws.numel(),
-        nv.stream_ptr(dev))
+    with nv.on_device(dev):
+        rc = L.moe_router_topk(
+            nv.ptr(x), nv.ptr(w), nv.ptr(bias), nv.dtype_code(bias, "w_bias") if bias is not None else 0, T, H, E, int(k),
+            act.value, int(bool(router_pre_norm)), int(bool(norm_topk_prob)), int(bool(_mask_to_topk)), int(bool(_pad_row)),
+            None if skip_store_router_logits else nv.ptr(router_logits),
+            nv.dtype_code(router_logits, "router_logits") if router_logits is not None else 0,
+            None if skip_store_expert_index else nv.ptr(expert_index), nv.ptr(expert_affinities),
+            nv.dtype_code(expert_affinities, "expert_affinities"), nv.ptr(topk_aff), nv.ptr(ws), ws.numel(),
+            nv.stream_ptr(dev))
     nv.check(rc, "router_topk")
     outs = [router_logits, expert_index, expert_affinities]
     if return_eager_affi:

@@ -37,8 +37,9 @@ def _find_nonzero_indices(input_tensor, col_start_id=None, n_cols=None, chunk_si
     counts = torch.empty((C_out,), dtype=torch.int32, device=dev)
     L = nv.lib()
     ws = nv.workspace(dev, L.moe_find_nonzero_indices_workspace_bytes(T, C_out))
-    rc = L.moe_find_nonzero_indices(nv.ptr(x), nv.index_dtype_code(x, "input_tensor"), T, C_full, nv.ptr(start), C_out,
-                                    nv.ptr(indices), nv.ptr(counts), nv.ptr(ws), ws.numel(), nv.stream_ptr(dev))
+    with nv.on_device(dev):
+        rc = L.moe_find_nonzero_indices(nv.ptr(x), nv.index_dtype_code(x, "input_tensor"), T, C_full, nv.ptr(start), C_out,
+                                        nv.ptr(indices), nv.ptr(counts), nv.ptr(ws), ws.numel(), nv.stream_ptr(dev))
     nv.check(rc, "find_nonzero_indices")
     return indices, counts
 

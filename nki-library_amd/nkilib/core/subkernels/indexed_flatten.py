@@ -34,8 +34,9 @@ def _indexed_flatten(input_tensor, f_len, output_len, row_offsets, row_offsets_s
         start = nv.require_device_tensor(row_offsets_start, "row_offsets_start").reshape(-1)
         kernel_assert(start.dtype == torch.int32 and start.numel() == 1, "row_offsets_start must be a [1] int32 tensor")
     out = torch.empty((output_len,), dtype=torch.int32, device=x.device)
-    rc = nv.lib().moe_indexed_flatten(nv.ptr(x), E, T, f_len, output_len, nv.ptr(offs), N, nv.ptr(start),
-                                      int(padding_val), nv.ptr(out), nv.stream_ptr(x.device))
+    with nv.on_device(x.device):
+        rc = nv.lib().moe_indexed_flatten(nv.ptr(x), E, T, f_len, output_len, nv.ptr(offs), N, nv.ptr(start),
+                                          int(padding_val), nv.ptr(out), nv.stream_ptr(x.device))
     nv.check(rc, "indexed_flatten")
     return out
 
