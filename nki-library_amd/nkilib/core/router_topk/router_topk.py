@@ -61,6 +61,15 @@ def _router_topk(x, w, w_bias, router_logits, expert_affinities, expert_index, a
     if expert_index is not None:
         kernel_assert(expert_index.dtype in (torch.int32, torch.uint32) and expert_index.is_contiguous(),
                       "expert_index must be a contiguous 32-bit integer tensor")
+    # (the kernel writes T rows of each output that is stored, one behind the other)
+    for out, what, least, stored in ((expert_affinities, "expert_affinities", rows * E, True),
+                                     (router_logits, "router_logits", T * E, not skip_store_router_logits),
+                                     (expert_index, "expert_index", T * int(k), not skip_store_expert_index)):
+        if stored and (out.device != dev or not out.is_contiguous() or out.numel() < least):
+            kernel_assert(False, f"{what} must be a contiguous tensor of {least} values on {dev} but is {tuple(out.shape)} on {out.device}")
+    for t, what in ((w, "w"), (bias, "w_bias")):
+        if t is not None and t.device != dev:
+            kernel_assert(False, f"{what} must be on {dev} but is on {t.device}")
     topk_aff = torch.empty((T, int(k)), dtype=torch.float32, device=dev) if return_eager_affi else None
     L = nv.lib()
     # (its size follows T: from the caching allocator, which knows the stream, not from the scratch that only grows)

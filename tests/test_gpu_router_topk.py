@@ -208,3 +208,24 @@ def test_route_for_moe_feeds_the_block_build():
     N = get_n_blocks(T, k, E, B, n_block_per_iter=2)
     tp2id, b2e, _ = build_token_blocks(ids, E, B, N, n_conditions=N + 2)
     assert int((tp2id.reshape(-1) < T).sum()) == T * k
+
+
+def test_outputs_that_are_too_small_are_refused():
+    import torch
+    from nkilib.core.router_topk import router_topk
+    from nkilib.core.utils.common_types import RouterActFnType
+
+    T, H, E, k = 9, 128, 8, 2
+    x, w = torch.ones((T, H), device="cuda").bfloat16(), torch.ones((H, E), device="cuda").bfloat16()
+    call = lambda logits, aff, ids, **kw: router_topk(x, w, None, logits, aff, ids, RouterActFnType.SOFTMAX, k, x_hbm_layout=1, **kw)
+    f = lambda *s: torch.zeros(s, device="cuda")
+    i = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+    for logits, aff, ids in ((f(T - 1, E), None, None), (f(E, T).t(), None, None), (f(T, E).cpu(), None, None), (None, f(T - 1, E), None),
+                             (None, f(T, E).cpu(), None), (None, None, i(T, k - 1)), (None, None, i(T, k).cpu())):
+        with pytest.raises(AssertionError, match="NCC_INKI016"):
+            call(logits, aff, ids)
+    got = call(f(T, E), f(T, E), i(T, k))
+    want = call(None, f(T, E), None)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    # what is not stored is not looked at
+    call(f(1, 1), None, i(1, 1), skip_store_router_logits=True, skip_store_expert_index=True)
