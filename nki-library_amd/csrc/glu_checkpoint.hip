@@ -243,16 +243,24 @@ __global__ __launch_bounds__(256) void glu_checkpoint_kernel(const GluArgs a, co
     load8<DT>(gate_up + off * ES, p.n, g);
     load8<DT>(gate_up + (off + a.I) * ES, p.n, u);
   }
-  uint32_t at_g = 0, at_u = 0;
+  if (a.clamped && p.n > 0) {
+    uint32_t at_g = 0, at_u = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (a.clamp_mask) {
+    for (int i = 0; i < 8; ++i) {
       const bool real = p.on && i < p.n;
       if (real && at_limit(g[i], a.clamp_mask, MOE_CLAMP_GATE_HI, MOE_CLAMP_GATE_LO, a.clamp[0], a.clamp[1])) at_g |= 1u << i;
       if (real && at_limit(u[i], a.clamp_mask, MOE_CLAMP_UP_HI, MOE_CLAMP_UP_LO, a.clamp[2], a.clamp[3])) at_u |= 1u << i;
+    }
+    const int64_t G8 = (a.I + 7) / 8;
+    a.clamped[p.row * 2 * G8 + p.v] = (uint8_t)at_g;
+    a.clamped[p.row * 2 * G8 + G8 + p.v] = (uint8_t)at_u;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (a.clamp_mask) {
       g[i] = clamp_value(g[i], a.clamp_mask, MOE_CLAMP_GATE_HI, MOE_CLAMP_GATE_LO, a.clamp[0], a.clamp[1]);
       u[i] = clamp_value(u[i], a.clamp_mask, MOE_CLAMP_UP_HI, MOE_CLAMP_UP_LO, a.clamp[2], a.clamp[3]);
-      if (!real) g[i] = u[i] = 0.f;
+      if (!p.on || i >= p.n) g[i] = u[i] = 0.f;
     }
     float s, xds;
     act_parts<ACT, DT == MOE_DT_FP32>(g[i], s, xds);
@@ -263,11 +271,6 @@ __global__ __launch_bounds__(256) void glu_checkpoint_kernel(const GluArgs a, co
     store8<DT>(h + (p.row * a.I + 8 * p.v) * ES, p.n, r);
     store_codes(codes + off, p.n, encode8(g, sg));
     store_codes(codes + off + a.I, p.n, encode8(u, su));
-    if (a.clamped) {
-      const int64_t G8 = (a.I + 7) / 8;
-      a.clamped[p.row * 2 * G8 + p.v] = (uint8_t)at_g;
-      a.clamped[p.row * 2 * G8 + G8 + p.v] = (uint8_t)at_u;
-    }
   }
   if ((p.v & 3) == 0) {
     scales[p.row * 2 * G + p.v / 4] = (uint8_t)sg;
