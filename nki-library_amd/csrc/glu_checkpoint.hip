@@ -278,8 +278,9 @@ __global__ __launch_bounds__(256) void glu_checkpoint_kernel(const GluArgs a, co
   }
 }
 
+// (fp32 rows: four waves per SIMD at most; 98048 rows (65536) of 2048 take 680 us so and 720 with eight, bf16 rows 299 and 278)
 template <int DT, int ACT>
-__global__ __launch_bounds__(256) void glu_checkpoint_bwd_kernel(const GluArgs a, const uint8_t* __restrict__ codes,
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, DT == MOE_DT_FP32 ? 4 : 8))) void glu_checkpoint_bwd_kernel(const GluArgs a, const uint8_t* __restrict__ codes,
                                                                  const uint8_t* __restrict__ scales,
                                                                  const uint8_t* __restrict__ dh, uint8_t* __restrict__ d_gate_up,
                                                                  uint8_t* __restrict__ h) {
