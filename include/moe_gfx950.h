@@ -382,7 +382,7 @@ int moe_prepare_kmajor_weights(const moe_bwmm_args* args, void* gate_up_kmajor, 
  * moe_permute_tokens: out[s] = x[token of s], zero rows for padding; any element type (rows of row_bytes < 2^31 bytes).
  *
  * moe_combine_tokens: out[t] = sum over t's slots s of expert_affinities[t, e(s)] * y[s]; affinities [T1 >= T, E] bf16 / fp32.
- * Slots of blocks whose expert is outside [0, E) count for nothing and are not read; rows of padding slots are not read.  With
+ * Slots of blocks whose expert is outside [0, E) count for nothing, whatever their rows hold; rows of padding slots are not read.  With
  * expert_affinities and block_to_expert NULL every weight is 1: the backward pass of moe_permute_tokens.  S = N * B rows in y.
  *
  * moe_combine_tokens_bwd: d_y[s] = expert_affinities[t, e(s)] * d_out[t], zero rows for padding; d_affinities fp32 [T1, E] =
@@ -408,7 +408,7 @@ int moe_combine_tokens_bwd(const void* d_out, const void* y, int dtype, const vo
  * code * 2^(byte - 127).  The scale is the smallest power of two with amax / scale <= 448 over the group's finite values;
  * infinities and NaN are kept as NaN codes.  I <= 131072, R < 2^31.  clamp_mask: MOE_CLAMP_*; clamps: host, gate upper, gate lower, up
  * upper, up lower (NULL when clamp_mask is 0).  token_position_to_id int32 [R] (nullable): rows of padding slots (outside
- * [0, n_tokens)) are not read, and zero in every output.
+ * [0, n_tokens)) have no part in a result, whatever they hold, and are zero in every output.
  *
  * moe_glu_checkpoint: gate_up [R, 2, I] -> intermediate [R, I] = act(gate) * up and the record of the clamped values.
  * moe_pack_gate_up_checkpoint: the same record of what moe_blockwise left in gate_up_activations_T (bf16 [N, 2, I, B]; R = N*B).

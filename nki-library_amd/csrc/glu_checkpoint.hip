@@ -20,10 +20,13 @@
 // act(x) = x s(x) for every kind: SiLU and Swish s = sigmoid(a x); GELU s = Phi(x); its tanh form 0.5 (1 + tanh z) = sigmoid(2 z).
 // All of it moves bytes: a pair of values costs 4 + 2 + 2 + 1/16 bytes forward in bf16, 2 + 1/16 + 2 + 4 + 2 backward.  Four lanes
 // share a group of 32, eight values each (16 bytes of bf16), so that a group's maximum is two exchanges between neighbours.
-// Rows of padding slots are neither read nor computed: their outputs are zero.
+// Rows of padding slots have no part in a result and zero outputs: the forward pass works them out as zeros, the backward pass leaves
+// them out, neither reads them; the pack reads what lies in a tile beside a token's row.
 // Measured: forward, fp16, 9088 rows (8192 of tokens) of I = 14336 174 us = 5.7 TB/s; backward, bf16, 98048 rows (65536) of 2048
-// 311 us = 5.6 TB/s, 330 with stores that stay in the caches, 321 with such loads; pack of 1408 rows (512) of 1024 8.7 us, of which the
+// 282 us = 6.2 TB/s, 296 with stores that stay in the caches, 286 with such loads; pack of 1408 rows (512) of 1024 8.7 us, of which the
 // bytes are 2 (with 2-byte loads and a lookup of the row's id for each 14).  A copy moves 4.9 TB/s, a fill 6.9.
+// 98048 rows (65536) of 2048, forward | backward, us: bf16 SiLU 230 | 278, Swish with clamps 263 | 288, with their bits 302 | 286, GELU
+// (erfc: arithmetic) 372 | 355; fp32 456 | 680.
 #include <type_traits>
 
 #include "rows.hpp"
@@ -35,7 +38,7 @@ struct GluArgs {
   int64_t n_tokens, R;
   int64_t I, V;          // V: pieces of eight values per row of I, a multiple of four (those past I are empty)
   uint32_t v_magic;      // ceil(2^32 / V)
-  int act_fn, clamp_mask;
+  int clamp_mask;
   float clamp[4];        // gate upper, gate lower, up upper, up lower
   float clamp16[4];      // the same as bf16 holds them: what the layer's checkpoint has of a clamped value
   uint8_t* clamped;      // [R][2][ceil(I/8)] or null: bit i of byte v for value 8 v + i
@@ -464,7 +467,6 @@ static int glu_args(GluArgs& a, int64_t R, int64_t I, int act_fn, int clamp_mask
   a.I = I;
   a.V = (I + 31) / 32 * 4;
   a.v_magic = (uint32_t)((((uint64_t)1 << 32) + a.V - 1) / a.V);
-  a.act_fn = act_fn;
   a.clamp_mask = clamp_mask;
   a.clamped = nullptr;
   for (int i = 0; i < 4; ++i) {

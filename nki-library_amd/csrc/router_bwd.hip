@@ -22,8 +22,8 @@
 //                              power leaves, and router_dx_list_kernel, by the vector ALU: 75 instructions a token and 256
 //                              columns, half of them to unpack w);
 //   3. router_reduce_kernel    the sums of the parts of dw and of db (large calls: the workgroups of dx, when done).
-// T = 8192, H = 7168, E = 256, top-8: 9 + 57 + 50 us; 52 for its bytes at the rate of a copy and 50 for 2 x 2 x 30 GFLOP at
-// that of a large product.
+// T = 8192, H = 7168, E = 256, top-8: 9 + 57 + 50 us; 52 for its bytes at the rate of a copy and 50 for 2 x 30 GFLOP, the products of
+// dw and of dx, at that of a large product.  (dw alone, with hi and lo, is as much.)
 #include <type_traits>
 
 #include "common.hpp"
@@ -40,7 +40,7 @@ struct RouterBwdArgs {
   const int32_t* ids;
   int aff_dtype, logits_dtype;
   int64_t T, H, E, k;
-  int softmax, chosen, norm, full;  // chosen: activation of the chosen logits only; full: affinities of all experts were handed out
+  int softmax, norm, full;          // full: affinities of all experts were handed out
   int dense, kp;                    // dense: every expert has a part in dl; kp: k rounded up to a power of two
   u32x4* dlx;   // [tokens / 16][KS][2][64]   K = experts, for dx
   u32x4* dlw;   // [tokens / 32][2 KS][2][64] K = tokens, for dw
@@ -697,10 +697,9 @@ extern "C" int moe_router_topk_bwd(const void* d_affinities, int aff_dtype, cons
   a.logits_dtype = logits_dtype;
   a.T = T; a.H = H; a.E = E; a.k = k;
   a.softmax = act_fn == 1;
-  a.chosen = !router_pre_norm;
   a.norm = router_pre_norm && norm_topk_prob;
   a.full = router_pre_norm && !norm_topk_prob && !mask_to_topk;
-  a.dense = a.full || (a.softmax && !a.chosen && !a.norm);
+  a.dense = a.full || (a.softmax && router_pre_norm && !a.norm);
   a.kp = k > 4 ? 8 : k > 2 ? 4 : 2;
   a.dlx = (u32x4*)(ws + p.dlx);
   a.dlw = (u32x4*)(ws + p.dlw);

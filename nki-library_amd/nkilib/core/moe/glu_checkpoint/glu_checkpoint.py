@@ -13,8 +13,10 @@ largest finite value of its group within 448.  Infinities and NaN become NaN and
 Where values are clamped, the record alone does not tell a clamped value from one that is rounded to its limit: see ``clamped`` of
 ``glu_checkpoint_bwd``.
 
-With ``token_position_to_id`` (one id per row) and ``n_tokens``, rows of padding slots (ids outside ``[0, n_tokens)``) are not
-read and are zero in every output.
+With ``token_position_to_id`` (one id per row) and ``n_tokens``, rows of padding slots (ids outside ``[0, n_tokens)``) have no part
+in a result, whatever they hold, and are zero in every output.
+
+Plain calls, outside of torch's autograd: what they return has no graph, also where an input requires a gradient.
 """
 
 import ctypes

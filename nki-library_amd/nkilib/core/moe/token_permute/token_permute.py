@@ -12,6 +12,8 @@ runs the backward pass of a layer, does it through these operators, on the table
 Slot s holds token ``token_position_to_id[s]``; ids outside ``[0, T)`` (T, or -1 with ``skip_token``) are padding, whose rows
 are zero on the way out and never read on the way in.  Sums are taken over a token's slots in ascending order in fp32 and
 rounded once.  Rows are bfloat16, float16 or float32.
+
+Plain calls, outside of torch's autograd: what they return has no graph, also where an input requires a gradient.
 """
 
 from typing import Optional

@@ -1,7 +1,7 @@
 """The gradient of ``router_topk`` over ``moe_router_topk_bwd`` of the C ABI.
 
 The reference has the forward pass only (src/nkilib_src/nkilib/core/router_topk/router_topk.py:55-75); the formulas are those of
-its semantics (router_topk_torch.py:23-135), differentiated.
+its semantics (router_topk_torch.py:23-135), differentiated.  A plain call, outside of torch's autograd: it returns no graph.
 """
 
 import torch
@@ -13,14 +13,18 @@ from ..utils.kernel_assert import kernel_assert
 
 def router_topk_bwd(d_expert_affinities, x, w, w_bias, router_logits, expert_index, act_fn, router_pre_norm=True,
                     norm_topk_prob=False, mask_to_topk=True):
-    """``d_expert_affinities`` ``[T or more, E]`` float32 or bfloat16 (``combine_tokens_bwd`` returns it) -> gradients
+    """By default the gradient of ``route_for_moe``, whose affinities are zero outside of the choice.  That of ``router_topk``'s full table
+    (its default, ``norm_topk_prob=False``: every expert has an affinity, and a loss over all of them a gradient) needs
+    ``mask_to_topk=False``; with ``True`` gradients of experts that were not chosen are ignored.
+
+    ``d_expert_affinities`` ``[T or more, E]`` float32 or bfloat16 (``combine_tokens_bwd`` returns it) -> gradients
     ``[d_x [T, H], d_w [H, E], d_bias]`` in the types of ``x``, ``w`` (bfloat16) and ``w_bias`` (``None`` without one).
 
     ``x`` ``[T, H]`` (``x_hbm_layout=1``), ``w`` ``[H, E]``, ``w_bias`` and the options are those of the forward call;
     ``router_logits`` ``[T, E]`` (float32, or bfloat16 at that precision) and ``expert_index`` ``[T, k]`` are what it returned.
-    ``mask_to_topk``: the affinities went to the selected experts only, as in ``route_for_moe`` and the tables of the block
-    build, and gradients of others are ignored; ``False`` differentiates the full table that ``router_topk`` returns without
-    ``norm_topk_prob``.  The gradient of the logits stays in fp32 and enters the products as a sum of two bf16."""
+    (``norm_topk_prob`` or ``router_pre_norm=False`` leave the selected experts alone an affinity, and ``mask_to_topk`` no choice.)
+    The gradient of the logits is fp32; into ``d_w``, and into the ``d_x`` of a softmax over all experts or of the full table, it enters
+    as the sum of two bf16 (2^-17 of it)."""
     x = nv.require_device_tensor(x, "x")
     w = nv.require_device_tensor(w, "w")
     g = nv.require_device_tensor(d_expert_affinities, "d_expert_affinities")
