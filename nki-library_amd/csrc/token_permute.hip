@@ -124,7 +124,8 @@ __global__ __launch_bounds__(1024) void rank_slots_kernel(int64_t T, int k, int 
 
 typedef uint32_t bytes16 __attribute__((ext_vector_type(4), aligned(1)));
 
-constexpr int64_t SHORT_ROW = 4096;  // bytes of a row that is a wave's work
+constexpr int64_t SHORT_ROW = 4096;           // bytes of a row that is a wave's work
+constexpr int64_t SHORT_WEIGHTED_ROW = 5120;  // with weights, in the combine
 // TPR threads per row or part of a row (a whole number of waves, so that everything about a row is uniform).
 template <int TPR>
 __device__ __forceinline__ int64_t row_of_group() {
@@ -486,11 +487,13 @@ extern "C" int moe_permute_tokens(const void* x, const int32_t* token_position_t
 template <int DT>
 static void launch_combine_tokens(const void* y, const SlotTables& a, const int32_t* tp2id, int64_t T, int64_t H, void* out,
                                   hipStream_t s) {
-  // a workgroup per token, or a wave where rows are short and tokens many (us a call, top-8 of 128 experts, caches cold, wave and
-  // workgroup: 1024 tokens of 1 KB 15.6 and 15.6, 3 KB 19.6 and 18.3; 8192 of 1 KB 35 and 37, 3 KB 59 and 68, 8 KB 130 and 125;
-  // the kernel for 8192 of 4 KB, whose pieces a workgroup has one of per thread, weighted 62 and 64, else 59 and 52); few tokens
-  // (decode): several per token, a piece per thread
-  const bool wide = H * Elem<DT>::SIZE >= SHORT_ROW || T < 2048;
+  // a workgroup per token, or a wave where rows are short and tokens many: weighted, each of a workgroup's four waves works out the
+  // weights, so that a wave alone pays up to longer rows (us a call with lists made before, bf16, wave | workgroup: 8192 tokens in 8
+  // slots of 2.0 KB 29.9 | 36.4, 3.9 KB 56.2 | 63.0, 4.0 KB 60.8 | 63.7, 4.5 KB 66.6 | 69.9, 5.5 KB 81.0 | 78.7, in 2 of 4.5 KB 26.2 |
+  // 32.0, 5.5 KB 31.0 | 34.7; unweighted in 8 of 1.0 KB 15.2 | 15.9, 2.0 KB 28.3 | 27.7, 3.9 KB 54.8 | 50.6, 4.0 KB 58.3 | 53.1, in 2 of
+  // 2.0 KB 12.0 | 16.8, 3.9 KB 20.9 | 22.3, 4.0 KB 22.5 | 22.3, 5.5 KB 29.6 | 28.8; 20000 tokens alike); few tokens (decode): several
+  // workgroups per token, a piece per thread
+  const bool wide = H * Elem<DT>::SIZE >= (a.b2e ? SHORT_WEIGHTED_ROW : SHORT_ROW) || T < 2048;
   const int64_t groups = wide ? T : (T + 3) / 4;
   int64_t parts = 1;
   if (wide && groups < 512) {

@@ -228,3 +228,32 @@ def test_more_blocks_of_a_checkpoint_than_a_launch_takes():
     assert torch.equal(c[-1000:], c1) and torch.equal(s[-1000:], s1)
     assert bool((c[:-1000] == c[0]).all()) and bool((s[:-1000] == s[0]).all())
     assert np.array_equal(c1.cpu().numpy(), ot.record(x[-1000:, :, :, 0].float().cpu().numpy())[0])
+
+
+@pytest.mark.parametrize("H,dtype", [(2047, "bfloat16"), (2048, "float16"), (2559, "bfloat16"), (2560, "bfloat16"), (1279, "float32"), (1281, "float32")])
+def test_a_row_is_summed_alike_by_a_wave_and_by_a_workgroup(H, dtype):
+    """Few tokens (a workgroup each) and the same among many (a wave each, up to the rule's length): the same bits."""
+    import torch
+    from nkilib.core.moe.token_permute import combine_tokens, permute_tokens_bwd
+
+    g = torch.Generator(device="cuda").manual_seed(H)
+    E, k, B = 8, 3, 16
+    for T in (2047, 2048):
+        ids = torch.arange(T * k, device="cuda", dtype=torch.int32) // k
+        N = (T * k + B - 1) // B
+        tp = torch.full((N * B,), T, dtype=torch.int32, device="cuda")
+        tp[: T * k] = ids[torch.randperm(T * k, generator=g, device="cuda")]
+        tp[: T * k][tp[: T * k] == T - 1] = T  # (the last token has no slot)
+        if T == 2047:
+            be = torch.randint(0, E, (N,), generator=g, device="cuda").int()
+            y = torch.randn((N * B, H), generator=g, device="cuda").to(getattr(torch, dtype))
+            aff = torch.rand((T, E), generator=g, device="cuda")
+            first = (tp, be, y, aff)
+            want = combine_tokens(y, aff, tp, be, B, T, k), permute_tokens_bwd(y, tp, T, k)
+        else:
+            tp, be, y, aff = first
+            aff = torch.cat((aff, aff[:1]))
+            tp = torch.where(tp == 2047, -1, tp)
+            got = combine_tokens(y, aff, tp, be, B, T, k), permute_tokens_bwd(y, tp, T, k)
+            for a, b in zip(got, want):
+                assert torch.equal(a[:2047], b) and not a[2047].any()
