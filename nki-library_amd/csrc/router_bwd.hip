@@ -572,9 +572,11 @@ __global__ __launch_bounds__(GRAD_THREADS) void router_grad_kernel(const RouterB
 __global__ __launch_bounds__(256) void router_reduce_kernel(const RouterBwdArgs a) { reduce_parts(a, 256); }
 
 // Or dw, and then dx with the sums behind it: dx by lists needs a quarter of dw's registers, so that a CU has 16 waves of it instead
-// of 8.  In one launch | two, us of a call: 128 tokens, top-8 of 128, H = 2048 15.6 | 19.3; 1999, top-4 of 60, 4096 24 |
-// 26; 8192, top-8 of 256, 7168 128 | 112.
-constexpr int64_t ONE_LAUNCH_VALUES = (int64_t)1 << 24;  // of x
+// of 8, and gains by it the earlier the more dw there is beside a token, which goes by the experts (k changes little).  In one
+// launch | two, us of a call by values of x (2^20): top-4 of 60 experts 8: 24.5 | 27.4, 16: 29.9 | 31.7, 32: 43.3 | 43.8; top-8 of 64 8:
+// 27.1 | 28.3, 16: 35.4 | 35.6, 32: 54.3 | 52.0; top-2 of 8 32: 38.3 | 39.6; top-8 of 128 4: 28.1 | 29.3, 8: 37.0 | 34.5, 16: 47.5 | 44.2;
+// top-2 of 128 4: 24.6 | 26.9, 8: 32.6 | 31.2; top-8 of 256 3.5: 35.7 | 37.6, 7: 42.1 | 38.5, 28: 75.7 | 64.5; of 512 4: 45.3 | 40.8.
+static int64_t one_launch_values(int64_t E) { return E <= 64 ? (int64_t)16 << 20 : (int64_t)6 << 20; }
 template <int KS>
 __global__ __launch_bounds__(GRAD_THREADS) void router_dw_kernel(const RouterBwdArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[DW_LDS];
@@ -626,7 +628,7 @@ static int launch_grad(RouterBwdArgs& a, hipStream_t s) {
   if (a.x_splits < 1) a.x_splits = 1;
   const int64_t n_dx = groups * a.x_splits;
   if constexpr (KP > 0) {
-    if (a.T * a.H > ONE_LAUNCH_VALUES) {
+    if (a.T * a.H > one_launch_values(a.E)) {
       constexpr int CPL = KS > 8 ? 2 : 4;
       if (allow_lds<router_dx_list_kernel<CPL, KP>>(GRAD_LDS) != hipSuccess) return MOE_E_LAUNCH;
       hipLaunchKernelGGL(router_dw_kernel<KS>, dim3((unsigned)a.n_dw), dim3(GRAD_THREADS), 0, s, a);

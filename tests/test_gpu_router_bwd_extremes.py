@@ -3,6 +3,7 @@
 import numpy as np
 import pytest
 
+import test_gpu_router_topk_bwd as base
 from test_gpu_router_topk_bwd import MODES, _case, _check, _dl_limits
 from train_helpers import tensor, values
 
@@ -105,3 +106,11 @@ def test_the_same_call_gives_the_same_bits():
         first = _call(g, x, w, l, ids, mode, torch.zeros(E, device="cuda"))
         for _ in range(3):
             assert all(torch.equal(a, b) for a, b in zip(first, _call(g, x, w, l, ids, mode, torch.zeros(E, device="cuda"))))
+
+
+# dw and dx in two launches from 16 M values of x on for up to 64 experts, from 6 M on beyond: every instance of either side
+@pytest.mark.parametrize("T,H,E,k,softmax", [(8200, 2176, 8, 2, False), (8200, 2176, 60, 3, True), (8200, 2176, 64, 7, False), (7600, 2176, 64, 8, True),
+                                             (3100, 2176, 65, 1, True), (3100, 2176, 128, 4, False), (3100, 2176, 128, 8, False), (2800, 2176, 128, 8, False),
+                                             (3100, 2176, 200, 2, True), (3100, 2176, 256, 5, False), (3100, 2176, 257, 4, True), (3100, 2176, 512, 8, False)])
+def test_one_launch_and_two(T, H, E, k, softmax):
+    base.test_large_shapes_on_the_device(T, H, E, k, softmax)
