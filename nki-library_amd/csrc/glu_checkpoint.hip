@@ -591,7 +591,7 @@ extern "C" int moe_pack_gate_up_checkpoint_clamped(const void* gate_up_activatio
                                                    uint8_t* codes, uint8_t* scales, uint8_t* clamped, void* stream) {
   if (!gate_up_activations_T || !codes || !scales || N < 0 || I < 1 || B < 1 || n_tokens < 0) return MOE_E_BAD_ARG;
   if ((clamp_mask & ~15) || (clamp_mask && !clamps)) return MOE_E_BAD_ARG;
-  if (I > 1 << 17 || N * B >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
+  if (I > 1 << 17 || N >= (int64_t)1 << 31 || B >= (int64_t)1 << 31 || N * B >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
   int ltb = 0;
   while (ltb < 6 && (1 << ltb) < B) ++ltb;
   const int tb = 1 << ltb, tc = PACK_TILE >> ltb;

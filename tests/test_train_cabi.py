@@ -110,6 +110,12 @@ def test_rows_of_a_record_as_its_values(L):
     assert L.moe_glu_checkpoint(P, 0, 2**31, 1, 0, 0, None, None, 0, P, P, P, None) == BAD_SHAPE
 
 
+def test_blocks_whose_product_is_past_64_bits_are_refused(L):
+    pack = lambda N, B: L.moe_pack_gate_up_checkpoint(P, N, 1, B, None, 0, P, P, None)
+    for N, B in ((2**62, 4), (4, 2**62), (2**33, 2**31), (2**31, 1), (1, 2**31)):
+        assert pack(N, B) == BAD_SHAPE, (N, B)
+
+
 def test_host_tensors_are_refused():
     """There is no CPU path: the operators say so."""
     import torch
