@@ -12,21 +12,21 @@
 //   backward   record, dh -> du = dh act(g), dg = dh u act'(g) (0 at and beyond a clamp), and h again for the down weights'
 //              gradient
 //
-// A clamped value is recorded as its limit rounded to e4m3 (7.2 as 7.0 or as 7.5, as the scale has it), so a record's value is at its
-// clamp where it reaches what the record makes of the limit in its group, not the limit itself.  Values that were not clamped but
-// round to the same code, up to half a step inside, cannot be told from those and count as clamped, unless the forward pass also keeps a
-// bit per value (`clamped`, an eighth of a record's bytes, one for the eight values of a lane) and the backward pass goes by those.
+// A clamped value is recorded as its limit rounded to e4m3 (7.2 as 7.0), so a record's value is at its clamp where it reaches
+// what the record makes of the limit in its group, not the limit itself.  Values that were not clamped but round to the same
+// code, up to half a step inside, cannot be told from those and count as clamped, unless the forward pass also keeps a bit per
+// value (`clamped`, an eighth of a record's bytes, one for the eight values of a lane) and the backward pass goes by those.
 //
 // act(x) = x s(x) for every kind: SiLU and Swish s = sigmoid(a x); GELU s = Phi(x); its tanh form 0.5 (1 + tanh z) = sigmoid(2 z).
 // All of it moves bytes: a pair of values costs 4 + 2 + 2 + 1/16 bytes forward in bf16, 2 + 1/16 + 2 + 4 + 2 backward.  Four lanes
 // share a group of 32, eight values each (16 bytes of bf16), so that a group's maximum is two exchanges between neighbours.
-// Rows of padding slots have no part in a result and zero outputs: the forward pass works them out as zeros, the backward pass leaves
-// them out, neither reads them; the pack reads what lies in a tile beside a token's row.
+// Rows of padding slots have no part in a result and zero outputs: the forward pass works them out as zeros, the backward pass
+// leaves them out, neither reads them; the pack reads what lies in a tile beside a token's row.
 // Measured: forward, fp16, 9088 rows (8192 of tokens) of I = 14336 174 us = 5.7 TB/s; backward, bf16, 98048 rows (65536) of 2048
-// 282 us = 6.2 TB/s, 296 with stores that stay in the caches, 286 with such loads; pack of 1408 rows (512) of 1024 8.7 us, of which the
-// bytes are 2 (with 2-byte loads and a lookup of the row's id for each 14).  A copy moves 4.9 TB/s, a fill 6.9.
-// 98048 rows (65536) of 2048, forward | backward, us: bf16 SiLU 230 | 278, Swish with clamps 263 | 288, with their bits 302 | 286, GELU
-// (erfc: arithmetic) 372 | 355; fp32 456 | 680.
+// 282 us = 6.2 TB/s, 296 with stores that stay in the caches, 286 with such loads; pack of 1408 rows (512) of 1024 8.7 us, of
+// which the bytes are 2 (with 2-byte loads and a lookup of the row's id for each 14).  A copy moves 4.9 TB/s, a fill 6.9.
+// 98048 rows (65536) of 2048, forward | backward, us: bf16 SiLU 230 | 278, Swish with clamps 263 | 288, with their bits 302 |
+// 286, GELU (erfc: arithmetic) 372 | 355; fp32 456 | 680.
 #include <type_traits>
 
 #include "rows.hpp"
@@ -132,9 +132,9 @@ __device__ __forceinline__ void decode8(const uint2& c, uint32_t byte, float (&v
     v[4 * h + 3] = b[1] * s;
   }
 }
-// The limits of a gate or up group as its record holds them.  The value recorded is the limit itself or, by way of moe_cte's checkpoint,
-// its bf16, which may round to another code (7.2503 to 7.5, its bf16 7.25 to 7.0): the one further inside.  A limit above 448 times the
-// scale is above every value of the group and stays what it is.
+// The limits of a gate or up group as its record holds them.  The value recorded is the limit itself or, by way of moe_cte's
+// checkpoint, its bf16, which may round to another code (7.2503 to 7.5, its bf16 7.25 to 7.0): the one further inside.  A limit
+// above 448 times the scale is above every value of the group and stays what it is.
 __device__ __forceinline__ void recorded_limits(const GluArgs& a, int upper, uint32_t byte, float& hi, float& lo) {
   const float inv = mx_inv_scale(byte), s = scale_value(byte);
   const float v[4] = {a.clamp[upper], a.clamp16[upper], a.clamp[upper + 1], a.clamp16[upper + 1]};
@@ -281,9 +281,11 @@ __global__ __launch_bounds__(256) void glu_checkpoint_kernel(const GluArgs a, co
   }
 }
 
-// (fp32 rows: four waves per SIMD at most; 98048 rows (65536) of 2048 take 680 us so and 720 with eight, bf16 rows 299 and 278)
+// Waves per SIMD: four at most for fp32 rows, eight for rows of 16 bits; 98048 rows (65536) of 2048 take, us, with four and with
+// eight: fp32 680 and 720, bf16 299 and 278.
 template <int DT, int ACT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, DT == MOE_DT_FP32 ? 4 : 8))) void glu_checkpoint_bwd_kernel(const GluArgs a, const uint8_t* __restrict__ codes,
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, DT == MOE_DT_FP32 ? 4 : 8)))
+void glu_checkpoint_bwd_kernel(const GluArgs a, const uint8_t* __restrict__ codes,
                                                                  const uint8_t* __restrict__ scales,
                                                                  const uint8_t* __restrict__ dh, uint8_t* __restrict__ d_gate_up,
                                                                  uint8_t* __restrict__ h) {
@@ -355,7 +357,8 @@ __global__ __launch_bounds__(256) void dequantize_checkpoint_kernel(const GluArg
 // a row and a group of 32 columns per thread.  Two bytes per value from LDS: neighbouring lanes hold neighbouring rows.
 // (Groups lie max(8, tb) values apart beyond their length, so that lanes of several groups do not meet in a bank.)
 constexpr int PACK_TILE = 8192;
-// The limits of gate and of up as the checkpoint holds them (bf16; NaN, which nothing reaches, where there is none), for `out`: which values lie there.
+// The limits of gate and of up as the checkpoint holds them (bf16; NaN, which nothing reaches, where there is none), for `out`:
+// which values lie there.
 struct PackClamps {
   float hi[2], lo[2];
   uint8_t* out;  // [N B][2][ceil(I/8)] or null
@@ -570,7 +573,8 @@ extern "C" int moe_dequantize_checkpoint(const uint8_t* codes, const uint8_t* sc
                                          void* stream) {
   if (!codes || !scales || !out) return MOE_E_BAD_ARG;
   GluArgs a;
-  const int rc = glu_args(a, rows, I, MOE_ACT_SILU, 0, nullptr, nullptr, 0, (int64_t)1 << 32);  // (a record of R rows has 2 R here)
+  // (a record of R rows has 2 R here)
+  const int rc = glu_args(a, rows, I, MOE_ACT_SILU, 0, nullptr, nullptr, 0, (int64_t)1 << 32);
   if (rc != MOE_OK) return rc;
   return by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;

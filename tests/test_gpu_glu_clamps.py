@@ -137,10 +137,11 @@ def test_a_clamped_layer_and_its_gradient():
     clamps = (0.8, -0.7, 0.9, -0.7)
     spec = MoECTESpec(MoECTEImplementation.shard_on_i_dropping, shard_on_I=ShardOnIConfig(checkpoint_activation=True))
     _, gate_up_T, _ = moe_cte(x, aff.reshape(-1, 1), wgu, wd, tp, be, B, spec, **_kwargs(clamps))
-    codes, scales = pack_gate_up_checkpoint(gate_up_T, tp, T)
-    d_gu, _ = glu_checkpoint_bwd(codes, scales, torch.ones((be.numel() * B, I), device="cuda"), token_position_to_id=tp,
-                                 n_tokens=T, **_kwargs(clamps))
-    got, tpn = values(d_gu), tp.cpu().numpy()
+    codes, scales, clamped = pack_gate_up_checkpoint(gate_up_T, tp, T, **_kwargs(clamps), return_clamped=True)
+    opts = dict(token_position_to_id=tp, n_tokens=T, **_kwargs(clamps))
+    ones = torch.ones((be.numel() * B, I), device="cuda")
+    got, tpn = values(glu_checkpoint_bwd(codes, scales, ones, **opts)[0]), tp.cpu().numpy()
+    told, bits = values(glu_checkpoint_bwd(codes, scales, ones, **opts, clamped=clamped)[0]), _bits(clamped, I)
     xv, wv, seen = values(x), values(wgu), 0
     for e in range(E):
         rows = np.flatnonzero((tpn >= 0) & (tpn < T) & (np.repeat(be.cpu().numpy(), B) == e))
@@ -155,6 +156,10 @@ def test_a_clamped_layer_and_its_gradient():
             assert not got[rows, half][out].any()
             both = inside & (np.abs(pre[:, 1 - half]) > 0.02)
             assert got[rows, half][both].all()
+            # with the bits: all that lies further inside than half a step of bf16 (2^-8, twice that here)
+            near = (p < hi * (1 - 2.0**-7) - o) & (p > lo * (1 - 2.0**-7) + o)
+            assert bits[rows, half][out].all() and not bits[rows, half][near].any() and not told[rows, half][out].any()
+            assert told[rows, half][near & (np.abs(p) > 0.02) & (np.abs(pre[:, 1 - half]) > 0.02)].all()
             seen += out.sum()
     assert seen > 1000
 
