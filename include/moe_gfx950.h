@@ -443,6 +443,32 @@ int moe_glu_checkpoint_bwd_clamped(const uint8_t* codes, const uint8_t* scales, 
 int moe_dequantize_checkpoint(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t I, void* out, int dtype,
                               void* stream);
 
+/* ---- products of the rows of every expert ------------------------------------------------------ */
+
+/* No counterpart in the reference (its layers multiply the experts inside, bwmm_shard_on_block.py:972-1038).  Rows
+ * row_offsets[e] .. row_offsets[e + 1] (int32 [E + 1], device) are expert e's; whatever the offsets are, they are taken into [0, S] and
+ * as never falling, and rows of no expert are zero in the result.  E <= 1024; K, N in [1, 2^20]; S < 2^31 - 1024.  Sums are taken in fp32 and
+ * rounded once.  Pointers aligned to their element; rows whose pitch and tensors whose address are multiples of 16 bytes are faster.
+ *
+ * moe_expert_row_offsets: block_to_expert [N], experts ascending (blocks of no expert in [0, E) behind the others), B rows a block ->
+ * row_offsets.
+ * moe_grouped_matmul: x [S, K], weight [E, K, N] -> out [S, N], all bf16 or all fp16.
+ * moe_grouped_matmul_bwd: d_out [S, N] -> d_x [S, K] (NULL: not asked for) and d_weight [E, K, N] (NULL: not asked for) of `dtype` or
+ * fp32, zero for an expert without rows.
+ * moe_int8_matmul: x int8 [S, K] with x_scales fp32 [S], weight int8 [E, N, K] with weight_scales fp32 [E, N] -> out [S, N] bf16,
+ * fp16 or fp32 = sum * x_scale * weight_scale (+ bias [N] of out's type).  row_offsets NULL: one matrix for all rows (E = 1); bias only
+ * then.  Sums are exact (int32): K < 2^17. */
+int moe_expert_row_offsets(const int32_t* block_to_expert, int64_t N, int64_t B, int64_t E, int32_t* row_offsets,
+                           void* stream);
+int moe_grouped_matmul(const void* x, const void* weight, int dtype, const int32_t* row_offsets, int64_t S, int64_t K,
+                       int64_t N, int64_t E, void* out, void* stream);
+int moe_grouped_matmul_bwd(const void* d_out, const void* x, const void* weight, int dtype, const int32_t* row_offsets,
+                           int64_t S, int64_t K, int64_t N, int64_t E, void* d_x, void* d_weight, int d_weight_dtype,
+                           void* stream);
+int moe_int8_matmul(const int8_t* x, const float* x_scales, const int8_t* weight, const float* weight_scales,
+                    const void* bias, const int32_t* row_offsets, int64_t S, int64_t K, int64_t N, int64_t E, void* out,
+                    int out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,7 +21,9 @@ OBJ_DIR = os.path.join(HERE, "build")
 OUT_DIR = os.path.join(HERE, "nkilib", "_lib")
 OUT = os.path.join(OUT_DIR, "libmoe_gfx950.so")
 SOURCES = ["rmsnorm_quant.hip", "build_blocks.hip", "combine.hip", "bwmm.hip", "bwmm_mx.hip", "bwmm_rows.hip", "router_topk.hip", "index_ops.hip", "token_permute.hip",
-           "glu_checkpoint.hip", "router_bwd.hip", "capi.hip"]
+           "glu_checkpoint.hip", "router_bwd.hip", "grouped_gemm.hip", "capi.hip"]
+# element types of the tiles of the grouped products, one translation unit each; types as GG_* in csrc/grouped_gemm.hpp
+GG_TYPES = {0: "bf16", 1: "fp16", 2: "int8"}
 # (stage, weight format, K that ends inside a slice) instances of the large-tile MX GEMM; formats as MX_WFMT_* in csrc/bwmm.hpp
 MX_INSTANCES = [(1, 4, 0), (1, 3, 0), (1, 0, 0), (1, 1, 0), (1, 2, 0), (2, 4, 0), (2, 3, 0), (2, 0, 0), (2, 1, 0), (2, 2, 0),
                 (2, 0, 1), (2, 1, 1), (2, 2, 1)]
@@ -33,8 +35,8 @@ FLAGS = [
     # packed fp32 ALU ops are kept off for every HIP translation unit
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
-# The two sources whose loads into LDS list M0 as clobbered (ld_lds_b128 in csrc/mx_tile.hpp, MXW_DMA in csrc/mx_wide.hpp,
-# the like in csrc/router_topk.hip) draw one inline-asm diagnostic per such load, thousands of times; every other translation
+# The sources whose loads into LDS list M0 as clobbered (ld_lds_b128 in csrc/mx_tile.hpp, MXW_DMA in csrc/mx_wide.hpp,
+# the like in csrc/router_topk.hip and csrc/grouped_tile.hip) draw one inline-asm diagnostic per such load, thousands of times; every other translation
 # unit keeps the diagnostic on
 MX_FLAGS = ["-Wno-inline-asm"]
 M0_CLOBBER_SOURCES = ("bwmm_mx.hip", "router_topk.hip")
@@ -128,6 +130,8 @@ def build(verbose=True, jobs=None):
         units.append((os.path.join(OBJ_DIR, f"bwmm_mx_s{stage}_f{fmt}_t{ktail}.o"),
                       [*MX_FLAGS, f"-DMX_INST_STAGE={stage}", f"-DMX_INST_WFMT={fmt}", f"-DMX_INST_KTAIL={ktail}"],
                       os.path.join(CSRC, "bwmm_mx.hip")))
+    for t, name in GG_TYPES.items():
+        units.append((os.path.join(OBJ_DIR, f"grouped_tile_{name}.o"), [*MX_FLAGS, f"-DGG_TYPE={t}"], os.path.join(CSRC, "grouped_tile.hip")))
     for s in SOURCES:
         units.append((os.path.join(OBJ_DIR, s.replace(".hip", ".o")), MX_FLAGS if s in M0_CLOBBER_SOURCES else [],
                       os.path.join(CSRC, s)))

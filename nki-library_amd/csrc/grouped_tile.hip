@@ -1,0 +1,473 @@
+// Tiles of products of ragged groups of rows, for one element type per translation unit (GG_TYPE: GG_BF16, GG_FP16, GG_INT8).
+//
+// A workgroup walks over tiles of BM x BN of the result.  A step takes 128 bytes along the terms from both operands: 64 terms of 16
+// bits or 128 of 8, two MFMAs deep.  Either operand lies in memory along its terms ("rows": a piece of 16 bytes is a lane's
+// operand as it is) or across them ("columns": a piece is 8 neighbouring columns of one term), and stays so in LDS, where the transposing read
+// (ds_read_b64_tr_b16) hands a lane the terms of its column.  So weights [E, K, N] are multiplied as they are, and their gradient, whose
+// terms are rows, takes both operands across.
+//   rows:    LDS row of 128 bytes per row; piece j of row r in place j ^ (r & 7)
+//   columns: LDS row of BN columns per term; piece j of term k in place j ^ f(k), f(k) = 2 (k & 3) + 8 ((k >> 3) & 1): the 16 lanes of
+//            a transposing read fetch 32 bytes from each of 4 terms, two such groups at a time terms 8 apart, all in other banks.
+// DMA: operands go global -> LDS without a register (rows aligned to 16 bytes); otherwise through registers, element by element
+// where a piece passes a row's end.  Two stages; a step's second half of fragments is read under the MFMAs of its first, the next
+// step's first half under those of its second; the one barrier of a step stands between them: all have read the step's stage, which then
+// takes the step after the next, and the next step's has landed.
+// The matrix is the MFMA's first operand, so that a lane holds four neighbouring columns of one row; rows go out through LDS in whole
+// 128-byte lines.
+#include <type_traits>
+
+#include "grouped_gemm.hpp"
+
+namespace moe {
+namespace {
+
+constexpr int TYPE = GG_TYPE;
+constexpr int ES = TYPE == GG_INT8 ? 1 : 2;
+constexpr int STEP = 128 / ES;  // terms of a step
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef uint32_t bytes16 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t words4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t lds_byte;
+using acc_t = std::conditional_t<TYPE == GG_INT8, v4i, v4f>;
+
+__device__ __forceinline__ acc_t mfma(const v4i& w, const v4i& x, const acc_t& c) {
+  if constexpr (TYPE == GG_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), c, 0, 0, 0);
+  else if constexpr (TYPE == GG_FP16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, x), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uni64(int64_t v) {
+  return ((int64_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v);
+}
+
+// Raw buffer over `bytes` (any number; offsets of a step stay below 2^31) from p on: what lies outside reads as zeros.
+__device__ __forceinline__ v4i buffer_of(const uint8_t* p, int64_t bytes) {
+  const uint64_t addr = (uint64_t)p;
+  const uint32_t n = bytes <= 0 ? 0u : bytes > 0x7ffffff0 ? 0x7ffffff0u : (uint32_t)bytes;
+  v4i d;
+  d[0] = uni((int)(uint32_t)addr);
+  d[1] = uni((int)(uint32_t)(addr >> 32)) & 0xffff;
+  d[2] = uni((int)n);
+  d[3] = 0x00020000;
+  return d;
+}
+constexpr uint32_t NOWHERE = 0x80000000u;  // or-ed to an offset: outside of every buffer
+// 16 bytes per lane to lds + 16 * lane.  (The wait states: a scalar operand may have been written by a vector instruction just before,
+// which the compiler does not see here.  It keeps nothing in M0 between instructions of its own.)
+__device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t off, const v4i& buf) {
+  asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(off), "s"(buf) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+__device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ int spread(int k) { return 2 * (k & 3) + 8 * ((k >> 3) & 1); }
+
+struct Tile {
+  const uint8_t* a;
+  const uint8_t* b;
+  int64_t a_bytes, b_bytes;  // from there to the end of what may be read
+  uint8_t* out;
+  int steps, rows, cols;  // rows and columns of the result that the tile holds
+  int64_t row0;           // GG_ROWS: first row
+  int64_t n0;
+  int expert;
+};
+
+// One operand's way into LDS.  ROWS_: lies along its terms.  BR: rows (columns) of a tile.
+template <bool ROWS_, int BR, int THREADS, bool DMA>
+struct Feed {
+  static constexpr int BYTES = BR * 128;
+  static constexpr int PITCH = ROWS_ ? 128 : BR * ES;  // of an LDS row
+  static constexpr int PPR = PITCH / 16;               // pieces of one
+  static constexpr int N = BYTES / 16 / THREADS;       // pieces of a thread
+  static constexpr int RPT = THREADS / PPR;            // rows between two pieces of a thread
+  static_assert(THREADS % PPR == 0 && RPT % 16 == 0, "a thread's pieces lie alike in all of its rows");
+  uint32_t off;  // of the thread's first piece; piece i lies i * RPT rows behind it
+  uint4 held[DMA ? 1 : N];
+
+  static __device__ __forceinline__ int row() { return threadIdx.x / PPR; }
+  static __device__ __forceinline__ int place() { return threadIdx.x % PPR; }
+  static __device__ __forceinline__ int swizzled() { return place() ^ (ROWS_ ? row() & 7 : spread(row())); }
+  __device__ __forceinline__ void begin(int pitch) { off = (uint32_t)(row() * pitch + (DMA ? swizzled() : place()) * 16); }
+  // Loads of step `step` into the stage at lds (DMA).  left: bytes of a row's terms from this step on (ROWS_).
+  __device__ __forceinline__ void load(uint32_t lds, const uint8_t* p, int64_t bytes, int pitch, int step, int left) {
+    const int64_t skip = ROWS_ ? (int64_t)step * 128 : (int64_t)step * STEP * pitch;
+    const uint32_t o = ROWS_ && swizzled() * 16 >= left ? NOWHERE : off;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t at = skip + (int64_t)i * RPT * pitch;
+      load_to_lds(uni(lds + (i * THREADS + (threadIdx.x & ~63)) * 16), o, buffer_of(p + at, bytes - at));
+    }
+  }
+  // Through registers: rows r < rows_left are read, terms_left bytes (ROWS_) or terms from this step on, cols_left bytes of a row.
+  __device__ __forceinline__ void fetch(const uint8_t* p, int pitch, int step, int rows_left, int terms_left, int cols_left) {
+    const int c = place() * 16;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = row() + i * RPT;
+      const uint8_t* src = p + (ROWS_ ? (int64_t)step * 128 : (int64_t)step * STEP * pitch) + (int64_t)i * RPT * pitch;
+      const int left = ROWS_ ? (r < rows_left ? terms_left - c : 0) : (r < terms_left ? cols_left - c : 0);
+      uint64_t lo = 0, hi = 0;
+      if (left > 0) {
+        // a piece that passes the row's end: the row's last 16 bytes, moved down (rows of fewer: element by element)
+        const int gone = left >= 16 ? 0 : 16 - left;
+        if (pitch >= 16) {
+          const bytes16 d = *(const bytes16*)(src + ((int)off - gone));  // (may lie ahead of src: the step before)
+          lo = (uint64_t)d[1] << 32 | d[0];
+          hi = (uint64_t)d[3] << 32 | d[2];
+          if (gone >= 8) {
+            lo = hi >> (8 * (gone - 8));
+            hi = 0;
+          } else if (gone > 0) {
+            lo = lo >> (8 * gone) | hi << (64 - 8 * gone);
+            hi >>= 8 * gone;
+          }
+        } else {
+#pragma unroll 1
+          for (int b = 0; b < left; b += ES) {
+            const uint64_t x = ES == 2 ? (uint64_t)*(const uint16_t*)(src + off + b) : (uint64_t)src[off + b];
+            if (b < 8) lo |= x << (8 * b);
+            else hi |= x << (8 * (b - 8));
+          }
+        }
+      }
+      held[i] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+    }
+  }
+  __device__ __forceinline__ void put(uint8_t* lds) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *(uint4*)(lds + (row() + i * RPT) * PITCH + swizzled() * 16) = held[i];
+  }
+};
+// ... and a wave's fragments out of it: tiles of 16 rows (columns) from `first` on.
+template <bool ROWS_, int BR, int TILES>
+struct Frags {
+  static constexpr int PITCH = ROWS_ ? 128 : BR * ES;
+  uint32_t at[ROWS_ ? 2 : TILES];
+  __device__ __forceinline__ void begin(int first) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    if constexpr (ROWS_) {
+      at[0] = (first + c) * 128 + ((g ^ (c & 7)) * 16);
+      at[1] = at[0] ^ 64;
+    } else {
+      const int k = 8 * g + (c >> 2);
+#pragma unroll
+      for (int j = 0; j < TILES; ++j)
+        at[j] = k * PITCH + (((first / 8 + 2 * j + ((c & 3) >> 1)) ^ spread(k)) * 16) + (c & 1) * 8;
+    }
+  }
+  template <int HALF>
+  __device__ __forceinline__ v4i read(const lds_byte* stage, int j) const {
+    if constexpr (ROWS_) {
+      return *(const __attribute__((address_space(3))) v4i*)(stage + at[HALF] + j * 2048);
+    } else {
+      const lds_byte* p = stage + at[j] + HALF * 32 * PITCH;
+      typedef __attribute__((address_space(3))) v4s* lds_v4s;
+      union { v4s s[2]; v4i v; } u;
+      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)p);
+      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(p + 4 * PITCH));
+      return u.v;
+    }
+  }
+};
+
+template <int BM_, int BN_, int WM_, int WN_, bool DMA_>
+struct Cfg {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = WM * WN * 64;
+  static constexpr bool DMA = DMA_;
+  static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
+  static constexpr int STAGE = (BM + BN) * 128;
+  static constexpr int EXCHANGE = 2048;  // per wave
+  static constexpr int LDS = 2 * STAGE + WM * WN * EXCHANGE;
+  static_assert(NT == 4, "a wave's 64 columns make lines of 128 bytes");
+};
+
+template <class C, int MODE, bool B_ROWS>
+__global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void grouped_kernel(const GroupedArgs p) {
+  constexpr bool A_ROWS = MODE == GG_ROWS;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int wm = wave / C::WN, wn = wave % C::WN;
+  lds_byte* const lds = (lds_byte*)smem;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
+  uint8_t* const exchange = smem + 2 * C::STAGE + wave * C::EXCHANGE;
+  int* const bound = (int*)(smem + C::LDS);
+  int* const cum = bound + p.E + 3;
+  build_group_table(p.offsets, p.E, (int)p.S, C::BM, bound, cum);
+
+  // Tiles go to the XCDs (workgroup b is on XCD b % 8) in eight runs of neighbours, so that what tiles share is in one L2: blocks of
+  // up to four row tiles of a group by all columns, row tiles fastest.
+  const int ntn = (int)((p.N + C::BN - 1) / C::BN), ntm = (int)((p.K + C::BM - 1) / C::BM);
+  const int64_t total = MODE == GG_ROWS ? (int64_t)uni(cum[p.E + 2]) * ntn : (int64_t)p.E * ntm * ntn;
+  const int64_t per = (total + 7) / 8, first = (blockIdx.x & 7) * per, end = first + per < total ? first + per : total;
+
+  auto find = [&](int64_t t) {
+    Tile q;
+    int64_t local;
+    int rt, tiles;
+    int j;
+    if (MODE == GG_ROWS) {
+      j = group_of_tile(cum, p.E, (int)(t / ntn));
+      const int c0 = uni(cum[j]);
+      tiles = uni(cum[j + 1]) - c0;
+      local = t - (int64_t)c0 * ntn;
+    } else {
+      j = (int)(t / ((int64_t)ntm * ntn)) + 1;
+      tiles = ntm;
+      local = t - (int64_t)(j - 1) * ntm * ntn;
+    }
+    const int blk = (int)(local / (4 * ntn)), in = (int)(local - (int64_t)blk * 4 * ntn);
+    const int h = tiles - blk * 4 < 4 ? tiles - blk * 4 : 4;
+    const int ct = in / h;
+    rt = blk * 4 + in - ct * h;
+    const int begin = uni(bound[j]), rows = uni(bound[j + 1]) - begin;
+    q.expert = j - 1;
+    q.n0 = (int64_t)ct * C::BN;
+    q.cols = (int)(p.N - q.n0 < C::BN ? p.N - q.n0 : C::BN);
+    const int64_t m0 = (int64_t)rt * C::BM;
+    if (MODE == GG_ROWS) {
+      q.row0 = begin + m0;
+      q.rows = (int)(rows - m0 < C::BM ? rows - m0 : C::BM);
+      const bool zero = j == 0 || j == p.E + 1;
+      q.steps = zero ? 0 : (int)((p.K * ES + 127) / 128);
+      q.a = p.a + q.row0 * p.a_pitch;
+      q.a_bytes = (p.S - q.row0) * p.a_pitch;
+      const uint8_t* b = p.b + (zero ? 0 : q.expert) * p.b_group;
+      q.b = b + (B_ROWS ? q.n0 * p.b_pitch : q.n0 * ES);
+      q.b_bytes = (B_ROWS ? (p.N - q.n0) * p.b_pitch : p.K * p.b_pitch - q.n0 * ES);
+      q.out = p.out + q.row0 * p.out_pitch;
+    } else {
+      q.row0 = m0;
+      q.rows = (int)(p.K - m0 < C::BM ? p.K - m0 : C::BM);
+      q.steps = (rows + STEP - 1) / STEP;
+      q.a = p.a + begin * p.a_pitch + m0 * ES;
+      q.a_bytes = rows * p.a_pitch - m0 * ES;
+      q.b = p.b + begin * p.b_pitch + q.n0 * ES;
+      q.b_bytes = rows * p.b_pitch - q.n0 * ES;
+      q.out = p.out + ((int64_t)q.expert * p.K + m0) * p.out_pitch;
+    }
+    return q;
+  };
+
+  Feed<A_ROWS, C::BM, C::THREADS, C::DMA> fa;
+  Feed<B_ROWS, C::BN, C::THREADS, C::DMA> fb;
+  Frags<A_ROWS, C::BM, C::MT> ra;
+  Frags<B_ROWS, C::BN, C::NT> rb;
+  fa.begin((int)p.a_pitch);
+  fb.begin((int)p.b_pitch);
+  ra.begin(wm * C::MT * 16);
+  rb.begin(wn * C::NT * 16);
+  constexpr int SA = C::BM * 128;
+
+  for (int64_t t = first + (blockIdx.x >> 3); t < end; t += gridDim.x >> 3) {
+    const Tile q = find(t);
+    acc_t acc[C::MT][C::NT];
+#pragma unroll
+    for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+      for (int n = 0; n < C::NT; ++n) acc[m][n] = acc_t{0, 0, 0, 0};
+
+    // terms of the tile (DMA, GG_CONTRACT: the group's rows end the buffers)
+    const int terms = MODE == GG_ROWS ? (int)p.K : uni(bound[q.expert + 2]) - uni(bound[q.expert + 1]);
+    const int pa = (int)p.a_pitch, pb = (int)p.b_pitch;
+    auto load = [&](int step) {
+      const uint32_t st = lds0 + (step & 1) * C::STAGE;
+      const bool in = step < q.steps;
+      const int left = (terms - step * STEP) * ES;
+      fa.load(st, q.a, in ? q.a_bytes : 0, pa, step, left);
+      fb.load(st + SA, q.b, in ? q.b_bytes : 0, pb, step, left);
+    };
+    auto fetch = [&](int step) {
+      const int left = terms - step * STEP;  // (none from the last step on)
+      fa.fetch(q.a, pa, step, q.rows, A_ROWS ? left * ES : left, q.rows * ES);
+      fb.fetch(q.b, pb, step, q.cols, B_ROWS ? left * ES : left, q.cols * ES);
+    };
+    auto put = [&](int step) {
+      uint8_t* st = smem + (step & 1) * C::STAGE;
+      fa.put(st);
+      fb.put(st + SA);
+    };
+    if (q.steps > 0) {
+      barrier();  // (the tile before has been read)
+      if constexpr (C::DMA) {
+        load(0);
+        load(1);
+        wait_loads<decltype(fa)::N + decltype(fb)::N>();
+      } else {
+        fetch(0);
+        put(0);
+        fetch(1);
+        put(1);
+        fetch(2);
+      }
+      barrier();
+      // Half a step: its MFMAs, and under those of its first rows the fragments of the next half.
+      auto half = [&](auto next_half, const lds_byte* st, v4i (&a)[C::MT], v4i (&b)[C::NT], v4i (&an)[C::MT], v4i (&bn)[C::NT]) {
+        constexpr int H = decltype(next_half)::value;
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n) bn[n] = rb.template read<H>(st + SA, n);
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m) {
+          if (2 * m < C::MT) {
+            an[2 * m] = ra.template read<H>(st, 2 * m);
+            an[2 * m + 1] = ra.template read<H>(st, 2 * m + 1);
+          }
+#pragma unroll
+          for (int n = 0; n < C::NT; ++n) acc[m][n] = mfma(b[n], a[m], acc[m][n]);
+        }
+      };
+      v4i a0[C::MT], b0[C::NT], a1[C::MT], b1[C::NT];
+#pragma unroll
+      for (int n = 0; n < C::NT; ++n) b0[n] = rb.template read<0>(lds + SA, n);
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) a0[m] = ra.template read<0>(lds, m);
+      for (int ks = 0; ks < q.steps; ++ks) {
+        half(std::integral_constant<int, 1>{}, lds + (ks & 1) * C::STAGE, a0, b0, a1, b1);
+        if constexpr (C::DMA) wait_loads<0>();
+        barrier();
+        if constexpr (C::DMA) {
+          load(ks + 2);
+        } else {
+          put(ks);
+          fetch(ks + 3);
+        }
+        half(std::integral_constant<int, 0>{}, lds + ((ks + 1) & 1) * C::STAGE, a1, b1, a0, b0);
+      }
+      if constexpr (C::DMA) wait_loads<0>();
+    }
+
+    // ---- results: 16 rows of a wave at a time, by way of its 2 KB of LDS
+    const int64_t col0 = q.n0 + wn * 64;  // of the wave, in the matrix
+    const int cols = q.cols - wn * 64;    // columns that it has
+    const int oes = p.out_dtype == MOE_DT_FP32 ? 4 : 2;
+    v4f ws[C::NT], bs[C::NT];
+    if constexpr (TYPE == GG_INT8) {
+#pragma unroll
+      for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int cc = n * 16 + 4 * g + i;
+          const bool on = cc < cols && q.steps > 0;
+          ws[n][i] = on ? p.b_scale[(int64_t)q.expert * p.N + col0 + cc] : 0.f;
+          bs[n][i] = on && p.bias ? load_as_f32(p.bias, p.out_dtype, col0 + cc) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < C::MT; ++m) {
+      const int r0 = (wm * C::MT + m) * 16;  // of these 16 rows, in the tile
+      if (r0 >= q.rows || cols <= 0) continue;
+      v4f v[C::NT];
+      if constexpr (TYPE == GG_INT8) {
+        const float xs = r0 + c < q.rows && q.steps > 0 ? p.a_scale[q.row0 + r0 + c] : 0.f;
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[n][i] = (float)acc[m][n][i] * xs * ws[n][i] + bs[n][i];
+      } else {
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n) v[n] = acc[m][n];
+      }
+      auto out_rows = [&](int first_col, int per_piece) {  // 8 pieces of 16 bytes a row
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = h * 8 + (lane >> 3), piece = (lane & 7) ^ (r & 7), col = first_col + piece * per_piece;
+          const uint4 d = *(const uint4*)(exchange + r * 128 + (lane & 7) * 16);
+          if (r0 + r < q.rows && col < cols) {
+            uint8_t* o = q.out + (int64_t)(r0 + r) * p.out_pitch + (col0 + col) * oes;
+            if (C::DMA || col + per_piece <= cols) {
+              *(bytes16*)o = bytes16{d.x, d.y, d.z, d.w};
+            } else {
+              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+              if (oes == 2) {
+                for (int i = 0; i < cols - col; ++i) ((uint16_t*)o)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+              } else {
+                for (int i = 0; i < cols - col; ++i) ((uint32_t*)o)[i] = w[i];
+              }
+            }
+          }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+      };
+      if (p.out_dtype == MOE_DT_FP32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) *(v4f*)(exchange + c * 128 + (((n * 4 + g) ^ (c & 7)) * 16)) = v[2 * h + n];
+          out_rows(h * 32, 4);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n) {
+          uint2 d;
+          if (p.out_dtype == MOE_DT_BF16) {
+            d = make_uint2(pack2_bf16(v[n][0], v[n][1]), pack2_bf16(v[n][2], v[n][3]));
+          } else {
+            typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+            const v4h h = __builtin_convertvector(v[n], v4h);
+            d = __builtin_bit_cast(uint2, h);
+          }
+          *(uint2*)(exchange + c * 128 + (((n * 2 + (g >> 1)) ^ (c & 7)) * 16) + (g & 1) * 8) = d;
+        }
+        out_rows(0, 8);
+      }
+    }
+  }
+}
+
+template <class C, int MODE, bool B_ROWS>
+int launch(const GroupedArgs& p, hipStream_t s) {
+  constexpr auto kernel = grouped_kernel<C, MODE, B_ROWS>;
+  const int lds = C::LDS + (p.E + 3) * 8;
+  if (allow_lds<kernel>(160 * 1024) != hipSuccess) return MOE_E_LAUNCH;
+  const int cus = device_cus();
+  const int64_t ntn = (p.N + C::BN - 1) / C::BN, ntm = (p.K + C::BM - 1) / C::BM;
+  // tiles at most (groups without rows have none), workgroups at most as many as run at once
+  const int64_t most = MODE == GG_ROWS ? ((p.S + C::BM - 1) / C::BM + (p.S < p.E + 1 ? p.S : p.E + 1)) * ntn : p.E * ntm * ntn;
+  const int64_t at_once = (int64_t)(cus > 0 ? cus : 256) * (C::THREADS == 512 ? 1 : 2);
+  const int64_t groups = (most < at_once ? most + 7 : at_once) / 8 * 8;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(C::THREADS), lds, s, p);
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
+typedef Cfg<256, 256, 2, 4, true> Large;
+typedef Cfg<128, 128, 2, 2, true> Small;
+typedef Cfg<128, 128, 2, 2, false> Any;
+
+template <int MODE, bool B_ROWS>
+int choose(const GroupedArgs& p, hipStream_t s) {
+  const uintptr_t at = (uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.out | (uintptr_t)p.a_pitch | (uintptr_t)p.b_pitch | (uintptr_t)p.out_pitch;
+  const bool aligned = (at & 15) == 0;
+  if (!aligned) return launch<Any, MODE, B_ROWS>(p, s);
+  const int64_t rows = MODE == GG_ROWS ? p.S / p.E : p.K;
+  if (rows >= 128 && p.N >= 256) return launch<Large, MODE, B_ROWS>(p, s);
+  return launch<Small, MODE, B_ROWS>(p, s);
+}
+
+}  // namespace
+
+#if GG_TYPE == 0
+int launch_grouped_bf16(const GroupedArgs& p, int mode, hipStream_t s) {
+#elif GG_TYPE == 1
+int launch_grouped_fp16(const GroupedArgs& p, int mode, hipStream_t s) {
+#else
+int launch_grouped_int8(const GroupedArgs& p, int mode, hipStream_t s) {
+#endif
+#if GG_TYPE == 2
+  return choose<GG_ROWS, true>(p, s);
+#else
+  if (mode == GG_CONTRACT) return choose<GG_CONTRACT, false>(p, s);
+  return p.b_rows ? choose<GG_ROWS, true>(p, s) : choose<GG_ROWS, false>(p, s);
+#endif
+}
+
+}  // namespace moe

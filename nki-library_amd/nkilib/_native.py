@@ -63,6 +63,10 @@ EXPORTED_SYMBOLS = (
     "moe_dequantize_checkpoint",
     "moe_router_topk_bwd_workspace_bytes",
     "moe_router_topk_bwd",
+    "moe_expert_row_offsets",
+    "moe_grouped_matmul",
+    "moe_grouped_matmul_bwd",
+    "moe_int8_matmul",
 )
 
 
@@ -217,6 +221,12 @@ def lib():
         "moe_dequantize_checkpoint": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p],
         "moe_router_topk_bwd": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int,
                                 c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p],
+        "moe_expert_row_offsets": [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p],
+        "moe_grouped_matmul": [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p],
+        "moe_grouped_matmul_bwd": [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                   c_void_p, c_int, c_void_p],
+        "moe_int8_matmul": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                            c_int, c_void_p],
     }.items():
         getattr(L, name).restype = c_int
         getattr(L, name).argtypes = args
