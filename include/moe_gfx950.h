@@ -49,6 +49,7 @@ int moe_check_device(void);
 #define MOE_DT_FP8_E5M2 4 /* OCP e5m2 bit patterns (MXFP8 weights only)                              */
 #define MOE_DT_FP4_E2M1 5 /* OCP e2m1 (MXFP4 weights only): four 4-bit values per 2-byte x4 element   */
 #define MOE_DT_INT32 6    /* the index operators only                                                */
+#define MOE_DT_INT8 7     /* codes of moe_rmsnorm_quant_rows                                         */
 
 /* ---- RMSNorm + quantise front end -------------------------------------------------- */
 
@@ -468,6 +469,30 @@ int moe_grouped_matmul_bwd(const void* d_out, const void* x, const void* weight,
 int moe_int8_matmul(const int8_t* x, const float* x_scales, const int8_t* weight, const float* weight_scales,
                     const void* bias, const int32_t* row_offsets, int64_t S, int64_t K, int64_t N, int64_t E, void* out,
                     int out_dtype, void* stream);
+
+/* ---- norm with the residual's addition into 8-bit rows ------------------------------------------ */
+
+/* No counterpart in the reference (its row quantisation has no residual, rmsnorm_quant.py:86-92, and its fused residual add quantises
+ * to MX, rmsnorm_mx_quantize_tkg.py:29-40).  H <= 16384 (moe_dequantize_rows: < 2^24); rows < 2^31; any row length, pointers
+ * aligned to their element.
+ *
+ * moe_rmsnorm_quant_rows: s = x + residual rounded to x's type (residual NULL: s = x), written to out_residual (given with residual;
+ * may be one of the inputs); y = s / sqrt(mean(s^2) + eps) * gamma with do_norm (gamma NULL: ones), else y = s; per row
+ * scale = max(max|y|, 2^-100) / M and code = y * (M / max(max|y|, 2^-100)) to nearest, M = 127 (code_dtype MOE_DT_INT8) or 448
+ * (MOE_DT_FP8_E4M3).  A row whose y is not finite has the scale NaN and codes 0.
+ * moe_rmsnorm_quant_rows_bwd: gradient through the norm (the rounding to codes passes gradients on): d_y and x (the normalised
+ * stream s) [rows, H] of one type -> d_x (+ d_residual unless NULL) of that type, the gradient of x and of residual alike, and d_gamma
+ * (NULL: not asked for) of gamma's type.  workspace (with d_gamma): moe_rmsnorm_quant_rows_bwd_workspace_bytes, 4-byte aligned.
+ * moe_dequantize_rows: code * scale of its row. */
+int moe_rmsnorm_quant_rows(const void* x, int dtype, const void* residual, const void* gamma, int gamma_dtype, int do_norm,
+                           double eps, int64_t rows, int64_t H, int code_dtype, void* codes, float* scales,
+                           void* out_residual, void* stream);
+size_t moe_rmsnorm_quant_rows_bwd_workspace_bytes(int64_t rows, int64_t H);
+int moe_rmsnorm_quant_rows_bwd(const void* d_y, const void* x, int dtype, const void* gamma, int gamma_dtype,
+                               const void* d_residual, double eps, int64_t rows, int64_t H, void* d_x, void* d_gamma,
+                               void* workspace, size_t workspace_bytes, void* stream);
+int moe_dequantize_rows(const void* codes, int code_dtype, const float* scales, int64_t rows, int64_t H, void* out,
+                        int dtype, void* stream);
 
 #ifdef __cplusplus
 }

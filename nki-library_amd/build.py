@@ -21,7 +21,7 @@ OBJ_DIR = os.path.join(HERE, "build")
 OUT_DIR = os.path.join(HERE, "nkilib", "_lib")
 OUT = os.path.join(OUT_DIR, "libmoe_gfx950.so")
 SOURCES = ["rmsnorm_quant.hip", "build_blocks.hip", "combine.hip", "bwmm.hip", "bwmm_mx.hip", "bwmm_rows.hip", "router_topk.hip", "index_ops.hip", "token_permute.hip",
-           "glu_checkpoint.hip", "router_bwd.hip", "grouped_gemm.hip", "capi.hip"]
+           "glu_checkpoint.hip", "router_bwd.hip", "grouped_gemm.hip", "rmsnorm_rows.hip", "capi.hip"]
 # element types of the tiles of the grouped products, one translation unit each; types as GG_* in csrc/grouped_gemm.hpp
 GG_TYPES = {0: "bf16", 1: "fp16", 2: "int8"}
 # (stage, weight format, K that ends inside a slice) instances of the large-tile MX GEMM; formats as MX_WFMT_* in csrc/bwmm.hpp

@@ -8,7 +8,7 @@ Loading is lazy and loud: if the shared library has not been built
 import contextlib
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
 
@@ -17,7 +17,7 @@ from .core.utils.kernel_assert import kernel_assert
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libmoe_gfx950.so")
 
 # element types (MOE_DT_*)
-DT_BF16, DT_FP16, DT_FP32, DT_FP8, DT_FP8_E5M2, DT_FP4_E2M1, DT_INT32 = 0, 1, 2, 3, 4, 5, 6
+DT_BF16, DT_FP16, DT_FP32, DT_FP8, DT_FP8_E5M2, DT_FP4_E2M1, DT_INT32, DT_INT8 = 0, 1, 2, 3, 4, 5, 6, 7
 # MOE_KIND_*
 KIND_BF16, KIND_FP8_ROW, KIND_MXFP8 = 0, 1, 2
 # MOE_MX_LAYOUT_*
@@ -67,6 +67,10 @@ EXPORTED_SYMBOLS = (
     "moe_grouped_matmul",
     "moe_grouped_matmul_bwd",
     "moe_int8_matmul",
+    "moe_rmsnorm_quant_rows",
+    "moe_rmsnorm_quant_rows_bwd_workspace_bytes",
+    "moe_rmsnorm_quant_rows_bwd",
+    "moe_dequantize_rows",
 )
 
 
@@ -227,11 +231,18 @@ def lib():
                                    c_void_p, c_int, c_void_p],
         "moe_int8_matmul": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
                             c_int, c_void_p],
+        "moe_rmsnorm_quant_rows": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_double, c_int64, c_int64, c_int, c_void_p,
+                                   c_void_p, c_void_p, c_void_p],
+        "moe_rmsnorm_quant_rows_bwd": [c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_double, c_int64, c_int64, c_void_p,
+                                       c_void_p, c_void_p, c_size_t, c_void_p],
+        "moe_dequantize_rows": [c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p],
     }.items():
         getattr(L, name).restype = c_int
         getattr(L, name).argtypes = args
     L.moe_router_topk_bwd_workspace_bytes.restype = c_size_t
     L.moe_router_topk_bwd_workspace_bytes.argtypes = [c_int64, c_int64, c_int64]
+    L.moe_rmsnorm_quant_rows_bwd_workspace_bytes.restype = c_size_t
+    L.moe_rmsnorm_quant_rows_bwd_workspace_bytes.argtypes = [c_int64, c_int64]
     _lib = L
     return L
 

@@ -67,3 +67,36 @@ def test_host_tensors_are_refused():
                  lambda: int8_matmul(q, f, q, f), lambda: grouped_int8_matmul(q, f, w.to(torch.int8), f, o)):
         with pytest.raises(NativeLibraryError, match="no CPU path"):
             call()
+
+
+def test_norm_refusals(L):
+    def fwd(x=P, dt=0, r=None, g=P, gd=0, norm=1, eps=1e-6, rows=0, H=64, cd=7, c=P, s=P, o=None):
+        return L.moe_rmsnorm_quant_rows(x, dt, r, g, gd, norm, eps, rows, H, cd, c, s, o, None)
+
+    assert fwd() == 0 and fwd(cd=3, r=P, o=P, g=None) == 0
+    for name in ("x", "c", "s"):
+        assert fwd(**{name: None}) == BAD_ARG, name
+    assert fwd(dt=3) == BAD_ARG and fwd(gd=7) == BAD_ARG and fwd(cd=4) == BAD_ARG and fwd(rows=-1) == BAD_ARG
+    assert fwd(r=P) == BAD_ARG and fwd(o=P) == BAD_ARG and fwd(eps=-1.0) == BAD_ARG and fwd(eps=float("nan")) == BAD_ARG
+    assert fwd(H=0) == BAD_SHAPE and fwd(H=16385) == BAD_SHAPE and fwd(rows=2**31) == BAD_SHAPE
+
+    need = L.moe_rmsnorm_quant_rows_bwd_workspace_bytes
+    assert need(1, 64) == 256 and need(5000, 100) == 1024 * 400 and need(0, 64) == 0 and need(4, 16385) == 0 and need(4, 0) == 0
+
+    def bwd(d=P, x=P, dt=0, g=P, gd=0, r=None, eps=1e-6, rows=4, H=64, dx=P, dg=P, ws=P, n=4 * 256):
+        return L.moe_rmsnorm_quant_rows_bwd(d, x, dt, g, gd, r, eps, rows, H, dx, dg, ws, n, None)
+
+    for name in ("d", "x", "dx", "g"):
+        assert bwd(**{name: None}) == BAD_ARG, name
+    assert bwd(dt=7) == BAD_ARG and bwd(gd=3) == BAD_ARG and bwd(eps=-1.0) == BAD_ARG and bwd(rows=-1) == BAD_ARG
+    assert bwd(rows=0) == BAD_SHAPE and bwd(H=0) == BAD_SHAPE and bwd(H=16385) == BAD_SHAPE
+    assert bwd(ws=None) == -3 and bwd(n=1023) == -3 and bwd(ws=ctypes.c_void_p(4098)) == BAD_ARG
+
+    def deq(c=P, cd=7, s=P, rows=0, H=64, o=P, dt=0):
+        return L.moe_dequantize_rows(c, cd, s, rows, H, o, dt, None)
+
+    assert deq() == 0 and deq(cd=3) == 0
+    for name in ("c", "s", "o"):
+        assert deq(**{name: None}) == BAD_ARG, name
+    assert deq(cd=4) == BAD_ARG and deq(dt=3) == BAD_ARG and deq(rows=-1) == BAD_ARG
+    assert deq(H=0) == BAD_SHAPE and deq(H=2**24) == BAD_SHAPE and deq(rows=2**31) == BAD_SHAPE
