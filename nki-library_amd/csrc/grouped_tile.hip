@@ -21,6 +21,9 @@
 namespace moe {
 namespace {
 
+#ifndef GG_ROWS_OF_LOADS
+#define GG_ROWS_OF_LOADS 8
+#endif
 constexpr int TYPE = GG_TYPE;
 constexpr int ES = TYPE == GG_INT8 ? 1 : 2;
 constexpr int STEP = 128 / ES;  // terms of a step
@@ -46,7 +49,8 @@ __device__ __forceinline__ int64_t uni64(int64_t v) {
 // Raw buffer over `bytes` (any number; offsets of a step stay below 2^31) from p on: what lies outside reads as zeros.
 __device__ __forceinline__ v4i buffer_of(const uint8_t* p, int64_t bytes) {
   const uint64_t addr = (uint64_t)p;
-  const uint32_t n = bytes <= 0 ? 0u : bytes > 0x7ffffff0 ? 0x7ffffff0u : (uint32_t)bytes;
+  const int64_t least = bytes > 0 ? bytes : 0;
+  const uint32_t n = least > 0x7ffffff0 ? 0x7ffffff0u : (uint32_t)least;
   v4i d;
   d[0] = uni((int)(uint32_t)addr);
   d[1] = uni((int)(uint32_t)(addr >> 32)) & 0xffff;
@@ -54,7 +58,7 @@ __device__ __forceinline__ v4i buffer_of(const uint8_t* p, int64_t bytes) {
   d[3] = 0x00020000;
   return d;
 }
-constexpr uint32_t NOWHERE = 0x80000000u;  // or-ed to an offset: outside of every buffer
+constexpr uint32_t NOWHERE = 0x80000000u;  // an offset outside of every buffer, as are those of the rows behind it (all below 2^31 apart)
 // 16 bytes per lane to lds + 16 * lane.  (The wait states: a scalar operand may have been written by a vector instruction just before,
 // which the compiler does not see here.  It keeps nothing in M0 between instructions of its own.)
 __device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t off, const v4i& buf) {
@@ -87,7 +91,9 @@ struct Feed {
   static constexpr int PPR = PITCH / 16;               // pieces of one
   static constexpr int N = BYTES / 16 / THREADS;       // pieces of a thread
   static constexpr int RPT = THREADS / PPR;            // rows between two pieces of a thread
-  static_assert(THREADS % PPR == 0 && RPT % 16 == 0, "a thread's pieces lie alike in all of its rows");
+  // a thread's pieces lie alike in all of its rows, or, where these are 8 apart, in every other one
+  static constexpr int ALIKE = !ROWS_ && RPT % 16 != 0 ? 2 : 1;
+  static_assert(THREADS % PPR == 0 && RPT % (16 / ALIKE) == 0 && (DMA || ALIKE == 1), "the places of a thread's pieces");
   uint32_t off;  // of the thread's first piece; piece i lies i * RPT rows behind it
   uint4 held[DMA ? 1 : N];
 
@@ -95,16 +101,23 @@ struct Feed {
   static __device__ __forceinline__ int place() { return threadIdx.x % PPR; }
   static __device__ __forceinline__ int swizzled() { return place() ^ (ROWS_ ? row() & 7 : spread(row())); }
   __device__ __forceinline__ void begin(int pitch) { off = (uint32_t)(row() * pitch + (DMA ? swizzled() : place()) * 16); }
-  // Loads of step `step` into the stage at lds (DMA).  left: bytes of a row's terms from this step on (ROWS_).
-  __device__ __forceinline__ void load(uint32_t lds, const uint8_t* p, int64_t bytes, int pitch, int step, int left) {
+  // DMA: what the loads of a step need, and the loads one by one, into the stage at lds.  left: bytes of a row's terms from this step
+  // on (ROWS_).
+  struct Step {
+    v4i buf;
+    uint32_t o[ALIKE], leap, lds;
+  };
+  __device__ __forceinline__ Step step_of(uint32_t lds, const uint8_t* p, int64_t bytes, int pitch, int step, int left) const {
     const int64_t skip = ROWS_ ? (int64_t)step * 128 : (int64_t)step * STEP * pitch;
-    const uint32_t o = ROWS_ && swizzled() * 16 >= left ? NOWHERE : off;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int64_t at = skip + (int64_t)i * RPT * pitch;
-      load_to_lds(uni(lds + (i * THREADS + (threadIdx.x & ~63)) * 16), o, buffer_of(p + at, bytes - at));
-    }
+    Step q;
+    q.buf = buffer_of(p + skip, bytes - skip);
+    q.o[0] = ROWS_ && swizzled() * 16 >= left ? NOWHERE : off;
+    if constexpr (ALIKE == 2) q.o[1] = off + ((swizzled() ^ 8) - swizzled()) * 16;
+    q.leap = (uint32_t)(RPT * pitch);
+    q.lds = uni(lds + (threadIdx.x & ~63) * 16);
+    return q;
   }
+  static __device__ __forceinline__ void load(const Step& q, int i) { load_to_lds(q.lds + i * THREADS * 16, q.o[i % ALIKE] + i * q.leap, q.buf); }
   // Through registers: rows r < rows_left are read, terms_left bytes (ROWS_) or terms from this step on, cols_left bytes of a row.
   __device__ __forceinline__ void fetch(const uint8_t* p, int pitch, int step, int rows_left, int terms_left, int cols_left) {
     const int c = place() * 16;
@@ -177,19 +190,20 @@ struct Frags {
   }
 };
 
-template <int BM_, int BN_, int WM_, int WN_, bool DMA_>
+template <int BM_, int BN_, int WM_, int WN_, bool DMA_, int PER_CU_>
 struct Cfg {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = WM * WN * 64;
   static constexpr bool DMA = DMA_;
+  static constexpr int PER_CU = PER_CU_;  // workgroups of a CU
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
   static constexpr int STAGE = (BM + BN) * 128;
   static constexpr int EXCHANGE = 2048;  // per wave
   static constexpr int LDS = 2 * STAGE + WM * WN * EXCHANGE;
-  static_assert(NT == 4, "a wave's 64 columns make lines of 128 bytes");
+  static_assert(NT % 4 == 0, "64 columns make lines of 128 bytes");
 };
 
 template <class C, int MODE, bool B_ROWS>
-__global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void grouped_kernel(const GroupedArgs p) {
+__global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::PER_CU * C::THREADS / 256, C::PER_CU * C::THREADS / 256))) void grouped_kernel(const GroupedArgs p) {
   constexpr bool A_ROWS = MODE == GG_ROWS;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), c = lane & 15, g = lane >> 4;
@@ -276,12 +290,26 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
     // terms of the tile (DMA, GG_CONTRACT: the group's rows end the buffers)
     const int terms = MODE == GG_ROWS ? (int)p.K : uni(bound[q.expert + 2]) - uni(bound[q.expert + 1]);
     const int pa = (int)p.a_pitch, pb = (int)p.b_pitch;
-    auto load = [&](int step) {
+    // DMA: the loads of a step, A's and B's; beyond the last step they bring zeros
+    typename decltype(fa)::Step sa;
+    typename decltype(fb)::Step sb;
+    auto prepare = [&](int step) {
       const uint32_t st = lds0 + (step & 1) * C::STAGE;
       const bool in = step < q.steps;
       const int left = (terms - step * STEP) * ES;
-      fa.load(st, q.a, in ? q.a_bytes : 0, pa, step, left);
-      fb.load(st + SA, q.b, in ? q.b_bytes : 0, pb, step, left);
+      sa = fa.step_of(st, q.a, in ? q.a_bytes : 0, pa, step, left);
+      sb = fb.step_of(st + SA, q.b, in ? q.b_bytes : 0, pb, step, left);
+    };
+    constexpr int LROWS = C::MT < GG_ROWS_OF_LOADS ? C::MT : GG_ROWS_OF_LOADS;  // row tiles under whose MFMAs the loads of a step go out
+    constexpr int LA = decltype(fa)::N, LOADS = LA + decltype(fb)::N;
+    auto load = [&](int i) {
+      if (i < LA) fa.load(sa, i);
+      else fb.load(sb, i - LA);
+    };
+    auto load_step = [&](int step) {
+      prepare(step);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) load(i);
     };
     auto fetch = [&](int step) {
       const int left = terms - step * STEP;  // (none from the last step on)
@@ -296,9 +324,9 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
     if (q.steps > 0) {
       barrier();  // (the tile before has been read)
       if constexpr (C::DMA) {
-        load(0);
-        load(1);
-        wait_loads<decltype(fa)::N + decltype(fb)::N>();
+        load_step(0);
+        load_step(1);
+        wait_loads<LOADS>();
       } else {
         fetch(0);
         put(0);
@@ -307,19 +335,24 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
         fetch(2);
       }
       barrier();
-      // Half a step: its MFMAs, and under those of its first rows the fragments of the next half.
-      auto half = [&](auto next_half, const lds_byte* st, v4i (&a)[C::MT], v4i (&b)[C::NT], v4i (&an)[C::MT], v4i (&bn)[C::NT]) {
+      // Half a step: its MFMAs, and under those of its first rows the fragments of the next half.  (The order is pinned: left to
+      // itself the compiler moves every read to where its value is used and waits for it there.)
+      auto half = [&](auto next_half, const lds_byte* st, v4i (&a)[C::MT], v4i (&b)[C::NT], v4i (&an)[C::MT], v4i (&bn)[C::NT], auto&& more) {
         constexpr int H = decltype(next_half)::value;
 #pragma unroll
-        for (int n = 0; n < C::NT; ++n) bn[n] = rb.template read<H>(st + SA, n);
-#pragma unroll
         for (int m = 0; m < C::MT; ++m) {
-          if (2 * m < C::MT) {
+          constexpr int R = C::MT / 2;  // rows under which they are read
+          if (m < R) {
+#pragma unroll
+            for (int n = m * C::NT / R; n < (m + 1) * C::NT / R; ++n) bn[n] = rb.template read<H>(st + SA, n);
             an[2 * m] = ra.template read<H>(st, 2 * m);
             an[2 * m + 1] = ra.template read<H>(st, 2 * m + 1);
           }
+          more(m);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int n = 0; n < C::NT; ++n) acc[m][n] = mfma(b[n], a[m], acc[m][n]);
+          __builtin_amdgcn_sched_barrier(0);
         }
       };
       v4i a0[C::MT], b0[C::NT], a1[C::MT], b1[C::NT];
@@ -328,96 +361,103 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
       for (int m = 0; m < C::MT; ++m) a0[m] = ra.template read<0>(lds, m);
       for (int ks = 0; ks < q.steps; ++ks) {
-        half(std::integral_constant<int, 1>{}, lds + (ks & 1) * C::STAGE, a0, b0, a1, b1);
+        if constexpr (C::DMA) prepare(ks + 2);
+        half(std::integral_constant<int, 1>{}, lds + (ks & 1) * C::STAGE, a0, b0, a1, b1, [](int) {});
         if constexpr (C::DMA) wait_loads<0>();
         barrier();
-        if constexpr (C::DMA) {
-          load(ks + 2);
-        } else {
+        if constexpr (!C::DMA) {
           put(ks);
           fetch(ks + 3);
         }
-        half(std::integral_constant<int, 0>{}, lds + ((ks + 1) & 1) * C::STAGE, a1, b1, a0, b0);
+        half(std::integral_constant<int, 0>{}, lds + ((ks + 1) & 1) * C::STAGE, a1, b1, a0, b0, [&](int m) {
+          if constexpr (C::DMA) {
+#pragma unroll
+            for (int i = m * LOADS / LROWS; i < (m + 1) * LOADS / LROWS && i < LOADS; ++i) load(i);
+          }
+        });
       }
       if constexpr (C::DMA) wait_loads<0>();
     }
 
     // ---- results: 16 rows of a wave at a time, by way of its 2 KB of LDS
-    const int64_t col0 = q.n0 + wn * 64;  // of the wave, in the matrix
-    const int cols = q.cols - wn * 64;    // columns that it has
     const int oes = p.out_dtype == MOE_DT_FP32 ? 4 : 2;
-    v4f ws[C::NT], bs[C::NT];
-    if constexpr (TYPE == GG_INT8) {
 #pragma unroll
-      for (int n = 0; n < C::NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int cc = n * 16 + 4 * g + i;
-          const bool on = cc < cols && q.steps > 0;
-          ws[n][i] = on ? p.b_scale[(int64_t)q.expert * p.N + col0 + cc] : 0.f;
-          bs[n][i] = on && p.bias ? load_as_f32(p.bias, p.out_dtype, col0 + cc) : 0.f;
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < C::MT; ++m) {
-      const int r0 = (wm * C::MT + m) * 16;  // of these 16 rows, in the tile
-      if (r0 >= q.rows || cols <= 0) continue;
-      v4f v[C::NT];
+    for (int n4 = 0; n4 < C::NT; n4 += 4) {
+      const int64_t col0 = q.n0 + (wn * C::NT + n4) * 16;  // of these 64 columns, in the matrix
+      const int cols = q.cols - (wn * C::NT + n4) * 16;    // that there are
+      v4f ws[4], bs[4];
       if constexpr (TYPE == GG_INT8) {
-        const float xs = r0 + c < q.rows && q.steps > 0 ? p.a_scale[q.row0 + r0 + c] : 0.f;
 #pragma unroll
-        for (int n = 0; n < C::NT; ++n)
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[n][i] = (float)acc[m][n][i] * xs * ws[n][i] + bs[n][i];
-      } else {
-#pragma unroll
-        for (int n = 0; n < C::NT; ++n) v[n] = acc[m][n];
+          for (int i = 0; i < 4; ++i) {
+            const int cc = n * 16 + 4 * g + i;
+            const bool on = cc < cols && q.steps > 0;
+            ws[n][i] = on ? p.b_scale[(int64_t)q.expert * p.N + col0 + cc] : 0.f;
+            bs[n][i] = on && p.bias ? load_as_f32(p.bias, p.out_dtype, col0 + cc) : 0.f;
+          }
       }
-      auto out_rows = [&](int first_col, int per_piece) {  // 8 pieces of 16 bytes a row
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = h * 8 + (lane >> 3), piece = (lane & 7) ^ (r & 7), col = first_col + piece * per_piece;
-          const uint4 d = *(const uint4*)(exchange + r * 128 + (lane & 7) * 16);
-          if (r0 + r < q.rows && col < cols) {
-            uint8_t* o = q.out + (int64_t)(r0 + r) * p.out_pitch + (col0 + col) * oes;
-            if (C::DMA || col + per_piece <= cols) {
-              *(bytes16*)o = bytes16{d.x, d.y, d.z, d.w};
-            } else {
-              const uint32_t w[4] = {d.x, d.y, d.z, d.w};
-              if (oes == 2) {
-                for (int i = 0; i < cols - col; ++i) ((uint16_t*)o)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      for (int m = 0; m < C::MT; ++m) {
+        const int r0 = (wm * C::MT + m) * 16;  // of these 16 rows, in the tile
+        if (r0 >= q.rows || cols <= 0) continue;
+        v4f v[4];
+        if constexpr (TYPE == GG_INT8) {
+          const float xs = r0 + c < q.rows && q.steps > 0 ? p.a_scale[q.row0 + r0 + c] : 0.f;
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[n][i] = (float)acc[m][n4 + n][i] * xs * ws[n][i] + bs[n][i];
+        } else {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) v[n] = acc[m][n4 + n];
+        }
+        auto out_rows = [&](int first_col, int per_piece) {  // 8 pieces of 16 bytes a row
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = h * 8 + (lane >> 3), piece = (lane & 7) ^ (r & 7), col = first_col + piece * per_piece;
+            const uint4 d = *(const uint4*)(exchange + r * 128 + (lane & 7) * 16);
+            if (r0 + r < q.rows && col < cols) {
+              uint8_t* o = q.out + (int64_t)(r0 + r) * p.out_pitch + (col0 + col) * oes;
+              if (C::DMA || col + per_piece <= cols) {
+                *(bytes16*)o = bytes16{d.x, d.y, d.z, d.w};
               } else {
-                for (int i = 0; i < cols - col; ++i) ((uint32_t*)o)[i] = w[i];
+                const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+                if (oes == 2) {
+                  for (int i = 0; i < cols - col; ++i) ((uint16_t*)o)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+                } else {
+                  for (int i = 0; i < cols - col; ++i) ((uint32_t*)o)[i] = w[i];
+                }
               }
             }
           }
-        }
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_wave_barrier();
-      };
-      if (p.out_dtype == MOE_DT_FP32) {
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_wave_barrier();
+        };
+        if (p.out_dtype == MOE_DT_FP32) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) *(v4f*)(exchange + c * 128 + (((n * 4 + g) ^ (c & 7)) * 16)) = v[2 * h + n];
-          out_rows(h * 32, 4);
-        }
-      } else {
-#pragma unroll
-        for (int n = 0; n < C::NT; ++n) {
-          uint2 d;
-          if (p.out_dtype == MOE_DT_BF16) {
-            d = make_uint2(pack2_bf16(v[n][0], v[n][1]), pack2_bf16(v[n][2], v[n][3]));
-          } else {
-            typedef _Float16 v4h __attribute__((ext_vector_type(4)));
-            const v4h h = __builtin_convertvector(v[n], v4h);
-            d = __builtin_bit_cast(uint2, h);
+            for (int n = 0; n < 2; ++n) *(v4f*)(exchange + c * 128 + (((n * 4 + g) ^ (c & 7)) * 16)) = v[2 * h + n];
+            out_rows(h * 32, 4);
           }
-          *(uint2*)(exchange + c * 128 + (((n * 2 + (g >> 1)) ^ (c & 7)) * 16) + (g & 1) * 8) = d;
+        } else {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            uint2 d;
+            if (p.out_dtype == MOE_DT_BF16) {
+              d = make_uint2(pack2_bf16(v[n][0], v[n][1]), pack2_bf16(v[n][2], v[n][3]));
+            } else {
+              typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+              const v4h h = __builtin_convertvector(v[n], v4h);
+              d = __builtin_bit_cast(uint2, h);
+            }
+            *(uint2*)(exchange + c * 128 + (((n * 2 + (g >> 1)) ^ (c & 7)) * 16) + (g & 1) * 8) = d;
+          }
+          out_rows(0, 8);
         }
-        out_rows(0, 8);
       }
     }
   }
@@ -432,16 +472,20 @@ int launch(const GroupedArgs& p, hipStream_t s) {
   const int64_t ntn = (p.N + C::BN - 1) / C::BN, ntm = (p.K + C::BM - 1) / C::BM;
   // tiles at most (groups without rows have none), workgroups at most as many as run at once
   const int64_t most = MODE == GG_ROWS ? ((p.S + C::BM - 1) / C::BM + (p.S < p.E + 1 ? p.S : p.E + 1)) * ntn : p.E * ntm * ntn;
-  const int64_t at_once = (int64_t)(cus > 0 ? cus : 256) * (C::THREADS == 512 ? 1 : 2);
+  const int64_t at_once = (int64_t)(cus > 0 ? cus : 256) * C::PER_CU;
   const int64_t groups = (most < at_once ? most + 7 : at_once) / 8 * 8;
   hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(C::THREADS), lds, s, p);
   MOE_CHECK_LAUNCH();
   return MOE_OK;
 }
 
-typedef Cfg<256, 256, 2, 4, true> Large;
-typedef Cfg<128, 128, 2, 2, true> Small;
-typedef Cfg<128, 128, 2, 2, false> Any;
+#ifdef GG_EIGHT
+typedef Cfg<256, 256, 2, 4, true, 1> Large;
+#else
+typedef Cfg<256, 256, 2, 2, true, 1> Large;
+#endif
+typedef Cfg<128, 128, 2, 2, true, 2> Small;
+typedef Cfg<128, 128, 2, 2, false, 2> Any;
 
 template <int MODE, bool B_ROWS>
 int choose(const GroupedArgs& p, hipStream_t s) {
