@@ -21,9 +21,6 @@
 namespace moe {
 namespace {
 
-#ifndef GG_ROWS_OF_LOADS
-#define GG_ROWS_OF_LOADS 8
-#endif
 constexpr int TYPE = GG_TYPE;
 constexpr int ES = TYPE == GG_INT8 ? 1 : 2;
 constexpr int STEP = 128 / ES;  // terms of a step
@@ -91,9 +88,7 @@ struct Feed {
   static constexpr int PPR = PITCH / 16;               // pieces of one
   static constexpr int N = BYTES / 16 / THREADS;       // pieces of a thread
   static constexpr int RPT = THREADS / PPR;            // rows between two pieces of a thread
-  // a thread's pieces lie alike in all of its rows, or, where these are 8 apart, in every other one
-  static constexpr int ALIKE = !ROWS_ && RPT % 16 != 0 ? 2 : 1;
-  static_assert(THREADS % PPR == 0 && RPT % (16 / ALIKE) == 0 && (DMA || ALIKE == 1), "the places of a thread's pieces");
+  static_assert(THREADS % PPR == 0 && RPT % 16 == 0, "a thread's pieces lie alike in all of its rows");
   uint32_t off;  // of the thread's first piece; piece i lies i * RPT rows behind it
   uint4 held[DMA ? 1 : N];
 
@@ -105,19 +100,18 @@ struct Feed {
   // on (ROWS_).
   struct Step {
     v4i buf;
-    uint32_t o[ALIKE], leap, lds;
+    uint32_t o, leap, lds;
   };
   __device__ __forceinline__ Step step_of(uint32_t lds, const uint8_t* p, int64_t bytes, int pitch, int step, int left) const {
     const int64_t skip = ROWS_ ? (int64_t)step * 128 : (int64_t)step * STEP * pitch;
     Step q;
     q.buf = buffer_of(p + skip, bytes - skip);
-    q.o[0] = ROWS_ && swizzled() * 16 >= left ? NOWHERE : off;
-    if constexpr (ALIKE == 2) q.o[1] = off + ((swizzled() ^ 8) - swizzled()) * 16;
+    q.o = ROWS_ && swizzled() * 16 >= left ? NOWHERE : off;
     q.leap = (uint32_t)(RPT * pitch);
     q.lds = uni(lds + (threadIdx.x & ~63) * 16);
     return q;
   }
-  static __device__ __forceinline__ void load(const Step& q, int i) { load_to_lds(q.lds + i * THREADS * 16, q.o[i % ALIKE] + i * q.leap, q.buf); }
+  static __device__ __forceinline__ void load(const Step& q, int i) { load_to_lds(q.lds + i * THREADS * 16, q.o + i * q.leap, q.buf); }
   // Through registers: rows r < rows_left are read, terms_left bytes (ROWS_) or terms from this step on, cols_left bytes of a row.
   __device__ __forceinline__ void fetch(const uint8_t* p, int pitch, int step, int rows_left, int terms_left, int cols_left) {
     const int c = place() * 16;
@@ -158,27 +152,27 @@ struct Feed {
     for (int i = 0; i < N; ++i) *(uint4*)(lds + (row() + i * RPT) * PITCH + swizzled() * 16) = held[i];
   }
 };
-// ... and a wave's fragments out of it: tiles of 16 rows (columns) from `first` on.
-template <bool ROWS_, int BR, int TILES>
+// ... and a wave's fragments out of it: tiles of 16 rows (columns), the first and every LEAP-th behind it.
+template <bool ROWS_, int BR, int TILES, int LEAP>
 struct Frags {
   static constexpr int PITCH = ROWS_ ? 128 : BR * ES;
   uint32_t at[ROWS_ ? 2 : TILES];
   __device__ __forceinline__ void begin(int first) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     if constexpr (ROWS_) {
-      at[0] = (first + c) * 128 + ((g ^ (c & 7)) * 16);
+      at[0] = (first * 16 + c) * 128 + ((g ^ (c & 7)) * 16);
       at[1] = at[0] ^ 64;
     } else {
       const int k = 8 * g + (c >> 2);
 #pragma unroll
       for (int j = 0; j < TILES; ++j)
-        at[j] = k * PITCH + (((first / 8 + 2 * j + ((c & 3) >> 1)) ^ spread(k)) * 16) + (c & 1) * 8;
+        at[j] = k * PITCH + (((2 * (first + j * LEAP) + ((c & 3) >> 1)) ^ spread(k)) * 16) + (c & 1) * 8;
     }
   }
   template <int HALF>
   __device__ __forceinline__ v4i read(const lds_byte* stage, int j) const {
     if constexpr (ROWS_) {
-      return *(const __attribute__((address_space(3))) v4i*)(stage + at[HALF] + j * 2048);
+      return *(const __attribute__((address_space(3))) v4i*)(stage + at[HALF] + j * LEAP * 2048);
     } else {
       const lds_byte* p = stage + at[j] + HALF * 32 * PITCH;
       typedef __attribute__((address_space(3))) v4s* lds_v4s;
@@ -206,7 +200,7 @@ template <class C, int MODE, bool B_ROWS>
 __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::PER_CU * C::THREADS / 256, C::PER_CU * C::THREADS / 256))) void grouped_kernel(const GroupedArgs p) {
   constexpr bool A_ROWS = MODE == GG_ROWS;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = uni(tid >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
   lds_byte* const lds = (lds_byte*)smem;
   const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
@@ -271,46 +265,58 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
 
   Feed<A_ROWS, C::BM, C::THREADS, C::DMA> fa;
   Feed<B_ROWS, C::BN, C::THREADS, C::DMA> fb;
-  Frags<A_ROWS, C::BM, C::MT> ra;
-  Frags<B_ROWS, C::BN, C::NT> rb;
+  Frags<A_ROWS, C::BM, C::MT, C::WM> ra;
+  Frags<B_ROWS, C::BN, C::NT, 1> rb;
   fa.begin((int)p.a_pitch);
   fb.begin((int)p.b_pitch);
-  ra.begin(wm * C::MT * 16);
-  rb.begin(wn * C::NT * 16);
+  ra.begin(wm);
+  rb.begin(wn * C::NT);
   constexpr int SA = C::BM * 128;
 
-  for (int64_t t = first + (blockIdx.x >> 3); t < end; t += gridDim.x >> 3) {
-    const Tile q = find(t);
+  const int pa = (int)p.a_pitch, pb = (int)p.b_pitch;
+  // terms of a tile (DMA, GG_CONTRACT: the group's rows end the buffers)
+  auto terms_of = [&](const Tile& q) { return MODE == GG_ROWS ? (int)p.K : uni(bound[q.expert + 2]) - uni(bound[q.expert + 1]); };
+  // DMA: the loads of a step, A's and B's; beyond the last step they bring zeros
+  typename decltype(fa)::Step sa;
+  typename decltype(fb)::Step sb;
+  auto prepare = [&](const Tile& q, int terms, int step) {
+    const uint32_t st = lds0 + (step & 1) * C::STAGE;
+    const bool in = step < q.steps;
+    const int left = (terms - step * STEP) * ES;
+    sa = fa.step_of(st, q.a, in ? q.a_bytes : 0, pa, step, left);
+    sb = fb.step_of(st + SA, q.b, in ? q.b_bytes : 0, pb, step, left);
+  };
+  constexpr int LA = decltype(fa)::N, LOADS = LA + decltype(fb)::N;
+  auto load = [&](int i) {
+    if (i < LA) fa.load(sa, i);
+    else fb.load(sb, i - LA);
+  };
+  auto load_two = [&](const Tile& q) {
+    if (q.steps == 0) return;
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+      prepare(q, terms_of(q), step);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) load(i);
+    }
+  };
+
+  // A tile's first two steps are requested ahead of the results of the tile before, whose stores then drain under its first steps:
+  // at least STORES of them stand behind the loads in the order in which these are waited for (stored), or nothing is counted on.
+  constexpr int STORES = 2 * C::MT;
+  bool stored = false;
+  int64_t t = first + (blockIdx.x >> 3);
+  if (t >= end) return;
+  Tile q = find(t);
+  if constexpr (C::DMA) load_two(q);
+  for (;;) {
+    const int terms = terms_of(q);
     acc_t acc[C::MT][C::NT];
 #pragma unroll
     for (int m = 0; m < C::MT; ++m)
 #pragma unroll
       for (int n = 0; n < C::NT; ++n) acc[m][n] = acc_t{0, 0, 0, 0};
 
-    // terms of the tile (DMA, GG_CONTRACT: the group's rows end the buffers)
-    const int terms = MODE == GG_ROWS ? (int)p.K : uni(bound[q.expert + 2]) - uni(bound[q.expert + 1]);
-    const int pa = (int)p.a_pitch, pb = (int)p.b_pitch;
-    // DMA: the loads of a step, A's and B's; beyond the last step they bring zeros
-    typename decltype(fa)::Step sa;
-    typename decltype(fb)::Step sb;
-    auto prepare = [&](int step) {
-      const uint32_t st = lds0 + (step & 1) * C::STAGE;
-      const bool in = step < q.steps;
-      const int left = (terms - step * STEP) * ES;
-      sa = fa.step_of(st, q.a, in ? q.a_bytes : 0, pa, step, left);
-      sb = fb.step_of(st + SA, q.b, in ? q.b_bytes : 0, pb, step, left);
-    };
-    constexpr int LROWS = C::MT < GG_ROWS_OF_LOADS ? C::MT : GG_ROWS_OF_LOADS;  // row tiles under whose MFMAs the loads of a step go out
-    constexpr int LA = decltype(fa)::N, LOADS = LA + decltype(fb)::N;
-    auto load = [&](int i) {
-      if (i < LA) fa.load(sa, i);
-      else fb.load(sb, i - LA);
-    };
-    auto load_step = [&](int step) {
-      prepare(step);
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) load(i);
-    };
     auto fetch = [&](int step) {
       const int left = terms - step * STEP;  // (none from the last step on)
       fa.fetch(q.a, pa, step, q.rows, A_ROWS ? left * ES : left, q.rows * ES);
@@ -321,13 +327,14 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
       fa.put(st);
       fb.put(st + SA);
     };
-    if (q.steps > 0) {
-      barrier();  // (the tile before has been read)
+    // The steps of a tile of which a wave has V row tiles.
+    auto multiply = [&](auto row_tiles) {
+      constexpr int V = decltype(row_tiles)::value;
       if constexpr (C::DMA) {
-        load_step(0);
-        load_step(1);
-        wait_loads<LOADS>();
+        if (stored) wait_loads<LOADS + STORES>();
+        else wait_loads<LOADS>();
       } else {
+        barrier();  // (the tile before has been read)
         fetch(0);
         put(0);
         fetch(1);
@@ -335,13 +342,12 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
         fetch(2);
       }
       barrier();
-      // Half a step: its MFMAs, and under those of its first rows the fragments of the next half.  (The order is pinned: left to
-      // itself the compiler moves every read to where its value is used and waits for it there.)
-      auto half = [&](auto next_half, const lds_byte* st, v4i (&a)[C::MT], v4i (&b)[C::NT], v4i (&an)[C::MT], v4i (&bn)[C::NT], auto&& more) {
-        constexpr int H = decltype(next_half)::value;
+      // Half a step: its MFMAs, and under those of its first rows the fragments of the next half and what `more` does.  (The order is
+      // pinned: left to itself the compiler moves every read to where its value is used and waits for it there.)
+      auto half = [&](auto next_half, const lds_byte* st, v4i (&a)[V], v4i (&b)[C::NT], v4i (&an)[V], v4i (&bn)[C::NT], auto&& more) {
+        constexpr int H = decltype(next_half)::value, R = V / 2;  // R: row tiles under which the fragments are read
 #pragma unroll
-        for (int m = 0; m < C::MT; ++m) {
-          constexpr int R = C::MT / 2;  // rows under which they are read
+        for (int m = 0; m < V; ++m) {
           if (m < R) {
 #pragma unroll
             for (int n = m * C::NT / R; n < (m + 1) * C::NT / R; ++n) bn[n] = rb.template read<H>(st + SA, n);
@@ -355,15 +361,18 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
           __builtin_amdgcn_sched_barrier(0);
         }
       };
-      v4i a0[C::MT], b0[C::NT], a1[C::MT], b1[C::NT];
+      v4i a0[V], b0[C::NT], a1[V], b1[C::NT];
 #pragma unroll
       for (int n = 0; n < C::NT; ++n) b0[n] = rb.template read<0>(lds + SA, n);
 #pragma unroll
-      for (int m = 0; m < C::MT; ++m) a0[m] = ra.template read<0>(lds, m);
+      for (int m = 0; m < V; ++m) a0[m] = ra.template read<0>(lds, m);
       for (int ks = 0; ks < q.steps; ++ks) {
-        if constexpr (C::DMA) prepare(ks + 2);
+        if constexpr (C::DMA) prepare(q, terms, ks + 2);
         half(std::integral_constant<int, 1>{}, lds + (ks & 1) * C::STAGE, a0, b0, a1, b1, [](int) {});
-        if constexpr (C::DMA) wait_loads<0>();
+        if constexpr (C::DMA) {
+          if (ks == 0 && stored) wait_loads<STORES>();
+          else wait_loads<0>();
+        }
         barrier();
         if constexpr (!C::DMA) {
           put(ks);
@@ -372,14 +381,34 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
         half(std::integral_constant<int, 0>{}, lds + ((ks + 1) & 1) * C::STAGE, a1, b1, a0, b0, [&](int m) {
           if constexpr (C::DMA) {
 #pragma unroll
-            for (int i = m * LOADS / LROWS; i < (m + 1) * LOADS / LROWS && i < LOADS; ++i) load(i);
+            for (int i = m * LOADS / V; i < (m + 1) * LOADS / V; ++i) load(i);
           }
         });
       }
       if constexpr (C::DMA) wait_loads<0>();
+      barrier();
+    };
+    if (q.steps > 0) {
+      const int v = (q.rows + 16 * C::WM - 1) / (16 * C::WM);
+      if (C::MT > 6 && v > 6) multiply(std::integral_constant<int, (C::MT > 6 ? 8 : 2)>{});
+      else if (C::MT > 4 && v > 4) multiply(std::integral_constant<int, (C::MT > 4 ? 6 : 2)>{});
+      else if (v > 2) multiply(std::integral_constant<int, 4>{});
+      else multiply(std::integral_constant<int, 2>{});
+    }
+    const bool last = t + (gridDim.x >> 3) >= end;
+    Tile following = q;
+    if (!last) {
+      t += gridDim.x >> 3;
+      following = find(t);
+      if constexpr (C::DMA) load_two(following);
     }
 
     // ---- results: 16 rows of a wave at a time, by way of its 2 KB of LDS
+    // (The lane is taken anew: what follows from it would otherwise be worked out ahead of the first tile and kept, for want of
+    // registers, in memory, whose loads wait for all that is under way.)
+    int lane = tid & 63;
+    asm volatile("" : "+v"(lane));
+    const int c = lane & 15, g = lane >> 4;
     const int oes = p.out_dtype == MOE_DT_FP32 ? 4 : 2;
 #pragma unroll
     for (int n4 = 0; n4 < C::NT; n4 += 4) {
@@ -399,7 +428,7 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
       }
 #pragma unroll
       for (int m = 0; m < C::MT; ++m) {
-        const int r0 = (wm * C::MT + m) * 16;  // of these 16 rows, in the tile
+        const int r0 = (m * C::WM + wm) * 16;  // of these 16 rows, in the tile
         if (r0 >= q.rows || cols <= 0) continue;
         v4f v[4];
         if constexpr (TYPE == GG_INT8) {
@@ -460,6 +489,9 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
         }
       }
     }
+    if (last) break;
+    stored = C::NT == 4 && q.rows == C::BM && q.cols == C::BN;
+    q = following;
   }
 }
 
@@ -479,11 +511,7 @@ int launch(const GroupedArgs& p, hipStream_t s) {
   return MOE_OK;
 }
 
-#ifdef GG_EIGHT
 typedef Cfg<256, 256, 2, 4, true, 1> Large;
-#else
-typedef Cfg<256, 256, 2, 2, true, 1> Large;
-#endif
 typedef Cfg<128, 128, 2, 2, true, 2> Small;
 typedef Cfg<128, 128, 2, 2, false, 2> Any;
 
