@@ -21,12 +21,17 @@ constexpr int NORM_MAX_H = 16384;
 constexpr float LEAST = 7.888609052210118e-31f;  // 2^-100: a row's largest value counts as no less, so that its inverse stays finite
 
 // Rows are dealt to groups of TPR threads (a wave or a workgroup); a thread holds P pieces of N neighbours, piece p from column
-// (p * TPR + lane) * N on.
+// (p * TPR + lane) * N on.  WHOLE: rows are whole pieces; a thread beyond the last one loads that and takes zeros.
 template <int DT>
 constexpr int NV = Elem<DT>::N;
 
-template <int DT>
+template <int DT, bool WHOLE>
 __device__ __forceinline__ u32x4 load_part(const uint8_t* row, int col, int H) {  // piece from col on, zeros behind the row's end
+  if constexpr (WHOLE) {
+    const u32x4 d = load_piece<DT>(row + (int64_t)(col < H ? col : H - NV<DT>) * Elem<DT>::SIZE);
+    const uint32_t keep = col < H ? ~0u : 0u;
+    return u32x4{d[0] & keep, d[1] & keep, d[2] & keep, d[3] & keep};
+  }
   if (col + NV<DT> <= H) return load_piece<DT>(row + (int64_t)col * Elem<DT>::SIZE);
   u32x4 d = {0, 0, 0, 0};
 #pragma unroll
@@ -38,50 +43,81 @@ __device__ __forceinline__ u32x4 load_part(const uint8_t* row, int col, int H) {
     }
   return d;
 }
-template <int DT>
+template <int DT, bool WHOLE>
 __device__ __forceinline__ void store_part(uint8_t* row, int col, int H, const u32x4& d) {
   if (col + NV<DT> <= H) {
     store_piece<DT>(row + (int64_t)col * Elem<DT>::SIZE, d);
     return;
   }
+  if constexpr (!WHOLE) {
 #pragma unroll
-  for (int i = 0; i < NV<DT>; ++i)
-    if (col + i < H) ((typename Elem<DT>::raw*)row)[col + i] = (typename Elem<DT>::raw)(Elem<DT>::SIZE == 4 ? d[i % 4] : d[i / 2] >> (16 * (i & 1)));
+    for (int i = 0; i < NV<DT>; ++i)
+      if (col + i < H)
+        ((typename Elem<DT>::raw*)row)[col + i] = (typename Elem<DT>::raw)(Elem<DT>::SIZE == 4 ? d[i % 4] : d[i / 2] >> (16 * (i & 1)));
+  }
 }
 
 // gamma of a piece; ones without one (zeros behind the row's end)
-template <int DT>
+template <int DT, bool WHOLE>
 __device__ __forceinline__ void load_gamma(const void* gamma, int dtype, int col, int H, float (&g)[NV<DT>]) {
-  if (gamma && dtype == DT && col + NV<DT> <= H) {
-    unpack<DT>(load_piece_kept<DT>((const uint8_t*)gamma + (int64_t)col * Elem<DT>::SIZE), g);
+  if (gamma && dtype == DT && (WHOLE || col + NV<DT> <= H)) {
+    unpack<DT>(load_piece_kept<DT>((const uint8_t*)gamma + (int64_t)(col < H ? col : 0) * Elem<DT>::SIZE), g);
     return;
   }
 #pragma unroll
   for (int i = 0; i < NV<DT>; ++i) g[i] = col + i < H ? (gamma ? load_as_f32(gamma, dtype, col + i) : 1.f) : 0.f;
 }
 
+// Sum and maximum over a wave, the same bits in all lanes: sixteen lanes by rotations (every lane adds the same pairs), then the four
+// sixteens through scalar registers.  (Shuffles go through LDS, six of them in a row were a third of a short row's time.)
+template <int N>
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xf, 0xf, true);  // row_ror:N
+}
+template <int N>
+__device__ __forceinline__ double turned(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)turned<N>((uint32_t)(b >> 32)) << 32 | turned<N>((uint32_t)b));
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double sum_of_wave(double v) {
+  v += turned<8>(v);
+  v += turned<4>(v);
+  v += turned<2>(v);
+  v += turned<1>(v);
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+__device__ __forceinline__ uint32_t max_of_wave(uint32_t v) {
+  auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  v = larger(v, turned<8>(v));
+  v = larger(v, turned<4>(v));
+  v = larger(v, turned<2>(v));
+  v = larger(v, turned<1>(v));
+  const uint32_t a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16);
+  const uint32_t c = __builtin_amdgcn_readlane((int)v, 32), d = __builtin_amdgcn_readlane((int)v, 48);
+  return larger(larger(a, b), larger(c, d));
+}
+// ... over a row.  One barrier each: `red` is a place of its own for every reduction between two others.
 template <int TPR>
 __device__ __forceinline__ double row_sum(double v, double* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  v = sum_of_wave(v);
   if constexpr (TPR == 64) return v;
-  __syncthreads();
+  const int first = threadIdx.x / TPR * (TPR / 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  double t = 0.0;
+  double t = red[first];
 #pragma unroll
-  for (int i = 0; i < TPR / 64; ++i) t += red[i];
+  for (int i = 1; i < TPR / 64; ++i) t += red[first + i];
   return t;
 }
 template <int TPR>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint32_t u = __shfl_xor(v, o, 64);
-    v = u > v ? u : v;
-  }
+  v = max_of_wave(v);
   if constexpr (TPR == 64) return v;
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   uint32_t t = red[0];
@@ -102,11 +138,12 @@ struct NormArgs {
   int H, gamma_dtype, do_norm;
 };
 
-template <int DT, int TPR, int P, bool E4M3>
+template <int DT, int TPR, int P, bool WHOLE, bool E4M3>
 __global__ __launch_bounds__(256) void norm_quant_kernel(const NormArgs a) {
   constexpr int N = NV<DT>;
   __shared__ double red_sum[4];
-  __shared__ uint32_t red_max[4];
+  __shared__ uint32_t red_max[2][4];
+  int turn = 0;
   const int lane = threadIdx.x % TPR, H = a.H;
   const int64_t row_bytes = (int64_t)H * Elem<DT>::SIZE;
   for (int64_t r = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR; r < a.rows; r += (int64_t)gridDim.x * (256 / TPR)) {
@@ -114,10 +151,10 @@ __global__ __launch_bounds__(256) void norm_quant_kernel(const NormArgs a) {
     float v[P][N];
     u32x4 d[P], e[P];
 #pragma unroll
-    for (int p = 0; p < P; ++p) d[p] = load_part<DT>(x, (p * TPR + lane) * N, H);
+    for (int p = 0; p < P; ++p) d[p] = load_part<DT, WHOLE>(x, (p * TPR + lane) * N, H);
     if (a.residual) {
 #pragma unroll
-      for (int p = 0; p < P; ++p) e[p] = load_part<DT>(a.residual + r * row_bytes, (p * TPR + lane) * N, H);
+      for (int p = 0; p < P; ++p) e[p] = load_part<DT, WHOLE>(a.residual + r * row_bytes, (p * TPR + lane) * N, H);
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -128,7 +165,7 @@ __global__ __launch_bounds__(256) void norm_quant_kernel(const NormArgs a) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[p][i] = v[p][i] + w[i];
         const u32x4 s = pack<DT>(v[p]);
-        store_part<DT>(a.out_residual + r * row_bytes, (p * TPR + lane) * N, H, s);
+        store_part<DT, WHOLE>(a.out_residual + r * row_bytes, (p * TPR + lane) * N, H, s);
         unpack<DT>(s, v[p]);
       }
     }
@@ -143,7 +180,7 @@ __global__ __launch_bounds__(256) void norm_quant_kernel(const NormArgs a) {
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         float g[N];
-        load_gamma<DT>(a.gamma, a.gamma_dtype, (p * TPR + lane) * N, H, g);
+        load_gamma<DT, WHOLE>(a.gamma, a.gamma_dtype, (p * TPR + lane) * N, H, g);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[p][i] = v[p][i] * inv * g[i];
       }
@@ -156,7 +193,8 @@ __global__ __launch_bounds__(256) void norm_quant_kernel(const NormArgs a) {
         const uint32_t b = (p * TPR + lane) * N + i < H ? __float_as_uint(v[p][i]) & 0x7fffffffu : 0u;
         most = b > most ? b : most;
       }
-    most = row_max<TPR>(most, red_max);
+    most = row_max<TPR>(most, red_max[turn]);
+    turn ^= 1;  // (without the norm the next barrier is the next row's maximum)
     const bool finite = most < 0x7f800000u;
     const float largest = fmaxf(__uint_as_float(most), LEAST);
     constexpr float M = E4M3 ? 448.0f : 127.0f;
@@ -186,7 +224,7 @@ __global__ __launch_bounds__(256) void norm_quant_kernel(const NormArgs a) {
         if constexpr (N == 4) o = c[0];
         else o = part_t{c[0], c[1]};
         __builtin_nontemporal_store(o, (part_t*)(codes + col));
-      } else {
+      } else if constexpr (!WHOLE) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
           if (col + i < H) codes[col + i] = (uint8_t)(c[i / 4] >> (8 * (i & 3)));
@@ -206,30 +244,35 @@ struct NormBwdArgs {
   double eps;
   int H, gamma_dtype;
 };
-// A workgroup takes every gridDim.x-th row; a thread has the same columns in all of them and adds up their d_gamma in registers.
-template <int DT, int P>
-__global__ __launch_bounds__(256) void norm_bwd_kernel(const NormBwdArgs a) {
+// A workgroup has SUB rows at a time, 256 threads each; a thread has the same columns in all of its rows and adds up their d_gamma in
+// registers.  The SUB sums are added in LDS, so that there are few parts to be read again.
+template <int DT, int P, int SUB, bool WHOLE>
+__global__ __launch_bounds__(SUB * 256) void norm_bwd_kernel(const NormBwdArgs a) {
   constexpr int N = NV<DT>;
-  __shared__ double red[8];
-  const int H = a.H, tid = threadIdx.x;
+  __shared__ double red[2][2][4 * SUB];
+  extern __shared__ float s_dg[];  // [H]; with SUB > 1
+  const int H = a.H, sub = threadIdx.x / 256, tid = threadIdx.x % 256;
   const int64_t row_bytes = (int64_t)H * Elem<DT>::SIZE;
   float dg[P][N], gm[P][N];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    load_gamma<DT>(a.gamma, a.gamma_dtype, (p * 256 + tid) * N, H, gm[p]);
+    load_gamma<DT, WHOLE>(a.gamma, a.gamma_dtype, (p * 256 + tid) * N, H, gm[p]);
 #pragma unroll
     for (int i = 0; i < N; ++i) dg[p][i] = 0.f;
   }
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+  int turn = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * SUB; r0 < a.rows; r0 += (int64_t)gridDim.x * SUB) {
+    const bool on = r0 + sub < a.rows;  // (the last round's threads beyond work on the last row and write nothing)
+    const int64_t r = on ? r0 + sub : a.rows - 1;
     u32x4 xs[P], ds[P], rs[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      xs[p] = load_part<DT>(a.x + r * row_bytes, (p * 256 + tid) * N, H);
-      ds[p] = load_part<DT>(a.d_y + r * row_bytes, (p * 256 + tid) * N, H);
+      xs[p] = load_part<DT, WHOLE>(a.x + r * row_bytes, (p * 256 + tid) * N, H);
+      ds[p] = load_part<DT, WHOLE>(a.d_y + r * row_bytes, (p * 256 + tid) * N, H);
     }
     if (a.d_residual) {
 #pragma unroll
-      for (int p = 0; p < P; ++p) rs[p] = load_part<DT>(a.d_residual + r * row_bytes, (p * 256 + tid) * N, H);
+      for (int p = 0; p < P; ++p) rs[p] = load_part<DT, WHOLE>(a.d_residual + r * row_bytes, (p * 256 + tid) * N, H);
     }
     double sx = 0.0, sd = 0.0;
 #pragma unroll
@@ -243,45 +286,55 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(const NormBwdArgs a) {
         sd = __builtin_fma((double)x[i], (double)(d[i] * gm[p][i]), sd);
       }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      sx += __shfl_xor(sx, o, 64);
-      sd += __shfl_xor(sd, o, 64);
-    }
-    __syncthreads();
+    sx = sum_of_wave(sx);
+    sd = sum_of_wave(sd);
     if ((tid & 63) == 0) {
-      red[tid >> 6] = sx;
-      red[4 + (tid >> 6)] = sd;
+      red[turn][0][threadIdx.x >> 6] = sx;
+      red[turn][1][threadIdx.x >> 6] = sd;
     }
     __syncthreads();
-    sx = (red[0] + red[1]) + (red[2] + red[3]);
-    sd = (red[4] + red[5]) + (red[6] + red[7]);
+    const double* const rx = red[turn][0] + 4 * sub;
+    const double* const rd = red[turn][1] + 4 * sub;
+    turn ^= 1;
+    sx = (rx[0] + rx[1]) + (rx[2] + rx[3]);
+    sd = (rd[0] + rd[1]) + (rd[2] + rd[3]);
     const double inv64 = 1.0 / sqrt(sx / H + a.eps);
     const float inv = (float)inv64, mean = (float)(sd * inv64 / H);  // mean of dn n
+    if (on) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      float x[N], d[N], o[N];
-      unpack<DT>(xs[p], x);
-      unpack<DT>(ds[p], d);
-      if (a.d_residual) unpack<DT>(rs[p], o);
+      for (int p = 0; p < P; ++p) {
+        float x[N], d[N], o[N];
+        unpack<DT>(xs[p], x);
+        unpack<DT>(ds[p], d);
+        if (a.d_residual) unpack<DT>(rs[p], o);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float n = x[i] * inv;
-        dg[p][i] += d[i] * n;
-        const float s = (d[i] * gm[p][i] - n * mean) * inv;
-        o[i] = a.d_residual ? s + o[i] : s;
+        for (int i = 0; i < N; ++i) {
+          const float n = x[i] * inv;
+          dg[p][i] += d[i] * n;
+          const float s = (d[i] * gm[p][i] - n * mean) * inv;
+          o[i] = a.d_residual ? s + o[i] : s;
+        }
+        store_part<DT, WHOLE>(a.d_x + r * row_bytes, (p * 256 + tid) * N, H, pack<DT>(o));
       }
-      store_part<DT>(a.d_x + r * row_bytes, (p * 256 + tid) * N, H, pack<DT>(o));
     }
   }
   if (!a.parts) return;
+  for (int part = 0; part < SUB; ++part) {
+    if (sub == part) {
 #pragma unroll
-  for (int p = 0; p < P; ++p)
+      for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int col = (p * 256 + tid) * N + i;
-      if (col < H) a.parts[(int64_t)blockIdx.x * H + col] = dg[p][i];
+        for (int i = 0; i < N; ++i) {
+          const int col = (p * 256 + tid) * N + i;
+          if (col < H) {
+            const float t = part == 0 ? dg[p][i] : s_dg[col] + dg[p][i];
+            if (part + 1 < SUB) s_dg[col] = t;
+            else a.parts[(int64_t)blockIdx.x * H + col] = t;
+          }
+        }
     }
+    if constexpr (SUB > 1) __syncthreads();
+  }
 }
 // d_gamma: 64 columns a workgroup, the parts' sums in 64 bits.
 template <int DT>
@@ -300,42 +353,43 @@ __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* __restric
   }
 }
 
-// 16 codes a thread.
+// A piece of the result, from 8 or 4 codes, of four rows a thread and round.  (8192 x 7168 int8 to bf16 in us: DEQ; 16 codes a thread,
+// whose two stores fill every other 16 bytes of a line each, 65.)
 template <int DT, bool E4M3>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, int64_t rows,
                                                               int H, uint8_t* __restrict__ out) {
-  typedef uint32_t bytes16 __attribute__((ext_vector_type(4), aligned(1)));
-  const int col = (blockIdx.y * 256 + threadIdx.x) * 16;
-  if (col >= H) return;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const float s = scales[r];
-    const uint8_t* src = codes + r * H + col;
-    uint32_t c[4] = {0, 0, 0, 0};
-    const int left = H - col;
-    if (left >= 16) {
-      const bytes16 d = __builtin_nontemporal_load((const bytes16*)src);
+  constexpr int U = 4, N = NV<DT>;
+  typedef uint32_t part_t __attribute__((ext_vector_type(N / 4), aligned(1)));
+  const int col = (blockIdx.y * 256 + threadIdx.x) * N, left = H - col;
+  if (left <= 0) return;
+  for (int64_t r0 = (int64_t)blockIdx.x * U; r0 < rows; r0 += (int64_t)gridDim.x * U) {
+    uint64_t c[U];
+    float s[U];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = d[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < left) c[i / 4] |= (uint32_t)src[i] << (8 * (i & 3));
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + u < rows ? r0 + u : rows - 1;
+      const uint8_t* src = codes + r * H + col;
+      s[u] = scales[r];
+      c[u] = 0;
+      if (left >= N) {
+        const part_t d = __builtin_nontemporal_load((const part_t*)src);
+        if constexpr (N == 8) c[u] = (uint64_t)d[1] << 32 | d[0];
+        else c[u] = d[0];
+      } else {
+        for (int i = 0; i < left; ++i) c[u] |= (uint64_t)src[i] << (8 * i);
+      }
     }
-    float v[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t b = (c[i / 4] >> (8 * (i & 3))) & 0xffu;
-      if constexpr (E4M3) v[i] = ((b & 0x7f) == 0x7f ? __uint_as_float(0x7fc00000u) : e4m3_to_f32(b)) * s;
-      else v[i] = (float)(int)(int8_t)b * s;
-    }
-    uint8_t* row = out + r * H * Elem<DT>::SIZE;
-    constexpr int N = NV<DT>;
-#pragma unroll
-    for (int p = 0; p < 16 / N; ++p) {
+    for (int u = 0; u < U; ++u) {
+      if (r0 + u >= rows) break;
       float w[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) w[i] = v[p * N + i];
-      store_part<DT>(row, col + p * N, H, pack<DT>(w));
+      for (int i = 0; i < N; ++i) {
+        const uint32_t b = (uint32_t)(c[u] >> (8 * i)) & 0xffu;
+        if constexpr (E4M3) w[i] = ((b & 0x7f) == 0x7f ? __uint_as_float(0x7fc00000u) : e4m3_to_f32(b)) * s[u];
+        else w[i] = (float)(int)(int8_t)b * s[u];
+      }
+      store_part<DT, false>(out + (r0 + u) * H * Elem<DT>::SIZE, col, H, pack<DT>(w));
     }
   }
 }
@@ -348,7 +402,12 @@ void launch_norm(const NormArgs& a, hipStream_t s) {
   const int64_t groups = wave ? (a.rows + 3) / 4 : a.rows;
   const dim3 grid((unsigned)(groups < 1 << 20 ? groups : 1 << 20));
   const int per = wave ? 64 * N : 256 * N, pieces = (a.H + per - 1) / per;
-#define MOE_NORM(TPR, P) hipLaunchKernelGGL((norm_quant_kernel<DT, TPR, P, E4M3>), grid, dim3(256), 0, s, a)
+  const bool whole = a.H % N == 0;
+#define MOE_NORM(TPR, P)                                                                                            \
+  do {                                                                                                              \
+    if (whole) hipLaunchKernelGGL((norm_quant_kernel<DT, TPR, P, true, E4M3>), grid, dim3(256), 0, s, a);           \
+    else hipLaunchKernelGGL((norm_quant_kernel<DT, TPR, P, false, E4M3>), grid, dim3(256), 0, s, a);                \
+  } while (0)
   if (wave) {
     if (pieces <= 1) MOE_NORM(64, 1);
     else if (pieces <= 2) MOE_NORM(64, 2);
@@ -362,10 +421,24 @@ void launch_norm(const NormArgs& a, hipStream_t s) {
   }
 #undef MOE_NORM
 }
-template <int DT>
-void launch_norm_bwd(const NormBwdArgs& a, int groups, hipStream_t s) {
-  const int per = 256 * NV<DT>, pieces = (a.H + per - 1) / per;
-#define MOE_NORM(P) hipLaunchKernelGGL((norm_bwd_kernel<DT, P>), dim3(groups), dim3(256), 0, s, a)
+// Rows that a workgroup of the gradient has at a time: what a thread holds of each has to fit its registers (128 with four rows, 256 with
+// two).
+constexpr int bwd_sub(int pieces) { return pieces <= 2 ? 4 : pieces <= 4 ? 2 : 1; }
+int bwd_sub_of(int dtype, int64_t H) {
+  const int n = dtype == MOE_DT_FP32 ? 4 : 8;
+  return bwd_sub((int)((H + 256 * n - 1) / (256 * n)));
+}
+// ... and workgroups: two per CU, one of four rows; a part of d_gamma each.
+int bwd_groups(int64_t rows, int sub) {
+  const int64_t n = (rows + sub - 1) / sub, most = sub == 4 ? 256 : 512;
+  return (int)(n < most ? n : most);
+}
+template <int DT, bool WHOLE>
+void launch_norm_bwd(const NormBwdArgs& a, hipStream_t s) {
+  const int per = 256 * NV<DT>, pieces = (a.H + per - 1) / per, sub = bwd_sub(pieces), groups = bwd_groups(a.rows, sub);
+#define MOE_NORM(P)                                                                                                          \
+  hipLaunchKernelGGL((norm_bwd_kernel<DT, P, bwd_sub(P), WHOLE>), dim3(groups), dim3(sub * 256),                         \
+                     bwd_sub(P) > 1 && a.parts ? a.H * sizeof(float) : 0, s, a)
   if (pieces <= 1) MOE_NORM(1);
   else if (pieces <= 2) MOE_NORM(2);
   else if (pieces <= 4) MOE_NORM(4);
@@ -373,8 +446,6 @@ void launch_norm_bwd(const NormBwdArgs& a, int groups, hipStream_t s) {
   else if constexpr (NV<DT> == 4) MOE_NORM(16);
 #undef MOE_NORM
 }
-// Workgroups of the gradient: as many as run at once, and no more parts of d_gamma than that.
-int bwd_groups(int64_t rows) { return (int)(rows < 1024 ? rows : 1024); }
 
 bool row_dtype(int d) { return d == MOE_DT_BF16 || d == MOE_DT_FP16 || d == MOE_DT_FP32; }
 
@@ -410,7 +481,7 @@ extern "C" int moe_rmsnorm_quant_rows(const void* x, int dtype, const void* resi
 
 extern "C" size_t moe_rmsnorm_quant_rows_bwd_workspace_bytes(int64_t rows, int64_t H) {
   if (rows < 1 || H < 1 || H > NORM_MAX_H || rows >= (int64_t)1 << 31) return 0;
-  return (size_t)bwd_groups(rows) * H * sizeof(float);
+  return (size_t)bwd_groups(rows, 1) * H * sizeof(float);  // (512 parts at most, whatever the type)
 }
 
 extern "C" int moe_rmsnorm_quant_rows_bwd(const void* d_y, const void* x, int dtype, const void* gamma, int gamma_dtype,
@@ -421,13 +492,21 @@ extern "C" int moe_rmsnorm_quant_rows_bwd(const void* d_y, const void* x, int dt
   if (H < 1 || H > NORM_MAX_H || rows < 1 || rows >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
   if (d_gamma && (!workspace || workspace_bytes < moe_rmsnorm_quant_rows_bwd_workspace_bytes(rows, H))) return MOE_E_WORKSPACE;
   if (d_gamma && ((uintptr_t)workspace & 3)) return MOE_E_BAD_ARG;
-  const int groups = bwd_groups(rows);
+  const int groups = bwd_groups(rows, bwd_sub_of(dtype, H));
   const NormBwdArgs a{(const uint8_t*)d_y, (const uint8_t*)x, gamma, (const uint8_t*)d_residual, (uint8_t*)d_x,
                       d_gamma ? (float*)workspace : nullptr, rows, eps, (int)H, gamma_dtype};
   const hipStream_t s = (hipStream_t)stream;
-  if (dtype == MOE_DT_BF16) launch_norm_bwd<MOE_DT_BF16>(a, groups, s);
-  else if (dtype == MOE_DT_FP16) launch_norm_bwd<MOE_DT_FP16>(a, groups, s);
-  else launch_norm_bwd<MOE_DT_FP32>(a, groups, s);
+#define MOE_NORM(DT)                                                   \
+  if (H % NV<DT> == 0) launch_norm_bwd<DT, true>(a, s);                \
+  else launch_norm_bwd<DT, false>(a, s)
+  if (dtype == MOE_DT_BF16) {
+    MOE_NORM(MOE_DT_BF16);
+  } else if (dtype == MOE_DT_FP16) {
+    MOE_NORM(MOE_DT_FP16);
+  } else {
+    MOE_NORM(MOE_DT_FP32);
+  }
+#undef MOE_NORM
   MOE_CHECK_LAUNCH();
   if (!d_gamma) return MOE_OK;
   const dim3 grid((unsigned)((H + 63) / 64));
@@ -447,7 +526,9 @@ extern "C" int moe_dequantize_rows(const void* codes, int code_dtype, const floa
     return MOE_E_BAD_ARG;
   if (H < 1 || H >= (int64_t)1 << 24 || rows >= (int64_t)1 << 31) return MOE_E_BAD_SHAPE;
   if (rows == 0) return MOE_OK;
-  const dim3 grid((unsigned)(rows < 1 << 20 ? rows : 1 << 20), (unsigned)((H + 4095) / 4096));
+  const int64_t fours = (rows + 3) / 4;
+  const int per = 256 * (dtype == MOE_DT_FP32 ? 4 : 8);  // columns of a workgroup
+  const dim3 grid((unsigned)(fours < 1 << 20 ? fours : 1 << 20), (unsigned)((H + per - 1) / per));
   const hipStream_t s = (hipStream_t)stream;
 #define MOE_DEQ(DT)                                                                                                               \
   do {                                                                                                                            \
