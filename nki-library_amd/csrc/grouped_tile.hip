@@ -115,6 +115,14 @@ struct Feed {
   // Through registers: rows r < rows_left are read, terms_left bytes (ROWS_) or terms from this step on, cols_left bytes of a row.
   __device__ __forceinline__ void fetch(const uint8_t* p, int pitch, int step, int rows_left, int terms_left, int cols_left) {
     const int c = place() * 16;
+    if (ROWS_ ? rows_left >= BR && terms_left >= 128 : terms_left >= STEP && cols_left >= BR * ES) {  // (nothing ends inside)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bytes16 d = *(const bytes16*)(p + (ROWS_ ? (int64_t)step * 128 : (int64_t)step * STEP * pitch) + (int64_t)i * RPT * pitch + (int)off);
+        held[i] = make_uint4(d[0], d[1], d[2], d[3]);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int r = row() + i * RPT;

@@ -32,7 +32,19 @@ __device__ __forceinline__ u32x4 load_part(const uint8_t* row, int col, int H) {
     const uint32_t keep = col < H ? ~0u : 0u;
     return u32x4{d[0] & keep, d[1] & keep, d[2] & keep, d[3] & keep};
   }
-  if (col + NV<DT> <= H) return load_piece<DT>(row + (int64_t)col * Elem<DT>::SIZE);
+  if (H >= NV<DT>) {  // a piece that passes the row's end: the row's last one, moved down
+    const int from = col <= H - NV<DT> ? col : H - NV<DT>, gone = 8 * Elem<DT>::SIZE * (col - from);
+    const u32x4 d = load_piece<DT>(row + (int64_t)from * Elem<DT>::SIZE);
+    uint64_t lo = (uint64_t)d[1] << 32 | d[0], hi = (uint64_t)d[3] << 32 | d[2];
+    if (gone >= 64) {
+      lo = gone < 128 ? hi >> (gone - 64) : 0;
+      hi = 0;
+    } else if (gone > 0) {
+      lo = lo >> gone | hi << (64 - gone);
+      hi >>= gone;
+    }
+    return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  }
   u32x4 d = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < NV<DT>; ++i)
@@ -353,7 +365,7 @@ __global__ __launch_bounds__(1024) void norm_parts_kernel(const float* __restric
   }
 }
 
-// A piece of the result, from 8 or 4 codes, of four rows a thread and round.  (8192 x 7168 int8 to bf16 in us: DEQ; 16 codes a thread,
+// A piece of the result, from 8 or 4 codes, of four rows a thread and round.  (8192 x 7168 int8 to bf16 in us: 33; 16 codes a thread,
 // whose two stores fill every other 16 bytes of a line each, 65.)
 template <int DT, bool E4M3>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, int64_t rows,
@@ -371,10 +383,11 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(const uint8_t* __r
       const uint8_t* src = codes + r * H + col;
       s[u] = scales[r];
       c[u] = 0;
-      if (left >= N) {
-        const part_t d = __builtin_nontemporal_load((const part_t*)src);
-        if constexpr (N == 8) c[u] = (uint64_t)d[1] << 32 | d[0];
-        else c[u] = d[0];
+      if (H >= N) {  // (the last piece of a row that is not whole: the row's last codes, moved down)
+        const int gone = left < N ? N - left : 0;
+        const part_t d = __builtin_nontemporal_load((const part_t*)(src - gone));
+        if constexpr (N == 8) c[u] = ((uint64_t)d[1] << 32 | d[0]) >> (8 * gone);
+        else c[u] = d[0] >> (8 * gone);
       } else {
         for (int i = 0; i < left; ++i) c[u] |= (uint64_t)src[i] << (8 * i);
       }
