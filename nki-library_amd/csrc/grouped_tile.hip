@@ -519,18 +519,53 @@ int launch(const GroupedArgs& p, hipStream_t s) {
   return MOE_OK;
 }
 
+#include "grouped_few.hpp"
+
 typedef Cfg<256, 256, 2, 4, true, 1> Large;
 typedef Cfg<128, 128, 2, 2, true, 2> Small;
 typedef Cfg<128, 128, 2, 2, false, 2> Any;
 
+// Which kernel: the one whose time per step of 64 terms (128 bytes), as it was measured, is the least, in ns; n: its tiles over the 256
+// CUs of the chip.  A launch of few tiles takes the time of one tile's steps, one of many grows with them:
+//   256 x 256  1250, from n = 0.86 on 1460 n   (8192 rows of 4096 x 1024 | 2048 bf16: 90 | 103 us)
+//   128 x 128   600, from n = 1.25 on  480 n   (the same 68 | 129 us; 1 row of 7168 x 4096 int8 33, 2048 rows 75)
+//   any address 1150, from there on 1200 n     (1999 rows of 1030 x 515 int8 22 us)
+//   few rows, weights along their terms: 16 rows at a time 82, from n = 0.78 on 105 n; 32 rows 100, from n = 0.65 on 154 n
+//     (7168 x 4096 int8, 1 | 16 | 32 | 64 rows: 10.5 | 10.6 | 13.6 | 22.4 us; tiles of 128 x 128 33 | 32 | 32 | 35)
+//   few rows, weights across them: 282 | 358 for every round of the chip
+//     (64 rows of 128 bf16 experts of 2048 x 1536: 61 us, tiles of 128 x 128 75; 2048 rows 166 and 161)
+// Rows of a group are not known here: they are taken as spread over as many groups as there may be, half a tile of each filled up.
+struct Estimate {
+  int64_t S, groups, cols;
+  int64_t tiles(int bm, int bn) const {
+    const int64_t t = groups > 1 ? S / bm + groups / 2 : (S + bm - 1) / bm;
+    return (t > groups ? t : groups) * ((cols + bn - 1) / bn);
+  }
+};
 template <int MODE, bool B_ROWS>
 int choose(const GroupedArgs& p, hipStream_t s) {
   const uintptr_t at = (uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.out | (uintptr_t)p.a_pitch | (uintptr_t)p.b_pitch | (uintptr_t)p.out_pitch;
   const bool aligned = (at & 15) == 0;
+  const int64_t groups = p.offsets ? (p.S < p.E ? p.S : p.E) : 1;
+  const Estimate e = MODE == GG_ROWS ? Estimate{p.S, groups, p.N} : Estimate{p.K, 1, p.N};
+  const int64_t each = MODE == GG_ROWS ? 1 : p.E;  // (a result per group)
+  auto larger = [](int64_t a, int64_t b) { return a > b ? a : b; };
+  const int64_t large = larger(1250, 1460 * each * e.tiles(256, 256) / 256), small = larger(600, 480 * each * e.tiles(128, 128) / 256);
+  const int64_t any = larger(1150, 1200 * each * e.tiles(128, 128) / 256);
+  const int64_t tile = !aligned ? any : large < small ? large : small;
+  if constexpr (MODE == GG_ROWS) {
+    constexpr int COLS = B_ROWS ? 16 : 128;
+    const int64_t n1 = e.tiles(16, COLS), n2 = e.tiles(32, COLS);
+    const int64_t few1 = B_ROWS ? larger(82, 105 * n1 / 256) : 282 * ((n1 + 255) / 256);
+    const int64_t few2 = B_ROWS ? larger(100, 154 * n2 / 256) : 358 * ((n2 + 255) / 256);
+    const int64_t few = few1 < few2 ? few1 : few2;
+    if (few < tile && p.K * ES >= 16 && p.N >= 8 && p.S < (1 << 19)) {  // (a launch has fewer than 2^16 workgroups along the rows)
+      const bool whole = p.a_pitch % 16 == 0;
+      return few1 <= few2 ? launch_few<B_ROWS, 1>(p, whole, s) : launch_few<B_ROWS, 2>(p, whole, s);
+    }
+  }
   if (!aligned) return launch<Any, MODE, B_ROWS>(p, s);
-  const int64_t rows = MODE == GG_ROWS ? p.S / p.E : p.K;
-  if (rows >= 128 && p.N >= 256) return launch<Large, MODE, B_ROWS>(p, s);
-  return launch<Small, MODE, B_ROWS>(p, s);
+  return large < small ? launch<Large, MODE, B_ROWS>(p, s) : launch<Small, MODE, B_ROWS>(p, s);
 }
 
 }  // namespace
