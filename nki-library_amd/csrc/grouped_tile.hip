@@ -217,11 +217,11 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
   int* const cum = bound + p.E + 3;
   build_group_table(p.offsets, p.E, (int)p.S, C::BM, bound, cum);
 
-  // Tiles go to the XCDs (workgroup b is on XCD b % 8) in eight runs of neighbours, so that what tiles share is in one L2: blocks of
-  // up to four row tiles of a group by all columns, row tiles fastest.
+  // Tiles go out in rounds, in each of them a run of neighbours to every XCD (workgroup b is on XCD b % 8), so that what tiles share is
+  // in one L2 and all XCDs work at the same group: blocks of up to four row tiles of a group by all columns, row tiles fastest.  (A run
+  // for all rounds gave one of 8 experts to each XCD: the gradient of their weights took 227 us for 8192 rows of 4096 x 2048 instead of DWROUND.)
   const int ntn = (int)((p.N + C::BN - 1) / C::BN), ntm = (int)((p.K + C::BM - 1) / C::BM);
   const int64_t total = MODE == GG_ROWS ? (int64_t)uni(cum[p.E + 2]) * ntn : (int64_t)p.E * ntm * ntn;
-  const int64_t per = (total + 7) / 8, first = (blockIdx.x & 7) * per, end = first + per < total ? first + per : total;
 
   auto find = [&](int64_t t) {
     Tile q;
@@ -313,8 +313,8 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
   // at least STORES of them stand behind the loads in the order in which these are waited for (stored), or nothing is counted on.
   constexpr int STORES = 2 * C::MT;
   bool stored = false;
-  int64_t t = first + (blockIdx.x >> 3);
-  if (t >= end) return;
+  int64_t t = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (t >= total) return;
   Tile q = find(t);
   if constexpr (C::DMA) load_two(q);
   for (;;) {
@@ -403,10 +403,10 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
       else if (v > 2) multiply(std::integral_constant<int, 4>{});
       else multiply(std::integral_constant<int, 2>{});
     }
-    const bool last = t + (gridDim.x >> 3) >= end;
+    const bool last = t + gridDim.x >= total;
     Tile following = q;
     if (!last) {
-      t += gridDim.x >> 3;
+      t += gridDim.x;
       following = find(t);
       if constexpr (C::DMA) load_two(following);
     }
