@@ -90,7 +90,7 @@ struct Feed {
   static constexpr int RPT = THREADS / PPR;            // rows between two pieces of a thread
   static_assert(THREADS % PPR == 0 && RPT % 16 == 0, "a thread's pieces lie alike in all of its rows");
   uint32_t off;  // of the thread's first piece; piece i lies i * RPT rows behind it
-  uint4 held[DMA ? 1 : N];
+  words4 held[DMA ? 1 : N];
 
   static __device__ __forceinline__ int row() { return threadIdx.x / PPR; }
   static __device__ __forceinline__ int place() { return threadIdx.x % PPR; }
@@ -119,7 +119,7 @@ struct Feed {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const bytes16 d = *(const bytes16*)(p + (ROWS_ ? (int64_t)step * 128 : (int64_t)step * STEP * pitch) + (int64_t)i * RPT * pitch + (int)off);
-        held[i] = make_uint4(d[0], d[1], d[2], d[3]);
+        held[i] = words4{d[0], d[1], d[2], d[3]};
       }
       return;
     }
@@ -152,12 +152,16 @@ struct Feed {
           }
         }
       }
-      held[i] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+      // (One value of 128 bits from here on: as two of 64 that meet in a branch, the compiler has been seen to take half of their registers
+      // for free while they wait to be put.)
+      words4 v = {(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+      asm volatile("" : "+v"(v));
+      held[i] = v;
     }
   }
   __device__ __forceinline__ void put(uint8_t* lds) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) *(uint4*)(lds + (row() + i * RPT) * PITCH + swizzled() * 16) = held[i];
+    for (int i = 0; i < N; ++i) *(words4*)(lds + (row() + i * RPT) * PITCH + swizzled() * 16) = held[i];
   }
 };
 // ... and a wave's fragments out of it: tiles of 16 rows (columns), the first and every LEAP-th behind it.
@@ -309,14 +313,30 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
     }
   };
 
-  // A tile's first two steps are requested ahead of the results of the tile before, whose stores then drain under its first steps:
+  // otherwise: a step into registers (nothing from the last one on), and from there into its stage
+  auto fetch = [&](const Tile& q, int terms, int step) {
+    const int left = terms - step * STEP;
+    fa.fetch(q.a, pa, step, q.rows, A_ROWS ? left * ES : left, q.rows * ES);
+    fb.fetch(q.b, pb, step, q.cols, B_ROWS ? left * ES : left, q.cols * ES);
+  };
+  auto put = [&](int step) {
+    uint8_t* st = smem + (step & 1) * C::STAGE;
+    fa.put(st);
+    fb.put(st + SA);
+  };
+  auto begin = [&](const Tile& q) {
+    if constexpr (C::DMA) load_two(q);
+    else if (q.steps > 0) fetch(q, terms_of(q), 0);
+  };
+
+  // A tile's first two steps (without DMA: the first) are requested ahead of the results of the tile before, whose stores then drain under its first steps:
   // at least STORES of them stand behind the loads in the order in which these are waited for (stored), or nothing is counted on.
   constexpr int STORES = 2 * C::MT;
   bool stored = false;
   int64_t t = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
   if (t >= total) return;
   Tile q = find(t);
-  if constexpr (C::DMA) load_two(q);
+  begin(q);
   for (;;) {
     const int terms = terms_of(q);
     acc_t acc[C::MT][C::NT];
@@ -325,16 +345,6 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
 #pragma unroll
       for (int n = 0; n < C::NT; ++n) acc[m][n] = acc_t{0, 0, 0, 0};
 
-    auto fetch = [&](int step) {
-      const int left = terms - step * STEP;  // (none from the last step on)
-      fa.fetch(q.a, pa, step, q.rows, A_ROWS ? left * ES : left, q.rows * ES);
-      fb.fetch(q.b, pb, step, q.cols, B_ROWS ? left * ES : left, q.cols * ES);
-    };
-    auto put = [&](int step) {
-      uint8_t* st = smem + (step & 1) * C::STAGE;
-      fa.put(st);
-      fb.put(st + SA);
-    };
     // The steps of a tile of which a wave has V row tiles.
     auto multiply = [&](auto row_tiles) {
       constexpr int V = decltype(row_tiles)::value;
@@ -342,12 +352,8 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
         if (stored) wait_loads<LOADS + STORES>();
         else wait_loads<LOADS>();
       } else {
-        barrier();  // (the tile before has been read)
-        fetch(0);
         put(0);
-        fetch(1);
-        put(1);
-        fetch(2);
+        fetch(q, terms, 1);
       }
       barrier();
       // Half a step: its MFMAs, and under those of its first rows the fragments of the next half and what `more` does.  (The order is
@@ -380,12 +386,11 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
         if constexpr (C::DMA) {
           if (ks == 0 && stored) wait_loads<STORES>();
           else wait_loads<0>();
+        } else {
+          put(ks + 1);  // (its stage was last read ahead of the barrier before)
         }
         barrier();
-        if constexpr (!C::DMA) {
-          put(ks);
-          fetch(ks + 3);
-        }
+        if constexpr (!C::DMA) fetch(q, terms, ks + 2);
         half(std::integral_constant<int, 0>{}, lds + ((ks + 1) & 1) * C::STAGE, a1, b1, a0, b0, [&](int m) {
           if constexpr (C::DMA) {
 #pragma unroll
@@ -408,7 +413,7 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
     if (!last) {
       t += gridDim.x;
       following = find(t);
-      if constexpr (C::DMA) load_two(following);
+      begin(following);
     }
 
     // ---- results: 16 rows of a wave at a time, by way of its 2 KB of LDS

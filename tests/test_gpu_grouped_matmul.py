@@ -267,3 +267,43 @@ def test_refusals():
         with pytest.raises(AssertionError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+# groups whose last tile of 256 rows holds every number of 32 rows, and tiles of 128 likewise; none at all; one of several tiles
+EVERY_TILE = [300, 250, 512, 190, 0, 130, 97, 60, 1, 34, 400, 225]
+
+
+@pytest.mark.parametrize("N", [136, 1032, 8200, 131, 1027, 8195])
+@pytest.mark.parametrize("K", [72, 256, 520, 77, 515])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_kind_of_tile(K, N, dtype):
+    """The kernel goes by the number of tiles: few columns, some and many; by whether rows are aligned; one step and several, whole
+    and cut."""
+    from nkilib.core.moe.grouped_matmul import grouped_matmul, grouped_matmul_bwd
+
+    g = torch.Generator(device="cuda").manual_seed(K + N)
+    dt, S, E = getattr(torch, dtype), sum(EVERY_TILE), len(EVERY_TILE)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(dt)
+    x, w, o = r(S, K), r(E, K, N), offsets_of(EVERY_TILE)
+    od = torch.from_numpy(o).cuda()
+    want, mag = products(x, w, o)
+    assert_near(grouped_matmul(x, w, od), want, mag, K, "forward")
+    # the gradient of the rows with the roles of the sizes changed, so that its columns are few, some and many as well
+    wt, d = r(E, N, K), r(S, K)
+    want, mag = products(d, wt.transpose(1, 2).contiguous(), o)
+    assert_near(grouped_matmul_bwd(d, None, wt, od, need_weight=False)[0], want, mag, K, "d_x")
+
+
+@pytest.mark.parametrize("K,N", [(136, 264), (1032, 1032), (2056, 1992), (131, 515), (1027, 1029), (2050, 1999), (1032, 1029)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_kind_of_tile_of_the_weights_gradient(K, N, dtype):
+    from nkilib.core.moe.grouped_matmul import grouped_matmul_bwd
+
+    g = torch.Generator(device="cuda").manual_seed(K + N)
+    dt, S, E = getattr(torch, dtype), sum(EVERY_TILE), len(EVERY_TILE)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(dt)
+    x, d, w, o = r(S, K), r(S, N), r(E, K, N), offsets_of(EVERY_TILE)
+    want, mag = outer_products(x, d, o)
+    for wdt in (dt, torch.float32):
+        _, dw = grouped_matmul_bwd(d, x, w, torch.from_numpy(o).cuda(), weight_grad_dtype=wdt, need_x=False)
+        assert_near(dw, want, mag, max(EVERY_TILE), str(wdt))

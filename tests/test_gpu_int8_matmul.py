@@ -157,3 +157,24 @@ def test_refusals():
         with pytest.raises(AssertionError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("N", [144, 1040, 8208, 131, 1027, 8195])
+@pytest.mark.parametrize("K", [64, 160, 1040, 77, 1030])
+@pytest.mark.parametrize("out", OUT)
+def test_every_kind_of_tile(K, N, out):
+    """As for the 16-bit products: few columns, some and many, aligned or not, one step and several; and a dense product of as many rows."""
+    from nkilib.core.int8_matmul import grouped_int8_matmul, int8_matmul
+    from test_gpu_grouped_matmul import EVERY_TILE
+
+    g = torch.Generator(device="cuda").manual_seed(K + N)
+    S, E, o = sum(EVERY_TILE), len(EVERY_TILE), offsets_of(EVERY_TILE)
+    x, w, xs, ws = _codes(g, S, K), _codes(g, E, N, K), _scales(g, S), _scales(g, E, N)
+    want = torch.zeros((S, N), dtype=torch.float64, device="cuda")
+    for e, a, b in groups(o, S):
+        want[a:b] = _want(x[a:b], xs[a:b], w[e], ws[e])
+    dt = getattr(torch, out)
+    assert_near(grouped_int8_matmul(x, xs, w, ws, torch.from_numpy(o).cuda(), out_dtype=dt), want, want.abs(), 4)
+    bias = torch.randn(N, generator=g, device="cuda").to(dt)
+    want = _want(x, xs, w[0], ws[0])
+    assert_near(int8_matmul(x, xs, w[0], ws[0], bias, dt), want + bias.double(), want.abs() + bias.double().abs(), 5, "dense")
