@@ -298,10 +298,11 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
     sa = fa.step_of(st, q.a, in ? q.a_bytes : 0, pa, step, left);
     sb = fb.step_of(st + SA, q.b, in ? q.b_bytes : 0, pb, step, left);
   };
-  constexpr int LA = decltype(fa)::N, LOADS = LA + decltype(fb)::N;
-  auto load = [&](int i) {
-    if (i < LA) fa.load(sa, i);
-    else fb.load(sb, i - LA);
+  constexpr int LA = decltype(fa)::N, LB = decltype(fb)::N, LOADS = LA + LB;
+  // (rows of A, RPT of them a load: those that a tile does not have are not loaded; what stands in their place has no part in its rows)
+  auto load = [&](int i, int a_loads) {
+    if (i < a_loads) fa.load(sa, i);
+    else fb.load(sb, i - a_loads);
   };
   auto load_two = [&](const Tile& q) {
     if (q.steps == 0) return;
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
     for (int step = 0; step < 2; ++step) {
       prepare(q, terms_of(q), step);
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) load(i);
+      for (int i = 0; i < LOADS; ++i) load(i, LA);
     }
   };
 
@@ -348,6 +349,8 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
     // The steps of a tile of which a wave has V row tiles.
     auto multiply = [&](auto row_tiles) {
       constexpr int V = decltype(row_tiles)::value;
+      constexpr int A_LOADS = A_ROWS ? V * C::WM * 16 / decltype(fa)::RPT : LA;
+      static_assert(!A_ROWS || V * C::WM * 16 % decltype(fa)::RPT == 0, "whole loads");
       if constexpr (C::DMA) {
         if (stored) wait_loads<LOADS + STORES>();
         else wait_loads<LOADS>();
@@ -394,7 +397,7 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
         half(std::integral_constant<int, 0>{}, lds + ((ks + 1) & 1) * C::STAGE, a1, b1, a0, b0, [&](int m) {
           if constexpr (C::DMA) {
 #pragma unroll
-            for (int i = m * LOADS / V; i < (m + 1) * LOADS / V; ++i) load(i);
+            for (int i = m * (A_LOADS + LB) / V; i < (m + 1) * (A_LOADS + LB) / V; ++i) load(i, A_LOADS);
           }
         });
       }
