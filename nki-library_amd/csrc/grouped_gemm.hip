@@ -38,9 +38,6 @@ static int check_groups(const int32_t* offsets, int64_t S, int64_t K, int64_t N,
     return MOE_E_BAD_SHAPE;
   return MOE_OK;
 }
-static int run(const GroupedArgs& p, int dtype, int mode, hipStream_t s) {
-  return dtype == MOE_DT_BF16 ? launch_grouped_bf16(p, mode, s) : launch_grouped_fp16(p, mode, s);
-}
 
 extern "C" int moe_expert_row_offsets(const int32_t* block_to_expert, int64_t N, int64_t B, int64_t E, int32_t* row_offsets,
                                       void* stream) {
@@ -63,7 +60,7 @@ extern "C" int moe_grouped_matmul(const void* x, const void* weight, int dtype, 
   p.S = S, p.K = K, p.N = N, p.E = (int)E;
   p.a_pitch = 2 * K, p.b_pitch = 2 * N, p.b_group = 2 * K * N, p.out_pitch = 2 * N;
   p.out_dtype = dtype;
-  return run(p, dtype, GG_ROWS, (hipStream_t)stream);
+  return dtype == MOE_DT_BF16 ? launch_grouped_bf16(p, (hipStream_t)stream) : launch_grouped_fp16(p, (hipStream_t)stream);
 }
 
 extern "C" int moe_grouped_matmul_bwd(const void* d_out, const void* x, const void* weight, int dtype, const int32_t* row_offsets,
@@ -74,24 +71,18 @@ extern "C" int moe_grouped_matmul_bwd(const void* d_out, const void* x, const vo
   if (d_weight && d_weight_dtype != dtype && d_weight_dtype != MOE_DT_FP32) return MOE_E_BAD_ARG;
   const int rc = check_groups(row_offsets, S, K, N, E);
   if (rc != MOE_OK) return rc;
-  GroupedArgs p{};
-  p.offsets = row_offsets, p.S = S, p.E = (int)E;
-  if (d_x && S > 0) {
-    p.a = (const uint8_t*)d_out, p.b = (const uint8_t*)weight, p.out = (uint8_t*)d_x;
-    p.K = N, p.N = K;
-    p.a_pitch = 2 * N, p.b_pitch = 2 * N, p.b_group = 2 * K * N, p.out_pitch = 2 * K;
-    p.out_dtype = dtype, p.b_rows = 1;
-    const int r = run(p, dtype, GG_ROWS, (hipStream_t)stream);
-    if (r != MOE_OK) return r;
-  }
-  if (d_weight) {
-    p.a = (const uint8_t*)x, p.b = (const uint8_t*)d_out, p.out = (uint8_t*)d_weight;
-    p.K = K, p.N = N;
-    p.a_pitch = 2 * K, p.b_pitch = 2 * N, p.b_group = 0, p.out_pitch = (d_weight_dtype == MOE_DT_FP32 ? 4 : 2) * N;
-    p.out_dtype = d_weight_dtype, p.b_rows = 0;
-    return run(p, dtype, GG_CONTRACT, (hipStream_t)stream);
-  }
-  return MOE_OK;
+  GroupedArgs px{}, pw{};
+  px.offsets = pw.offsets = row_offsets, px.S = pw.S = S, px.E = pw.E = (int)E;
+  px.a = (const uint8_t*)d_out, px.b = (const uint8_t*)weight, px.out = (uint8_t*)d_x;
+  px.K = N, px.N = K;
+  px.a_pitch = px.b_pitch = 2 * N, px.b_group = 2 * K * N, px.out_pitch = 2 * K;
+  px.out_dtype = dtype;
+  pw.a = (const uint8_t*)x, pw.b = (const uint8_t*)d_out, pw.out = (uint8_t*)d_weight;
+  pw.K = K, pw.N = N;
+  pw.a_pitch = 2 * K, pw.b_pitch = 2 * N, pw.out_pitch = (d_weight_dtype == MOE_DT_FP32 ? 4 : 2) * N;
+  pw.out_dtype = d_weight_dtype;
+  const auto launch = dtype == MOE_DT_BF16 ? launch_grouped_bwd_bf16 : launch_grouped_bwd_fp16;
+  return launch(d_x ? &px : nullptr, d_weight ? &pw : nullptr, (hipStream_t)stream);
 }
 
 extern "C" int moe_int8_matmul(const int8_t* x, const float* x_scales, const int8_t* weight, const float* weight_scales,
@@ -109,6 +100,6 @@ extern "C" int moe_int8_matmul(const int8_t* x, const float* x_scales, const int
   p.a_scale = x_scales, p.b_scale = weight_scales, p.bias = bias;
   p.S = S, p.K = K, p.N = N, p.E = (int)E;
   p.a_pitch = K, p.b_pitch = K, p.b_group = K * N, p.out_pitch = (out_dtype == MOE_DT_FP32 ? 4 : 2) * N;
-  p.out_dtype = out_dtype, p.b_rows = 1;
-  return launch_grouped_int8(p, GG_ROWS, (hipStream_t)stream);
+  p.out_dtype = out_dtype;
+  return launch_grouped_int8(p, (hipStream_t)stream);
 }

@@ -24,7 +24,6 @@ struct GroupedArgs {
   int64_t a_pitch, b_pitch, b_group, out_pitch;  // bytes from row to row, from matrix to matrix
   int E;
   int out_dtype;  // MOE_DT_*
-  int b_rows;     // the matrices' rows are the result's columns ([E, N, K]), not its terms ([E, K, N])
 };
 
 // The groups' bounds as a workgroup keeps them: group j of E + 2 holds rows [bound[j], bound[j + 1]) and tiles [cum[j], cum[j + 1])
@@ -98,8 +97,11 @@ __device__ __forceinline__ int group_of_tile(const int* cum, int E, int r) {
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-int launch_grouped_bf16(const GroupedArgs& p, int mode, hipStream_t s);
-int launch_grouped_fp16(const GroupedArgs& p, int mode, hipStream_t s);
-int launch_grouped_int8(const GroupedArgs& p, int mode, hipStream_t s);
+// A product, and its gradients (either may be null).
+int launch_grouped_bf16(const GroupedArgs& p, hipStream_t s);
+int launch_grouped_fp16(const GroupedArgs& p, hipStream_t s);
+int launch_grouped_bwd_bf16(const GroupedArgs* px, const GroupedArgs* pw, hipStream_t s);
+int launch_grouped_bwd_fp16(const GroupedArgs* px, const GroupedArgs* pw, hipStream_t s);
+int launch_grouped_int8(const GroupedArgs& p, hipStream_t s);
 
 }  // namespace moe

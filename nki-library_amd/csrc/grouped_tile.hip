@@ -208,10 +208,11 @@ struct Cfg {
   static_assert(NT % 4 == 0, "64 columns make lines of 128 bytes");
 };
 
+// The tiles t, t + workgroups and so on of a product; the first such number behind them is the result, counted from the last tile on.
+// (The groups' table stands behind C::LDS.)
 template <class C, int MODE, bool B_ROWS>
-__global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::PER_CU * C::THREADS / 256, C::PER_CU * C::THREADS / 256))) void grouped_kernel(const GroupedArgs p) {
+__device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const smem, int64_t t) {
   constexpr bool A_ROWS = MODE == GG_ROWS;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, wave = uni(tid >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
   lds_byte* const lds = (lds_byte*)smem;
@@ -219,11 +220,7 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
   uint8_t* const exchange = smem + 2 * C::STAGE + wave * C::EXCHANGE;
   int* const bound = (int*)(smem + C::LDS);
   int* const cum = bound + p.E + 3;
-  build_group_table(p.offsets, p.E, (int)p.S, C::BM, bound, cum);
-
-  // Tiles go out in rounds, in each of them a run of neighbours to every XCD (workgroup b is on XCD b % 8), so that what tiles share is
-  // in one L2 and all XCDs work at the same group: blocks of up to four row tiles of a group by all columns, row tiles fastest.  (A run
-  // for all rounds gave one of 8 experts to each XCD: the gradient of their weights took 227 us for 8192 rows of 4096 x 2048 instead of DWROUND.)
+  // blocks of up to four row tiles of a group by all columns, row tiles fastest
   const int ntn = (int)((p.N + C::BN - 1) / C::BN), ntm = (int)((p.K + C::BM - 1) / C::BM);
   const int64_t total = MODE == GG_ROWS ? (int64_t)uni(cum[p.E + 2]) * ntn : (int64_t)p.E * ntm * ntn;
 
@@ -334,8 +331,7 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
   // at least STORES of them stand behind the loads in the order in which these are waited for (stored), or nothing is counted on.
   constexpr int STORES = 2 * C::MT;
   bool stored = false;
-  int64_t t = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  if (t >= total) return;
+  if (t >= total) return t - total;
   Tile q = find(t);
   begin(q);
   for (;;) {
@@ -505,24 +501,62 @@ __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::P
         }
       }
     }
-    if (last) break;
+    if (last) return t + gridDim.x - total;
     stored = C::NT == 4 && q.rows == C::BM && q.cols == C::BN;
     q = following;
   }
 }
 
+// Tiles go out in rounds, in each of them a run of neighbours to every XCD (workgroup b is on XCD b % 8), so that what tiles share is
+// in one L2 and all XCDs work at the same group.  (A run for all rounds gave one of 8 experts to each XCD: the gradient of their
+// weights took 227 us for 8192 rows of 4096 x 2048, popular and unpopular, instead of 164.)
+__device__ __forceinline__ int64_t first_tile() { return (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3); }
+#define GG_KERNEL __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::PER_CU * C::THREADS / 256, C::PER_CU * C::THREADS / 256)))
+
+template <class C, int MODE, bool B_ROWS>
+GG_KERNEL void grouped_kernel(const GroupedArgs p) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  int* const bound = (int*)(smem + C::LDS);
+  build_group_table(p.offsets, p.E, (int)p.S, C::BM, bound, bound + p.E + 3);
+  tiles_of<C, MODE, B_ROWS>(p, smem, first_tile());
+}
+// Both gradients, of the rows and then of the weights (the same groups): the workgroups that the last round of the first leaves idle begin
+// with the second.  (8192 rows of 4096 x 2048 bf16 in 8 groups: 2.25 and 4 rounds, 303 us; one after the other 322.)
+template <class C>
+GG_KERNEL void grouped_bwd_kernel(const GroupedArgs px, const GroupedArgs pw) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  int* const bound = (int*)(smem + C::LDS);
+  build_group_table(px.offsets, px.E, (int)px.S, C::BM, bound, bound + px.E + 3);
+  const int64_t t = tiles_of<C, GG_ROWS, true>(px, smem, first_tile());
+  __syncthreads();
+  tiles_of<C, GG_CONTRACT, false>(pw, smem, t);
+}
+
+template <class C, int MODE>
+int64_t most_tiles(const GroupedArgs& p) {  // (groups without rows have none)
+  const int64_t ntn = (p.N + C::BN - 1) / C::BN, ntm = (p.K + C::BM - 1) / C::BM;
+  return MODE == GG_ROWS ? ((p.S + C::BM - 1) / C::BM + (p.S < p.E + 1 ? p.S : p.E + 1)) * ntn : p.E * ntm * ntn;
+}
+template <class C>
+unsigned workgroups(int64_t tiles) {  // no more than run at once
+  const int cus = device_cus();
+  const int64_t at_once = (int64_t)(cus > 0 ? cus : 256) * C::PER_CU;
+  return (unsigned)((tiles < at_once ? tiles + 7 : at_once) / 8 * 8);
+}
 template <class C, int MODE, bool B_ROWS>
 int launch(const GroupedArgs& p, hipStream_t s) {
   constexpr auto kernel = grouped_kernel<C, MODE, B_ROWS>;
-  const int lds = C::LDS + (p.E + 3) * 8;
   if (allow_lds<kernel>(160 * 1024) != hipSuccess) return MOE_E_LAUNCH;
-  const int cus = device_cus();
-  const int64_t ntn = (p.N + C::BN - 1) / C::BN, ntm = (p.K + C::BM - 1) / C::BM;
-  // tiles at most (groups without rows have none), workgroups at most as many as run at once
-  const int64_t most = MODE == GG_ROWS ? ((p.S + C::BM - 1) / C::BM + (p.S < p.E + 1 ? p.S : p.E + 1)) * ntn : p.E * ntm * ntn;
-  const int64_t at_once = (int64_t)(cus > 0 ? cus : 256) * C::PER_CU;
-  const int64_t groups = (most < at_once ? most + 7 : at_once) / 8 * 8;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(C::THREADS), lds, s, p);
+  hipLaunchKernelGGL(kernel, dim3(workgroups<C>(most_tiles<C, MODE>(p))), dim3(C::THREADS), C::LDS + (p.E + 3) * 8, s, p);
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+template <class C>
+int launch_bwd(const GroupedArgs& px, const GroupedArgs& pw, hipStream_t s) {
+  constexpr auto kernel = grouped_bwd_kernel<C>;
+  if (allow_lds<kernel>(160 * 1024) != hipSuccess) return MOE_E_LAUNCH;
+  const int64_t tiles = most_tiles<C, GG_ROWS>(px) + most_tiles<C, GG_CONTRACT>(pw);
+  hipLaunchKernelGGL(kernel, dim3(workgroups<C>(tiles)), dim3(C::THREADS), C::LDS + (px.E + 3) * 8, s, px, pw);
   MOE_CHECK_LAUNCH();
   return MOE_OK;
 }
@@ -550,8 +584,9 @@ struct Estimate {
     return (t > groups ? t : groups) * ((cols + bn - 1) / bn);
   }
 };
+enum Kind { ANY, SMALL, LARGE, FEW1, FEW2 };
 template <int MODE, bool B_ROWS>
-int choose(const GroupedArgs& p, hipStream_t s) {
+Kind choose(const GroupedArgs& p) {
   const uintptr_t at = (uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.out | (uintptr_t)p.a_pitch | (uintptr_t)p.b_pitch | (uintptr_t)p.out_pitch;
   const bool aligned = (at & 15) == 0;
   const int64_t groups = p.offsets ? (p.S < p.E ? p.S : p.E) : 1;
@@ -567,30 +602,40 @@ int choose(const GroupedArgs& p, hipStream_t s) {
     const int64_t few1 = B_ROWS ? larger(82, 105 * n1 / 256) : 282 * ((n1 + 255) / 256);
     const int64_t few2 = B_ROWS ? larger(100, 154 * n2 / 256) : 358 * ((n2 + 255) / 256);
     const int64_t few = few1 < few2 ? few1 : few2;
-    if (few < tile && p.K * ES >= 16 && p.N >= 8 && p.S < (1 << 19)) {  // (a launch has fewer than 2^16 workgroups along the rows)
-      const bool whole = p.a_pitch % 16 == 0;
-      return few1 <= few2 ? launch_few<B_ROWS, 1>(p, whole, s) : launch_few<B_ROWS, 2>(p, whole, s);
-    }
+    // (a launch has fewer than 2^16 workgroups along the rows)
+    if (few < tile && p.K * ES >= 16 && p.N >= 8 && p.S < (1 << 19)) return few1 <= few2 ? FEW1 : FEW2;
   }
-  if (!aligned) return launch<Any, MODE, B_ROWS>(p, s);
-  return large < small ? launch<Large, MODE, B_ROWS>(p, s) : launch<Small, MODE, B_ROWS>(p, s);
+  return !aligned ? ANY : large < small ? LARGE : SMALL;
+}
+template <int MODE, bool B_ROWS>
+int run(const GroupedArgs& p, hipStream_t s) {
+  const Kind kind = choose<MODE, B_ROWS>(p);
+  if constexpr (MODE == GG_ROWS) {
+    if (kind == FEW1) return launch_few<B_ROWS, 1>(p, p.a_pitch % 16 == 0, s);
+    if (kind == FEW2) return launch_few<B_ROWS, 2>(p, p.a_pitch % 16 == 0, s);
+  }
+  return kind == ANY ? launch<Any, MODE, B_ROWS>(p, s) : kind == LARGE ? launch<Large, MODE, B_ROWS>(p, s) : launch<Small, MODE, B_ROWS>(p, s);
 }
 
 }  // namespace
 
-#if GG_TYPE == 0
-int launch_grouped_bf16(const GroupedArgs& p, int mode, hipStream_t s) {
-#elif GG_TYPE == 1
-int launch_grouped_fp16(const GroupedArgs& p, int mode, hipStream_t s) {
-#else
-int launch_grouped_int8(const GroupedArgs& p, int mode, hipStream_t s) {
-#endif
 #if GG_TYPE == 2
-  return choose<GG_ROWS, true>(p, s);
+int launch_grouped_int8(const GroupedArgs& p, hipStream_t s) { return run<GG_ROWS, true>(p, s); }
 #else
-  if (mode == GG_CONTRACT) return choose<GG_CONTRACT, false>(p, s);
-  return p.b_rows ? choose<GG_ROWS, true>(p, s) : choose<GG_ROWS, false>(p, s);
+#if GG_TYPE == 0
+#define GG_NAME(WHAT) WHAT##_bf16
+#else
+#define GG_NAME(WHAT) WHAT##_fp16
 #endif
+int GG_NAME(launch_grouped)(const GroupedArgs& p, hipStream_t s) { return run<GG_ROWS, false>(p, s); }
+int GG_NAME(launch_grouped_bwd)(const GroupedArgs* px, const GroupedArgs* pw, hipStream_t s) {
+  if (px && pw && px->S > 0 && choose<GG_ROWS, true>(*px) == LARGE && choose<GG_CONTRACT, false>(*pw) == LARGE) return launch_bwd<Large>(*px, *pw, s);
+  if (px && px->S > 0) {
+    const int rc = run<GG_ROWS, true>(*px, s);
+    if (rc != MOE_OK) return rc;
+  }
+  return pw ? run<GG_CONTRACT, false>(*pw, s) : MOE_OK;
 }
+#endif
 
 }  // namespace moe

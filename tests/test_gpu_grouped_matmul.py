@@ -307,3 +307,24 @@ def test_every_kind_of_tile_of_the_weights_gradient(K, N, dtype):
     for wdt in (dt, torch.float32):
         _, dw = grouped_matmul_bwd(d, x, w, torch.from_numpy(o).cuda(), weight_grad_dtype=wdt, need_x=False)
         assert_near(dw, want, mag, max(EVERY_TILE), str(wdt))
+
+
+@pytest.mark.parametrize("K,N", [(4104, 520), (4096, 264)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_both_gradients_in_one_launch(K, N, dtype):
+    """Many large tiles of either: the same bits as one after the other."""
+    from nkilib.core.moe.grouped_matmul import grouped_matmul_bwd
+
+    g = torch.Generator(device="cuda").manual_seed(K + N)
+    dt, S, E = getattr(torch, dtype), sum(EVERY_TILE), len(EVERY_TILE)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(dt)
+    x, d, w, o = r(S, K), r(S, N), r(E, K, N), offsets_of(EVERY_TILE)
+    od = torch.from_numpy(o).cuda()
+    for wdt in (dt, torch.float32):
+        dx, dw = grouped_matmul_bwd(d, x, w, od, weight_grad_dtype=wdt)
+        want, mag = products(d, w.transpose(1, 2).contiguous(), o)
+        assert_near(dx, want, mag, N, "d_x")
+        want, mag = outer_products(x, d, o)
+        assert_near(dw, want, mag, max(EVERY_TILE), "d_w")
+        assert torch.equal(dx, grouped_matmul_bwd(d, None, w, od, need_weight=False)[0])
+        assert torch.equal(dw, grouped_matmul_bwd(d, x, w, od, weight_grad_dtype=wdt, need_x=False)[1])
