@@ -449,7 +449,7 @@ int moe_dequantize_checkpoint(const uint8_t* codes, const uint8_t* scales, int64
 /* No counterpart in the reference (its layers multiply the experts inside, bwmm_shard_on_block.py:972-1038).  Rows
  * row_offsets[e] .. row_offsets[e + 1] (int32 [E + 1], device) are expert e's; whatever the offsets are, they are taken into [0, S] and
  * as never falling, and rows of no expert are zero in the result.  E <= 1024; K, N in [1, 2^20]; S < 2^31 - 1024.  Sums are taken in fp32 and
- * rounded once.  Pointers aligned to their element; rows whose pitch and tensors whose address are multiples of 16 bytes are faster.
+ * rounded once.  Pointers aligned to their element; rows whose pitch and tensors whose address are multiples of 16 bytes, or of 4, are faster.
  *
  * moe_expert_row_offsets: block_to_expert [N], experts ascending (blocks of no expert in [0, E) behind the others), B rows a block ->
  * row_offsets.

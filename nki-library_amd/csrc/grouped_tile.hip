@@ -8,10 +8,14 @@
 //   rows:    LDS row of 128 bytes per row; piece j of row r in place j ^ (r & 7)
 //   columns: LDS row of BN columns per term; piece j of term k in place j ^ f(k), f(k) = 2 (k & 3) + 8 ((k >> 3) & 1): the 16 lanes of
 //            a transposing read fetch 32 bytes from each of 4 terms, two such groups at a time terms 8 apart, all in other banks.
-// DMA: operands go global -> LDS without a register (rows aligned to 16 bytes); otherwise through registers, element by element
-// where a piece passes a row's end.  Two stages; a step's second half of fragments is read under the MFMAs of its first, the next
-// step's first half under those of its second; the one barrier of a step stands between them: all have read the step's stage, which then
-// takes the step after the next, and the next step's has landed.
+// DMA: operands go global -> LDS without a register (rows that begin at 4 bytes; at 16 they come faster, 8192 rows of 4160 x 4160 bf16 348
+// | 408 us); otherwise through registers, where a piece that passes a row's end is the row's last one moved down (641 us).  Two stages; a
+// step's second half of fragments is read under the MFMAs of its first, the next step's first half under those of its second; the one
+// barrier of a step stands between them: all have read the step's stage, which then takes the step after the next, and the next step's
+// has landed.  The loads go out one per row tile of the second half: all at once they hold up the waves' issue (8192^3 bf16 895 | 857 us).
+// What bounds it: 70 % of the cycles the matrix pipes work (2950 cycles for a step of 256 x 256, MFMAs alone 2048), the rest is the barrier
+// and what stands around it; after some milliseconds power leaves a clock of 1.5 GHz.  8192^3, us: bf16 weights across 806 (1.36 PFLOP/s),
+// along 793, their gradient 808, int8 500 (2.2 POP/s).
 // The matrix is the MFMA's first operand, so that a lane holds four neighbouring columns of one row; rows go out through LDS in whole
 // 128-byte lines.
 #include <type_traits>
@@ -39,9 +43,6 @@ __device__ __forceinline__ acc_t mfma(const v4i& w, const v4i& x, const acc_t& c
 }
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uni64(int64_t v) {
-  return ((int64_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v);
-}
 
 // Raw buffer over `bytes` (any number; offsets of a step stay below 2^31) from p on: what lies outside reads as zeros.
 __device__ __forceinline__ v4i buffer_of(const uint8_t* p, int64_t bytes) {
@@ -196,10 +197,11 @@ struct Frags {
   }
 };
 
-template <int BM_, int BN_, int WM_, int WN_, bool DMA_, int PER_CU_>
+// WHOLE: rows of all operands are multiples of 16 bytes and begin at such.
+template <int BM_, int BN_, int WM_, int WN_, bool DMA_, bool WHOLE_, int PER_CU_>
 struct Cfg {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = WM * WN * 64;
-  static constexpr bool DMA = DMA_;
+  static constexpr bool DMA = DMA_, WHOLE = WHOLE_;
   static constexpr int PER_CU = PER_CU_;  // workgroups of a CU
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;
   static constexpr int STAGE = (BM + BN) * 128;
@@ -322,6 +324,20 @@ __device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const
     fa.put(st);
     fb.put(st + SA);
   };
+  // DMA: a row's end inside a piece leaves the next row's first terms behind it in the last step's stage: zeros in their place
+  const int last_bytes = MODE == GG_ROWS ? (int)((p.K * ES - 1) % 128 + 1) : 128;
+  auto cut = [&](int step) {
+    uint8_t* const st = smem + (step & 1) * C::STAGE;
+    const int piece = last_bytes / 16;
+    if constexpr (A_ROWS)
+      for (int r = tid; r < C::BM; r += C::THREADS)
+        for (int w = last_bytes & 15; w < 16; w += 4) *(uint32_t*)(st + r * 128 + ((piece ^ (r & 7)) * 16) + w) = 0;
+    if constexpr (B_ROWS)
+      for (int r = tid; r < C::BN; r += C::THREADS)
+        for (int w = last_bytes & 15; w < 16; w += 4) *(uint32_t*)(st + SA + r * 128 + ((piece ^ (r & 7)) * 16) + w) = 0;
+    barrier();
+  };
+  const bool cuts = C::DMA && !C::WHOLE && last_bytes % 16 != 0;
   auto begin = [&](const Tile& q) {
     if constexpr (C::DMA) load_two(q);
     else if (q.steps > 0) fetch(q, terms_of(q), 0);
@@ -355,6 +371,7 @@ __device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const
         fetch(q, terms, 1);
       }
       barrier();
+      if (cuts && q.steps == 1) cut(0);
       // Half a step: its MFMAs, and under those of its first rows the fragments of the next half and what `more` does.  (The order is
       // pinned: left to itself the compiler moves every read to where its value is used and waits for it there.)
       auto half = [&](auto next_half, const lds_byte* st, v4i (&a)[V], v4i (&b)[C::NT], v4i (&an)[V], v4i (&bn)[C::NT], auto&& more) {
@@ -389,6 +406,7 @@ __device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const
           put(ks + 1);  // (its stage was last read ahead of the barrier before)
         }
         barrier();
+        if (cuts && ks + 2 == q.steps) cut(ks + 1);
         if constexpr (!C::DMA) fetch(q, terms, ks + 2);
         half(std::integral_constant<int, 0>{}, lds + ((ks + 1) & 1) * C::STAGE, a1, b1, a0, b0, [&](int m) {
           if constexpr (C::DMA) {
@@ -462,7 +480,7 @@ __device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const
             const uint4 d = *(const uint4*)(exchange + r * 128 + (lane & 7) * 16);
             if (r0 + r < q.rows && col < cols) {
               uint8_t* o = q.out + (int64_t)(r0 + r) * p.out_pitch + (col0 + col) * oes;
-              if (C::DMA || col + per_piece <= cols) {
+              if (C::WHOLE || col + per_piece <= cols) {
                 *(bytes16*)o = bytes16{d.x, d.y, d.z, d.w};
               } else {
                 const uint32_t w[4] = {d.x, d.y, d.z, d.w};
@@ -563,9 +581,11 @@ int launch_bwd(const GroupedArgs& px, const GroupedArgs& pw, hipStream_t s) {
 
 #include "grouped_few.hpp"
 
-typedef Cfg<256, 256, 2, 4, true, 1> Large;
-typedef Cfg<128, 128, 2, 2, true, 2> Small;
-typedef Cfg<128, 128, 2, 2, false, 2> Any;
+typedef Cfg<256, 256, 2, 4, true, true, 1> Large;
+typedef Cfg<128, 128, 2, 2, true, true, 2> Small;
+typedef Cfg<256, 256, 2, 4, true, false, 1> LargeCut;
+typedef Cfg<128, 128, 2, 2, true, false, 2> SmallCut;
+typedef Cfg<128, 128, 2, 2, false, false, 2> Any;
 
 // Which kernel: the one whose time per step of 64 terms (128 bytes), as it was measured, is the least, in ns; n: its tiles over the 256
 // CUs of the chip.  A launch of few tiles takes the time of one tile's steps, one of many grows with them:
@@ -585,10 +605,14 @@ struct Estimate {
   }
 };
 enum Kind { ANY, SMALL, LARGE, FEW1, FEW2 };
+bool rows_at(const GroupedArgs& p, int bytes) {
+  const uintptr_t at = (uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.a_pitch | (uintptr_t)p.b_pitch;
+  return (at & (bytes - 1)) == 0;
+}
+bool whole_rows(const GroupedArgs& p) { return rows_at(p, 16) && (((uintptr_t)p.out | (uintptr_t)p.out_pitch) & 15) == 0; }
 template <int MODE, bool B_ROWS>
 Kind choose(const GroupedArgs& p) {
-  const uintptr_t at = (uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.out | (uintptr_t)p.a_pitch | (uintptr_t)p.b_pitch | (uintptr_t)p.out_pitch;
-  const bool aligned = (at & 15) == 0;
+  const bool aligned = rows_at(p, 4);
   const int64_t groups = p.offsets ? (p.S < p.E ? p.S : p.E) : 1;
   const Estimate e = MODE == GG_ROWS ? Estimate{p.S, groups, p.N} : Estimate{p.K, 1, p.N};
   const int64_t each = MODE == GG_ROWS ? 1 : p.E;  // (a result per group)
@@ -614,7 +638,9 @@ int run(const GroupedArgs& p, hipStream_t s) {
     if (kind == FEW1) return launch_few<B_ROWS, 1>(p, p.a_pitch % 16 == 0, s);
     if (kind == FEW2) return launch_few<B_ROWS, 2>(p, p.a_pitch % 16 == 0, s);
   }
-  return kind == ANY ? launch<Any, MODE, B_ROWS>(p, s) : kind == LARGE ? launch<Large, MODE, B_ROWS>(p, s) : launch<Small, MODE, B_ROWS>(p, s);
+  if (kind == ANY) return launch<Any, MODE, B_ROWS>(p, s);
+  if (whole_rows(p)) return kind == LARGE ? launch<Large, MODE, B_ROWS>(p, s) : launch<Small, MODE, B_ROWS>(p, s);
+  return kind == LARGE ? launch<LargeCut, MODE, B_ROWS>(p, s) : launch<SmallCut, MODE, B_ROWS>(p, s);
 }
 
 }  // namespace
@@ -629,7 +655,9 @@ int launch_grouped_int8(const GroupedArgs& p, hipStream_t s) { return run<GG_ROW
 #endif
 int GG_NAME(launch_grouped)(const GroupedArgs& p, hipStream_t s) { return run<GG_ROWS, false>(p, s); }
 int GG_NAME(launch_grouped_bwd)(const GroupedArgs* px, const GroupedArgs* pw, hipStream_t s) {
-  if (px && pw && px->S > 0 && choose<GG_ROWS, true>(*px) == LARGE && choose<GG_CONTRACT, false>(*pw) == LARGE) return launch_bwd<Large>(*px, *pw, s);
+  if (px && pw && px->S > 0 && choose<GG_ROWS, true>(*px) == LARGE && choose<GG_CONTRACT, false>(*pw) == LARGE && whole_rows(*px) &&
+      whole_rows(*pw))
+    return launch_bwd<Large>(*px, *pw, s);
   if (px && px->S > 0) {
     const int rc = run<GG_ROWS, true>(*px, s);
     if (rc != MOE_OK) return rc;

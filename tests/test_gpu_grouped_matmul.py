@@ -273,12 +273,12 @@ def test_refusals():
 EVERY_TILE = [300, 250, 512, 190, 0, 130, 97, 60, 1, 34, 400, 225]
 
 
-@pytest.mark.parametrize("N", [136, 1032, 8200, 131, 1027, 8195])
-@pytest.mark.parametrize("K", [72, 256, 520, 77, 515])
+@pytest.mark.parametrize("N", [136, 1032, 8200, 131, 1027, 8195, 1030, 8198])
+@pytest.mark.parametrize("K", [72, 256, 520, 77, 515, 58, 74, 518])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_every_kind_of_tile(K, N, dtype):
-    """The kernel goes by the number of tiles: few columns, some and many; by whether rows are aligned; one step and several, whole
-    and cut."""
+    """The kernel goes by the number of tiles: few columns, some and many; by whether rows are aligned (16 bytes, 4 or 2); one step and
+    several, whole and cut, also inside 16 bytes."""
     from nkilib.core.moe.grouped_matmul import grouped_matmul, grouped_matmul_bwd
 
     g = torch.Generator(device="cuda").manual_seed(K + N)
@@ -294,7 +294,8 @@ def test_every_kind_of_tile(K, N, dtype):
     assert_near(grouped_matmul_bwd(d, None, wt, od, need_weight=False)[0], want, mag, K, "d_x")
 
 
-@pytest.mark.parametrize("K,N", [(136, 264), (1032, 1032), (2056, 1992), (131, 515), (1027, 1029), (2050, 1999), (1032, 1029)])
+@pytest.mark.parametrize("K,N", [(136, 264), (1032, 1032), (2056, 1992), (131, 515), (1027, 1029), (2050, 1999), (1032, 1029), (1030, 1030),
+                                 (2054, 1998), (1030, 1032)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_every_kind_of_tile_of_the_weights_gradient(K, N, dtype):
     from nkilib.core.moe.grouped_matmul import grouped_matmul_bwd

@@ -160,7 +160,7 @@ def test_refusals():
 
 
 @pytest.mark.parametrize("N", [144, 1040, 8208, 131, 1027, 8195])
-@pytest.mark.parametrize("K", [64, 160, 1040, 77, 1030])
+@pytest.mark.parametrize("K", [64, 160, 1040, 77, 1030, 68, 124, 1028])
 @pytest.mark.parametrize("out", OUT)
 def test_every_kind_of_tile(K, N, out):
     """As for the 16-bit products: few columns, some and many, aligned or not, one step and several; and a dense product of as many rows."""
