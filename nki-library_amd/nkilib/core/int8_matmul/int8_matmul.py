@@ -35,7 +35,7 @@ def _scales(t, what, shape, dev):
     t = nv.require_device_tensor(t, what)
     if t.dtype != torch.float32:
         kernel_assert(False, f"{what} must be float32 but got {t.dtype}")
-    if tuple(t.shape) not in (tuple(shape), (*shape, 1)):
+    if t.shape != shape and t.shape != (*shape, 1):
         kernel_assert(False, f"{what} must be {list(shape)} but got {tuple(t.shape)}")
     if t.device != dev:
         kernel_assert(False, f"tensors must be on one device but are on {dev} and {t.device}")
@@ -55,7 +55,7 @@ def _run(x, x_scales, weight, weight_scales, bias, row_offsets, S, K, N, E, shap
         bias = nv.require_device_tensor(bias, "bias")
         if bias.dtype != out_dtype or bias.shape != (N,) or bias.device != dev:
             kernel_assert(False, f"bias must be {out_dtype} [{N}] on {dev} but got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
-    out = torch.empty(shape, dtype=out_dtype, device=dev)
+    out = x.new_empty(shape, dtype=out_dtype)
     if K == 0 and out.numel():  # (sums of nothing)
         return out.zero_() if bias is None else out.copy_(bias.expand(shape))
     if out.numel() == 0:
@@ -74,15 +74,13 @@ def int8_matmul(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, w
     float16 or float32; ``bias`` ``[N]`` of that type is added ahead of the rounding."""
     x = _codes(x, "x")
     w = _codes(weight, "weight", 2)
-    K, N = x.shape[-1], w.shape[0]
-    if w.shape[1] != K:
+    (N, Kw), lead, dev = w.shape, x.shape[:-1], x.device
+    K = x.shape[-1]
+    if Kw != K:
         kernel_assert(False, f"weight must be [N, {K}] but got {tuple(w.shape)}")
-    lead = tuple(x.shape[:-1])
-    S = 1
-    for n in lead:
-        S *= n
-    xs = _scales(x_scales, "x_scales", lead, x.device)
-    ws = _scales(weight_scales, "weight_scales", (N,), x.device)
+    S = lead.numel()
+    xs = _scales(x_scales, "x_scales", lead, dev)
+    ws = _scales(weight_scales, "weight_scales", (N,), dev)
     return _run(x, xs, w, ws, bias, None, S, K, N, 1, (*lead, N), out_dtype, "int8_matmul")
 
 
