@@ -2,9 +2,9 @@
 //
 // A workgroup walks over tiles of BM x BN of the result.  A step takes 128 bytes along the terms from both operands: 64 terms of 16
 // bits or 128 of 8, two MFMAs deep.  Either operand lies in memory along its terms ("rows": a piece of 16 bytes is a lane's
-// operand as it is) or across them ("columns": a piece is 8 neighbouring columns of one term), and stays so in LDS, where the transposing read
-// (ds_read_b64_tr_b16) hands a lane the terms of its column.  So weights [E, K, N] are multiplied as they are, and their gradient, whose
-// terms are rows, takes both operands across.
+// operand as it is) or across them ("columns": a piece is 8 neighbouring columns of one term), and stays so in LDS, where the
+// transposing read (ds_read_b64_tr_b16) hands a lane the terms of its column.  So weights [E, K, N] are multiplied as they are, and
+// their gradient, whose terms are rows, takes both operands across.
 //   rows:    LDS row of 128 bytes per row; piece j of row r in place j ^ (r & 7)
 //   columns: LDS row of BN columns per term; piece j of term k in place j ^ f(k), f(k) = 2 (k & 3) + 8 ((k >> 3) & 1): the 16 lanes of
 //            a transposing read fetch 32 bytes from each of 4 terms, two such groups at a time terms 8 apart, all in other banks.
@@ -37,8 +37,10 @@ typedef __attribute__((address_space(3))) uint8_t lds_byte;
 using acc_t = std::conditional_t<TYPE == GG_INT8, v4i, v4f>;
 
 __device__ __forceinline__ acc_t mfma(const v4i& w, const v4i& x, const acc_t& c) {
-  if constexpr (TYPE == GG_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), c, 0, 0, 0);
-  else if constexpr (TYPE == GG_FP16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, x), c, 0, 0, 0);
+  if constexpr (TYPE == GG_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), c, 0, 0, 0);
+  else if constexpr (TYPE == GG_FP16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, x), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0);
 }
 
@@ -60,7 +62,8 @@ constexpr uint32_t NOWHERE = 0x80000000u;  // an offset outside of every buffer,
 // 16 bytes per lane to lds + 16 * lane.  (The wait states: a scalar operand may have been written by a vector instruction just before,
 // which the compiler does not see here.  It keeps nothing in M0 between instructions of its own.)
 __device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t off, const v4i& buf) {
-  asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(off), "s"(buf) : "memory", "m0");
+  asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               : : "s"(lds), "v"(off), "s"(buf) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -119,7 +122,8 @@ struct Feed {
     if (ROWS_ ? rows_left >= BR && terms_left >= 128 : terms_left >= STEP && cols_left >= BR * ES) {  // (nothing ends inside)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const bytes16 d = *(const bytes16*)(p + (ROWS_ ? (int64_t)step * 128 : (int64_t)step * STEP * pitch) + (int64_t)i * RPT * pitch + (int)off);
+        const uint8_t* src = p + (ROWS_ ? (int64_t)step * 128 : (int64_t)step * STEP * pitch) + (int64_t)i * RPT * pitch;
+        const bytes16 d = *(const bytes16*)(src + (int)off);
         held[i] = words4{d[0], d[1], d[2], d[3]};
       }
       return;
@@ -343,8 +347,9 @@ __device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const
     else if (q.steps > 0) fetch(q, terms_of(q), 0);
   };
 
-  // A tile's first two steps (without DMA: the first) are requested ahead of the results of the tile before, whose stores then drain under its first steps:
-  // at least STORES of them stand behind the loads in the order in which these are waited for (stored), or nothing is counted on.
+  // A tile's first two steps (without DMA: the first) are requested ahead of the results of the tile before, whose stores then drain
+  // under its first steps: at least STORES of them stand behind the loads in the order in which these are waited for (stored), or nothing
+  // is counted on.
   constexpr int STORES = 2 * C::MT;
   bool stored = false;
   if (t >= total) return t - total;
@@ -529,7 +534,9 @@ __device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const
 // in one L2 and all XCDs work at the same group.  (A run for all rounds gave one of 8 experts to each XCD: the gradient of their
 // weights took 227 us for 8192 rows of 4096 x 2048, popular and unpopular, instead of 164.)
 __device__ __forceinline__ int64_t first_tile() { return (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3); }
-#define GG_KERNEL __global__ __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::PER_CU * C::THREADS / 256, C::PER_CU * C::THREADS / 256)))
+#define GG_KERNEL                                          \
+  __global__ __launch_bounds__(C::THREADS) __attribute__(( \
+      amdgpu_waves_per_eu(C::PER_CU * C::THREADS / 256, C::PER_CU * C::THREADS / 256)))
 
 template <class C, int MODE, bool B_ROWS>
 GG_KERNEL void grouped_kernel(const GroupedArgs p) {

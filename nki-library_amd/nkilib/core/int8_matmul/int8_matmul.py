@@ -57,7 +57,7 @@ def _run(x, x_scales, weight, weight_scales, bias, row_offsets, S, K, N, E, shap
             kernel_assert(False, f"bias must be {out_dtype} [{N}] on {dev} but got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
     out = x.new_empty(shape, dtype=out_dtype)
     if K == 0 and out.numel():  # (sums of nothing)
-        return out.zero_() if bias is None else out.copy_(bias.expand(shape))
+        return out.zero_() if bias is None else out.copy_(bias.detach().expand(shape))
     if out.numel() == 0:
         return out
     with nv.on_device(dev):

@@ -157,7 +157,8 @@ def test_views_addresses_and_strides(K, N):
     o = offsets_of([40, 0, 31])
     od = torch.from_numpy(o).cuda()
     for shift in (1, 3, 8):
-        x, w, d = r(71 * K + 8)[shift:][: 71 * K].view(71, K), r(3 * K * N + 8)[shift:][: 3 * K * N].view(3, K, N), r(71 * N + 8)[shift:][: 71 * N].view(71, N)
+        x, w, d = r(71 * K + 8)[shift:][: 71 * K].view(71, K), r(3 * K * N + 8)[shift:][: 3 * K * N].view(3, K, N), \
+            r(71 * N + 8)[shift:][: 71 * N].view(71, N)
         want, mag = products(x, w, o)
         assert_near(grouped_matmul(x, w, od), want, mag, K, f"shift {shift}")
         dx, dw = grouped_matmul_bwd(d, x, w, od)

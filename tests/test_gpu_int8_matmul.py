@@ -28,7 +28,8 @@ def _want(x, xs, w, ws):
     return (x.double() @ w.double().t().contiguous()) * xs.double()[:, None] * ws.double()
 
 
-@pytest.mark.parametrize("S,K,N", [(1, 64, 64), (1, 7168, 4096), (2, 1, 1), (3, 7, 5), (5, 16, 1), (16, 128, 136), (17, 129, 515), (33, 1030, 77),
+@pytest.mark.parametrize("S,K,N", [(1, 64, 64), (1, 7168, 4096), (2, 1, 1), (3, 7, 5), (5, 16, 1),
+                                   (16, 128, 136), (17, 129, 515), (33, 1030, 77),
                                    (64, 2048, 256), (100, 200, 264), (257, 384, 512), (300, 1040, 1030), (1000, 14336, 320), (7, 131071, 24)])
 @pytest.mark.parametrize("out", OUT)
 def test_dense(S, K, N, out):
@@ -63,7 +64,8 @@ def test_extreme_codes_are_exact():
         assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("counts,ahead,behind,K,N", [([1], 0, 0, 64, 64), ([0] * 60 + [1, 2, 0, 1], 0, 0, 2048, 768), ([3, 0, 20, 1], 2, 3, 77, 39),
+@pytest.mark.parametrize("counts,ahead,behind,K,N", [([1], 0, 0, 64, 64), ([0] * 60 + [1, 2, 0, 1], 0, 0, 2048, 768),
+                                                        ([3, 0, 20, 1], 2, 3, 77, 39),
                                                     ([40, 0, 129, 300, 16], 1, 9, 256, 520), ([512, 256, 255, 257], 0, 0, 512, 512),
                                                     ([0, 0], 3, 4, 128, 128), ([700, 2, 90], 0, 0, 1030, 515)])
 @pytest.mark.parametrize("out", OUT)
@@ -115,7 +117,9 @@ def test_leading_dimensions_views_and_addresses():
         assert torch.equal(int8_matmul(moved, xs, w, ws), want)
     assert torch.equal(int8_matmul(x.t().contiguous().t(), xs, w, ws), want)
     bias = torch.ones(72, device="cuda").bfloat16()
-    assert torch.equal(int8_matmul(x[:, :0], xs, w[:, :0], ws, bias), bias.expand(6, 72)) and not int8_matmul(x[:, :0], xs, w[:, :0], ws).any()
+    assert torch.equal(int8_matmul(x[:, :0], xs, w[:, :0], ws, bias), bias.expand(6, 72))
+    assert not int8_matmul(x[:, :0], xs, w[:, :0], ws, bias.clone().requires_grad_()).requires_grad
+    assert not int8_matmul(x[:, :0], xs, w[:, :0], ws).any()
 
 
 def test_in_a_graph():
@@ -147,7 +151,8 @@ def test_refusals():
     bad = [
         lambda: int8_matmul(x.float(), xs, w, ws), lambda: int8_matmul(x, xs, w.float(), ws), lambda: int8_matmul(x, xs.half(), w, ws),
         lambda: int8_matmul(x, xs, w, ws.double()), lambda: int8_matmul(x, f(5), w, ws), lambda: int8_matmul(x, xs, w, f(7)),
-        lambda: int8_matmul(x, xs, z(6, 9), ws), lambda: int8_matmul(x, xs, z(1, 6, 8), ws), lambda: int8_matmul(x, xs, w, ws, out_dtype=torch.float64),
+        lambda: int8_matmul(x, xs, z(6, 9), ws), lambda: int8_matmul(x, xs, z(1, 6, 8), ws),
+        lambda: int8_matmul(x, xs, w, ws, out_dtype=torch.float64),
         lambda: int8_matmul(x, xs, w, ws, bias=f(6)), lambda: int8_matmul(x, xs, w, ws, bias=f(5), out_dtype=torch.float32),
         lambda: int8_matmul(z(1, 2**17), f(1), z(2, 2**17), f(2)), lambda: grouped_int8_matmul(x, xs, z(2, 6, 8), f(2, 6), o.long()),
         lambda: grouped_int8_matmul(x, xs, z(2, 6, 8), f(2, 6), o[:2]), lambda: grouped_int8_matmul(x, xs, z(2, 6, 8), f(6, 2), o),

@@ -207,7 +207,8 @@ def test_launches_are_made_on_the_tensors_device(monkeypatch):
     o = torch.tensor([0, 3, 8], dtype=torch.int32, device="cuda")
     c, s = rmsnorm_quant_rows(x, None)
     wc, ws = rmsnorm_quant_rows(w.transpose(1, 2).contiguous(), None, do_norm=False)
-    calls = [lambda: grouped_matmul(x, w, o), lambda: grouped_matmul_bwd(grouped_matmul(x, w, o), x, w, o), lambda: expert_row_offsets(o, 1, 9),
+    calls = [lambda: grouped_matmul(x, w, o), lambda: grouped_matmul_bwd(grouped_matmul(x, w, o), x, w, o),
+             lambda: expert_row_offsets(o, 1, 9),
              lambda: int8_matmul(c, s, wc[0], ws[0]), lambda: grouped_int8_matmul(c, s, wc, ws, o), lambda: rmsnorm_quant_rows(x, None),
              lambda: rmsnorm_quant_rows_bwd(x, x, None), lambda: dequantize_rows(c, s)]
     for i, call in enumerate(calls):
