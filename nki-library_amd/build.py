@@ -36,8 +36,8 @@ FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 # The sources whose loads into LDS list M0 as clobbered (ld_lds_b128 in csrc/mx_tile.hpp, MXW_DMA in csrc/mx_wide.hpp,
-# the like in csrc/router_topk.hip and csrc/grouped_tile.hip) draw one inline-asm diagnostic per such load, thousands of times; every other translation
-# unit keeps the diagnostic on
+# the like in csrc/router_topk.hip and csrc/grouped_tile.hip) draw one inline-asm diagnostic per such load, thousands of times;
+# every other translation unit keeps the diagnostic on
 MX_FLAGS = ["-Wno-inline-asm"]
 M0_CLOBBER_SOURCES = ("bwmm_mx.hip", "router_topk.hip")
 NOISE = "is not a recognized feature for this target"
