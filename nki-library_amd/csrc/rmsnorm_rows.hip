@@ -11,6 +11,8 @@
 // time that the row's bytes take), in an order that is the row's (row_sum), and 1 / sqrt is rounded to fp32 once; every other operation
 // is one fp32 operation (no contraction), so that a code depends on its row alone, not on the launch.  A row whose y is not finite has
 // the scale NaN and codes 0.
+#include <type_traits>
+
 #include "rows.hpp"
 
 #pragma clang fp contract(off)
@@ -149,6 +151,20 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
   return t;
 }
 
+// 1 / sqrt(mean + eps), rounded once, is no normal float where a row's values are denormal (it passes the largest float) or near the
+// largest (it is denormal itself).  Then: the power of two that brings it back among the normal ones, by which it is divided and the
+// row's values are multiplied, which is exact for all that are of weight.  (fp16 does not reach either end.)  A branch of its own, which
+// hardly a row takes: with a product by 1 in the others the kernels of long rows lose their registers (16384 rows of 7168 bf16 255 us).
+__device__ __forceinline__ float far_factor(double inv, float& inv32) {
+  const float far = inv > 1.0 ? 0x1p64f : inv <= 1.0 ? 0x1p-64f : 1.f;
+  inv32 = (float)(inv / far);
+  return far;
+}
+template <int DT>
+__device__ __forceinline__ bool is_far(float inv) {
+  return DT != MOE_DT_FP16 && !__builtin_isnormal(inv);
+}
+
 struct NormArgs {
   const uint8_t* x;
   const uint8_t* residual;
@@ -201,11 +217,23 @@ __global__ __launch_bounds__(256) void norm_quant_kernel(const NormArgs a) {
         for (int i = 0; i < N; ++i) part[p] = __builtin_fma((double)v[p][i], (double)v[p][i], part[p]);
       }
       const double sum = row_sum<TPR, P>(part, red_sum);
-      const float inv = (float)(1.0 / sqrt(sum / H + a.eps));
+      const double inv64 = 1.0 / sqrt(sum / H + a.eps);
+      float inv = (float)inv64;
+      if (is_far<DT>(inv)) [[unlikely]] {
+        const float far = far_factor(inv64, inv);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[p][i] = v[p][i] * far;
+      }
+      // (The lane is taken anew: the addresses of gamma's elements would otherwise be worked out ahead of the first row and kept.  16384 rows
+      // of 7168 bf16: 256 registers and 136 us, or 120 and 92.)
+      int at = lane;
+      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         float g[N];
-        load_gamma<DT, WHOLE>(a.gamma, a.gamma_dtype, (p * TPR + lane) * N, H, g);
+        load_gamma<DT, WHOLE>(a.gamma, a.gamma_dtype, (p * TPR + at) * N, H, g);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[p][i] = v[p][i] * inv * g[i];
       }
@@ -324,22 +352,37 @@ __global__ __launch_bounds__(SUB * 256) void norm_bwd_kernel(const NormBwdArgs a
     sx = (rx[0] + rx[1]) + (rx[2] + rx[3]);
     sd = (rd[0] + rd[1]) + (rd[2] + rd[3]);
     const double inv64 = 1.0 / sqrt(sx / H + a.eps);
-    const float inv = (float)inv64, mean = (float)(sd * inv64 / H);  // mean of dn n
-    if (on) {
+    const float mean = (float)(sd * inv64 / H);  // mean of dn n
+    auto finish = [&](float inv, float far, auto use_far) {
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         float x[N], d[N], o[N];
         unpack<DT>(xs[p], x);
         unpack<DT>(ds[p], d);
-        if (a.d_residual) unpack<DT>(rs[p], o);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+          if (use_far) x[i] = x[i] * far;
           const float n = x[i] * inv;
           dg[p][i] += d[i] * n;
-          const float s = (d[i] * gm[p][i] - n * mean) * inv;
-          o[i] = a.d_residual ? s + o[i] : s;
+          o[i] = (d[i] * gm[p][i] - n * mean) * inv;
+          if (use_far) o[i] = o[i] * far;
+        }
+        if (a.d_residual) {
+          float r[N];
+          unpack<DT>(rs[p], r);
+#pragma unroll
+          for (int i = 0; i < N; ++i) o[i] = o[i] + r[i];
         }
         store_part<DT, WHOLE>(a.d_x + r * row_bytes, (p * 256 + tid) * N, H, pack<DT>(o));
+      }
+    };
+    if (on) {
+      float inv = (float)inv64;
+      if (is_far<DT>(inv)) [[unlikely]] {
+        const float far = far_factor(inv64, inv);
+        finish(inv, far, std::true_type{});
+      } else {
+        finish(inv, 1.f, std::false_type{});
       }
     }
   }
