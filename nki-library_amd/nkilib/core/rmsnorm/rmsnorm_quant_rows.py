@@ -45,7 +45,7 @@ def _gamma(gamma, H, dev):
     """The tensor and its type's code."""
     g = nv.require_device_tensor(gamma, "gamma")
     code = nv.dtype_code(g, "gamma")
-    if g.numel() != H or g.shape[-1] != H or g.device != dev:
+    if g.numel() != H or g.shape[-1:] != (H,) or g.device != dev:
         kernel_assert(False, f"gamma must hold {H} values on {dev} but got {tuple(g.shape)} on {g.device}")
     return g, code
 
