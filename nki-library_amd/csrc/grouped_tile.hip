@@ -157,8 +157,10 @@ struct Feed {
           }
         }
       }
-      // (One value of 128 bits from here on: as two of 64 that meet in a branch, the compiler has been seen to take half of their registers
-      // for free while they wait to be put.)
+      // (One value of 128 bits from here on.  Kept as 32-bit parts that meet behind the branches, as a struct of four is, AMD clang 22 (ROCm 7.2)
+      // takes two of a piece's four registers for free in the gradient of the weights while the piece waits to be put, and writes addresses
+      // in its place.  Seen in an emulation of the build's assembly, in which every load was waited for; with the compiler's instruction
+      // scheduler off the same source came out right, so the fault is behind its intermediate code.  The build looks for such a write.)
       words4 v = {(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
       asm volatile("" : "+v"(v));
       held[i] = v;
