@@ -1,4 +1,4 @@
-// Products of ragged groups of rows with a matrix per group (grouped_gemm.hip, int8_gemm.hip).
+// Products of ragged groups of rows with a matrix per group (grouped_gemm.hip, grouped_tile.hip, grouped_few.hpp).
 #pragma once
 
 #include "common.hpp"

@@ -14,8 +14,8 @@
 // barrier of a step stands between them: all have read the step's stage, which then takes the step after the next, and the next step's
 // has landed.  The loads go out one per row tile of the second half: all at once they hold up the waves' issue (8192^3 bf16 895 | 857 us).
 // What bounds it: 70 % of the cycles the matrix pipes work (2950 cycles for a step of 256 x 256, MFMAs alone 2048), the rest is the barrier
-// and what stands around it; after some milliseconds power leaves a clock of 1.5 GHz.  8192^3, us: bf16 weights across 806 (1.36 PFLOP/s),
-// along 793, their gradient 808, int8 500 (2.2 POP/s).
+// and what stands around it, and a tile's edges (see STORES); after some milliseconds power leaves a clock of 1.5 GHz.  8192^3, us:
+// bf16 weights across 806 (1.36 PFLOP/s), along 793, their gradient 808, int8 500 (2.2 POP/s).
 // The matrix is the MFMA's first operand, so that a lane holds four neighbouring columns of one row; rows go out through LDS in whole
 // 128-byte lines.
 #include <type_traits>
@@ -116,7 +116,8 @@ struct Feed {
     return q;
   }
   static __device__ __forceinline__ void load(const Step& q, int i) { load_to_lds(q.lds + i * THREADS * 16, q.o + i * q.leap, q.buf); }
-  // Through registers: rows r < rows_left are read, terms_left bytes (ROWS_) or terms from this step on, cols_left bytes of a row.
+  // Through registers: rows r < rows_left are read, terms_left bytes (ROWS_) or terms from this step on, cols_left bytes of a row.  Where
+  // rows, terms or columns end inside the tile (all steps of a group's last row tile) the pieces are waited for one or two at a time.
   __device__ __forceinline__ void fetch(const uint8_t* p, int pitch, int step, int rows_left, int terms_left, int cols_left) {
     const int c = place() * 16;
     if (ROWS_ ? rows_left >= BR && terms_left >= 128 : terms_left >= STEP && cols_left >= BR * ES) {  // (nothing ends inside)
@@ -159,8 +160,8 @@ struct Feed {
       }
       // (One value of 128 bits from here on.  Kept as 32-bit parts that meet behind the branches, as a struct of four is, AMD clang 22 (ROCm 7.2)
       // takes two of a piece's four registers for free in the gradient of the weights while the piece waits to be put, and writes addresses
-      // in its place.  Seen in an emulation of the build's assembly, in which every load was waited for; with the compiler's instruction
-      // scheduler off the same source came out right, so the fault is behind its intermediate code.  The build looks for such a write.)
+      // in its place.  Seen in an emulation of the compiled code, in which every load was waited for; with the compiler's instruction
+      // scheduler off the same source came out right, so the fault is behind its intermediate code.  build.py looks for such a write.)
       words4 v = {(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
       asm volatile("" : "+v"(v));
       held[i] = v;
@@ -349,9 +350,12 @@ __device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const
     else if (q.steps > 0) fetch(q, terms_of(q), 0);
   };
 
-  // A tile's first two steps (without DMA: the first) are requested ahead of the results of the tile before, whose stores then drain
+  // A tile's first two steps (without DMA: the first) are requested ahead of the results of the tile before, whose stores may then drain
   // under its first steps: at least STORES of them stand behind the loads in the order in which these are waited for (stored), or nothing
-  // is counted on.
+  // is counted on.  (In the tiles of 128 x 128 they do.  Those of 256 x 256 have 3 to 15 of their registers in scratch memory, offsets of the
+  // loads mostly: a reload waits for all that is under way, and some stand between these requests, ahead of the results and between the
+  // loads of the first step.  So there both steps have landed before the first result leaves, and the stores have drained by the
+  // tile's first loads.)
   constexpr int STORES = 2 * C::MT;
   bool stored = false;
   if (t >= total) return t - total;
@@ -442,7 +446,7 @@ __device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const
 
     // ---- results: 16 rows of a wave at a time, by way of its 2 KB of LDS
     // (The lane is taken anew: what follows from it would otherwise be worked out ahead of the first tile and kept, for want of
-    // registers, in memory, whose loads wait for all that is under way.)
+    // registers, in memory, whose loads wait for all that is under way.  Offsets of the loads still are, see above.)
     int lane = tid & 63;
     asm volatile("" : "+v"(lane));
     const int c = lane & 15, g = lane >> 4;
@@ -451,6 +455,8 @@ __device__ __forceinline__ int64_t tiles_of(const GroupedArgs& p, uint8_t* const
     for (int n4 = 0; n4 < C::NT; n4 += 4) {
       const int64_t col0 = q.n0 + (wn * C::NT + n4) * 16;  // of these 64 columns, in the matrix
       const int cols = q.cols - (wn * C::NT + n4) * 16;    // that there are
+      // (int8: what the scales and the bias bring waits for the stores ahead of them, a row tile's scale for those of the row tile before; with
+      // a bias each of its 16 columns is waited for by itself.)
       v4f ws[4], bs[4];
       if constexpr (TYPE == GG_INT8) {
 #pragma unroll
@@ -605,7 +611,8 @@ typedef Cfg<128, 128, 2, 2, false, false, 2> Any;
 //     (7168 x 4096 int8, 1 | 16 | 32 | 64 rows: 10.5 | 10.6 | 13.6 | 22.4 us; tiles of 128 x 128 33 | 32 | 32 | 35)
 //   few rows, weights across them: 282 | 358 for every round of the chip
 //     (64 rows of 128 bf16 experts of 2048 x 1536: 61 us, tiles of 128 x 128 75; 2048 rows 166 and 161)
-// Rows of a group are not known here: they are taken as spread over as many groups as there may be, half a tile of each filled up.
+// Rows of a group are not known here: they are taken as spread over as many groups as there may be, half a tile of each filled up.  Where
+// few of many groups have all the rows there are fewer tiles than that; what another kernel would then take has not been measured.
 struct Estimate {
   int64_t S, groups, cols;
   int64_t tiles(int bm, int bn) const {

@@ -10,7 +10,8 @@ multiplies the rows that ``permute_tokens`` put into the order of the experts th
 
 Rows ``[row_offsets[e], row_offsets[e + 1])`` are expert e's.  Offsets are read on the device and nothing waits for them: whatever they
 are, they are taken into ``[0, S]`` and as never falling; rows of no expert are zero in a result.  Everything is bfloat16 or
-float16; sums are taken in fp32 and rounded once.
+float16; sums are taken in fp32 and rounded once.  What is not contiguous is copied in every call, weights ``[E, N, K]`` handed over as
+their transposed view among it.
 
 Plain calls, outside of torch's autograd: what they return has no graph, also where an input requires a gradient.
 """
