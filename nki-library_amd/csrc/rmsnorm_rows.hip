@@ -118,7 +118,7 @@ __device__ __forceinline__ uint32_t max_of_wave(uint32_t v) {
 }
 // Sum over a row of what its threads have of its pieces, P each.  A row of up to 256 pieces may be a wave's (up to four pieces a thread) or
 // a workgroup's (one): wave w's threads then have what the wave's have as piece w.  Either adds the four numbers of a lane first and the
-// lanes then, so that the sum is the row's alone.  (A wave's sum of every piece by itself: 16384 rows of 2048 bf16 57 us instead of 54.)
+// lanes then, so that the sum is the row's alone.  (A wave's sum of every piece by itself cost 7 % with the residual, 16384 rows of 2048 bf16.)
 // One barrier here and in the maximum: `red` is a place of its own for every reduction between two others.
 template <int TPR, int P>
 __device__ __forceinline__ double row_sum(const double (&v)[P], double* red) {
@@ -154,7 +154,8 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* red) {
 // 1 / sqrt(mean + eps), rounded once, is no normal float where a row's values are denormal (it passes the largest float) or near the
 // largest (it is denormal itself).  Then: the power of two that brings it back among the normal ones, by which it is divided and the
 // row's values are multiplied, which is exact for all that are of weight.  (fp16 does not reach either end.)  A branch of its own, which
-// hardly a row takes: with a product by 1 in the others the kernels of long rows lose their registers (16384 rows of 7168 bf16 255 us).
+// hardly a row takes: with a product by 1 in the others 16384 rows of 7168 fp32 take 171 us instead of 137, the gradient of 65536 rows of
+// 1024 bf16 147 instead of 141.
 __device__ __forceinline__ float far_factor(double inv, float& inv32) {
   const float far = inv > 1.0 ? 0x1p64f : inv <= 1.0 ? 0x1p-64f : 1.f;
   inv32 = (float)(inv / far);
